@@ -34,6 +34,7 @@ extern "C" {
 #define W4A16_ERR_DEVICE        -4  /* device is not sm_100 or cannot be queried */
 #define W4A16_ERR_TIMEOUT       -5  /* a kernel's bounded wait expired (sticky device flag) */
 #define W4A16_ERR_WORKSPACE     -6  /* workspace missing, too small or misaligned */
+#define W4A16_ERR_INDEX         -8  /* an index read from device memory was out of range (sticky flag) */
 
 /* Input dtypes accepted by w4a16_quantize. */
 #define W4A16_DTYPE_F16  0
@@ -261,9 +262,11 @@ int w4a16_dequantize(const int32_t* qweight, const void* scales, const void* zer
 /*
  * Read and clear the device's sticky error flags for the current device
  * (bit 0: a bounded wait in a GEMM kernel ran out of its time budget and the
- * kernel abandoned its tile). Synchronises the given stream.
- * Returns W4A16_OK when no flag was set, W4A16_ERR_TIMEOUT when one was; in
- * that case it also zeroes this device's w4a16_gemm_noalloc scratch array (if
+ * kernel abandoned its tile; bit 1: a position, slot, page id or row that a kernel
+ * of the cache read from device memory was out of range, and was skipped or read as
+ * index 0). Synchronises the given stream.
+ * Returns W4A16_OK when no flag was set, W4A16_ERR_INDEX when bit 1 alone was,
+ * W4A16_ERR_TIMEOUT when bit 0 was; in that last case it also zeroes this device's w4a16_gemm_noalloc scratch array (if
  * it has been set up) on `stream` and synchronises again, since its callers
  * cannot clear it themselves. Results of the launches since the last check are
  * unspecified after a timeout. Caller-owned workspaces and peer buffers may
@@ -413,6 +416,123 @@ int w4a16_p2p_alloc(int64_t bytes, void** ptr_out, void* handle_out);
 int w4a16_p2p_open(const void* handle, void** ptr_out);
 int w4a16_p2p_close(void* ptr);
 int w4a16_p2p_free(void* ptr);
+
+/*
+ * ---------------------------------------------------------------------------
+ * Attention over a 4-bit paged key/value cache (no counterpart in the reference,
+ * which ends at the linear layers): what lies between a block's qkv projection and
+ * its output projection.
+ *
+ * A cached value is offset + scale * code, code in 0..15, with one fp16 (scale,
+ * offset) pair per token, kv head and group of group_size channels: offset =
+ * fp16(min), scale = fp16((max - offset) / 15) (1 when not > 0), code =
+ * clamp(rint((x - offset) / scale), 0, 15). Values beyond +-65504 are stored as that;
+ * a group with an infinity or NaN in it gets the offset NaN. Sixteen tokens of a head
+ * make a block: key codes [16, D/2] bytes (channel 2i in the low nibble of byte i),
+ * value codes, key pairs [16, D/group_size, 2] fp16, value pairs. A page is
+ * page_size / 16 blocks of each kv head. pool: [layers, pages, kv_heads, page bytes],
+ * 16-byte aligned.
+ */
+typedef struct {
+  void* pool;
+  int64_t layers, pages;
+  int32_t kv_heads;
+  int32_t head_dim;      /* 64 or 128 */
+  int32_t page_size;     /* tokens, a multiple of 16, at most 4096 */
+  int32_t group_size;    /* 64, or head_dim */
+} w4a16_kv4_cache;
+
+/* Which sequence holds which pages, in device memory: refs [pages] (how many rows hold
+ * a page; 0: free), block_table [rows, width] (page ids, -1: none), kv_lens [rows]. */
+typedef struct {
+  int32_t *refs, *block_table, *kv_lens;
+  int32_t pages, rows, width, page_size;
+} w4a16_kv4_tables;
+
+/* Bytes of a page of one kv head. */
+int w4a16_kv4_page_bytes(int head_dim, int page_size, int group_size, int64_t* bytes_out);
+
+/*
+ * Queries [T, heads, D] and keys [T, kv_heads, D] (fp16 or bf16, channels contiguous, any
+ * token and head strides, in elements): RMS norm of each head (x / sqrt(mean(x^2) + eps) *
+ * weight; a null weight skips it), then the rotation of the first `rot` channels (a multiple
+ * of 8): pairs (i, i + rot/2), or (2i, 2i+1) when interleaved, by the angle whose cosine and
+ * sine are cos_sin[position][i] and cos_sin[position][rot/2 + i] (fp32 [max_position, rot]).
+ * positions: [T] (axes 1), or [3, T] (axes 3): frequencies i < axis0_end turn by the first
+ * row's position, i < axis1_end by the second's, the others by the third's. fp32 arithmetic,
+ * one rounding. q_out, k_out: dense, 16-byte aligned. weight_dtype: dtype, or fp32.
+ */
+int w4a16_qk_norm_rope(const void* q, const void* k, int dtype, int64_t T, int heads, int kv_heads, int head_dim,
+                       int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                       const int64_t* positions, int axes, int axis0_end, int axis1_end, const float* cos_sin,
+                       int64_t max_position, int rot, int interleaved, const void* q_weight, const void* k_weight,
+                       int weight_dtype, float eps, void* q_out, void* k_out, void* stream);
+
+/*
+ * The same, with the keys (normed and rotated, not rounded before) and the values [T, kv_heads, D]
+ * quantised into `layer` of the cache instead: token t goes to slots[t] = page * page_size +
+ * offset in the page (negative: not cached). No slot may appear twice in one call.
+ */
+int w4a16_qk_norm_rope_append(const void* q, const void* k, const void* v, int dtype, int64_t T, int heads,
+                              int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                              int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                              const int64_t* positions, int axes, int axis0_end, int axis1_end, const float* cos_sin,
+                              int64_t max_position, int rot, int interleaved, const void* q_weight,
+                              const void* k_weight, int weight_dtype, float eps, void* q_out,
+                              const w4a16_kv4_cache* cache, int64_t layer, const int64_t* slots, void* stream);
+
+/* Cached tokens back in 16 bits: out [2, n, kv_heads, D] (fp16 or bf16; keys, then values) of the
+ * tokens in slots [n]; a negative slot gives zeros. */
+int w4a16_kv4_gather(const w4a16_kv4_cache* cache, int64_t layer, const int64_t* slots, int64_t n, void* out, int dtype,
+                     void* stream);
+
+/*
+ * Attention of new tokens over the cache: q [T, heads, D] (fp16 or bf16, 16-byte aligned, strides
+ * multiples of 8 elements), o [T, heads, D] dense, lse [T, heads] fp32 or null (natural log-sum-exp
+ * of the scaled scores). Query head h reads kv head h / (heads / kv_heads). Sequence b has kv_lens[b]
+ * cached tokens, the new ones (already appended) among them, in the pages block_table[b, :] (entries
+ * beyond its length are not read); its queries are q[cu_q[b] : cu_q[b + 1]], or T / seqs each when
+ * cu_q is null, the last of which stands at position kv_lens[b] - 1. A query sees the tokens up to its
+ * own position, or the last `window` of those when window > 0; one that sees none (a length of 0)
+ * gives zeros and lse = -inf. max_q: at least the longest sequence's queries (ignored when cu_q is
+ * null). workspace: w4a16_kv4_attention_workspace_size bytes, 256-byte aligned, ZEROED before its
+ * first use and left ready for the next call on the same stream; calls that may run at the same time
+ * need one each.
+ */
+int w4a16_kv4_attention(const void* q, int dtype, int64_t T, int heads, int64_t q_token_stride, int64_t q_head_stride,
+                        const w4a16_kv4_cache* cache, int64_t layer, const int32_t* block_table, int64_t table_width,
+                        const int32_t* kv_lens, const int32_t* cu_q, int64_t seqs, int64_t max_q, float scale,
+                        int window, void* o, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+int w4a16_kv4_attention_workspace_size(const w4a16_kv4_cache* cache, int64_t T, int heads, int64_t seqs, int64_t max_q,
+                                       int64_t* bytes_out);
+
+/* Page src[i] copied to page dst[i] in every layer (pairs with a negative entry are skipped). A page
+ * that is some pair's dst must be no other pair's src or dst. */
+int w4a16_kv4_copy_pages(const w4a16_kv4_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+
+/* Row rows[i] gets free pages (the lowest ids, in the order of the requests) up to lens[i] tokens, and
+ * kv_lens[rows[i]] = lens[i]. ok[i] = 1; 0, with the row unchanged, where the free pages do not reach
+ * that far down the list, the table is too narrow or lens[i] is less than the row holds. No row twice.
+ * scratch: n + 1 ints. */
+int w4a16_kv4_reserve(const w4a16_kv4_tables* tables, const int32_t* rows, const int32_t* lens, int64_t n, int32_t* ok,
+                      int32_t* scratch, void* stream);
+
+/* Child row children[i] becomes a copy of sequence parents[i]: full pages are shared (refs + 1), a partly
+ * filled last page is copied, in every layer, into the lowest free page. ok[i] = 0 (and an empty child)
+ * where no page is free. Children hold no pages before, appear once, and are no parents. Writes the
+ * tables `out` (which may be `in`). scratch: 2 n ints. */
+int w4a16_kv4_fork(const w4a16_kv4_cache* cache, const w4a16_kv4_tables* in, const w4a16_kv4_tables* out,
+                   const int32_t* parents, const int32_t* children, int64_t n, int32_t* ok, int32_t* scratch,
+                   void* stream);
+
+/* The rows give their pages back (refs - 1) and are empty. Writes `out` (which may be `in`). */
+int w4a16_kv4_release(const w4a16_kv4_tables* in, const w4a16_kv4_tables* out, const int32_t* rows, int64_t n,
+                      void* stream);
+
+/* With c pages in use, the i-th page in use with an id >= c moves to the i-th free page with an id < c, in
+ * every layer, and refs and block_table follow. Writes `out` (which may be `in`). scratch: 2 * pages + 1 ints. */
+int w4a16_kv4_compact(const w4a16_kv4_cache* cache, const w4a16_kv4_tables* in, const w4a16_kv4_tables* out,
+                      int32_t* scratch, void* stream);
 
 #ifdef __cplusplus
 }

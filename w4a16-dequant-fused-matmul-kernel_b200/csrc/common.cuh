@@ -17,8 +17,11 @@ namespace w4a16 {
 // Sticky device error word (one per device, lives in this library's module;
 // the library is one translation unit, so this is its only definition).
 // Bit 0: a bounded pipeline wait expired and a CTA abandoned its tile.
+// Bit 1: a position, slot, page or row read from device memory was out of range (the
+//        access was skipped or redirected to index 0).
 // ---------------------------------------------------------------------------
 constexpr uint32_t kErrWaitTimeout = 1u;
+constexpr uint32_t kErrIndex = 2u;
 __device__ uint32_t g_device_error = 0;
 
 // Default time budget of one bounded wait, in nanoseconds of %globaltimer. Every

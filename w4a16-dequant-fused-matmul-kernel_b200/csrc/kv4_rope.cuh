@@ -1,0 +1,314 @@
+// kv4_rope.cuh -- queries and keys on their way to attention, in one pass over them: RMS norm
+// of each head, rotary position embedding (one position per token, or time / height / width
+// axes), and, for the form with a cache, the 4-bit quantisation of keys and values into their
+// slots. And its inverse, reading cached tokens back.
+//
+//   y = x * (1 / sqrt(mean(x^2) + eps)) * w           (per head; skipped without w)
+//   (a, b) -> (a cos - b sin, b cos + a sin)          (pairs (i, i + rot / 2), or (2i, 2i + 1))
+//   offset = fp16(min), scale = fp16((max - offset) / 15) (1 when not > 0),
+//   code = clamp(rint((x - offset) * (1 / scale)), 0, 15)        (per group of G channels)
+//
+// All arithmetic is fp32 with one rounding of the result; products are rounded one by one (no
+// contraction into FMAs) so that a key's code does not depend on how the compiler fuses them.
+// A group that holds an infinity or NaN gets the offset NaN: what reads it sees NaN instead of
+// a value made up.
+//
+// Memory-bound. D / 8 lanes share a head, each with two quads of channels chosen so that a pair
+// of the rotation lies in one lane: in the half-split form lane l holds channels 4l .. and
+// rot / 2 + 4l ..; without exchange between lanes the rotation costs no shuffles, and every
+// 8-byte access of the group still covers whole 32-byte sectors. A group handles UN heads of one
+// token, so that their loads are in flight together and share the angles.
+#pragma once
+
+#include "kv4_common.cuh"
+
+namespace w4a16 {
+namespace kv4 {
+
+constexpr int ROPE_THREADS = 256;
+constexpr int UN = 4;             // heads of a token per group of lanes
+
+struct RopeParams {
+  const void *q, *k, *v;          // [T, heads, D] each, channels contiguous
+  long long q_st, q_sh, k_st, k_sh, v_st, v_sh;   // token and head strides, in elements
+  void *q_out, *k_out;            // [T, heads, D] dense
+  long long T;
+  int heads, kv_heads;
+  int chunks;                     // groups per token
+  const long long* positions;     // [axes, T]
+  int axes, end0, end1;           // frequencies < end0 turn by axis 0, < end1 by axis 1, else axis 2
+  const float* cos_sin;           // [max_pos, rot]: cosines, then sines
+  long long max_pos;
+  int rot;                        // rotated channels (the first of each head), a multiple of 8
+  int interleaved;
+  const void *qw, *kw;            // [D] or null: no norm
+  int w_f32;                      // weights fp32, else of the inputs' type
+  float eps;
+  int vec;                        // every quad of q, k, v is 8-byte aligned
+  const long long* slots;         // APPEND: [T], page * page_size + offset; < 0: not cached
+  CacheView cache;
+  int groups;                     // D / G: 1 or 2
+};
+
+template <typename T>
+__device__ __forceinline__ void load_quad(const T* src, int vec, float* x) {
+  T v[4];
+  if (vec) {
+    *reinterpret_cast<uint2*>(v) = __ldg(reinterpret_cast<const uint2*>(src));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = src[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(v[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_quad(T* dst, const float* x) {
+  uint2 v;
+  v.x = pack2<T>(x[0], x[1]);
+  v.y = pack2<T>(x[2], x[3]);
+  *reinterpret_cast<uint2*>(dst) = v;
+}
+
+__device__ __forceinline__ void rotate_pair(float& a, float& b, float cs, float sn) {
+  const float x = a, y = b;
+  a = __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn));
+  b = __fadd_rn(__fmul_rn(y, cs), __fmul_rn(x, sn));
+}
+
+// A lane's quads (channels e0 .. e0 + 3 and e1 .. e1 + 3) of one head quantised into its token's
+// row; every lane of the warp calls it (`store` says which have something to write).
+template <int D>
+__device__ __forceinline__ void quantise_row(const float (&x)[8], int e0, int e1, int groups, bool store,
+                                             uint8_t* codes, uint32_t* pairs) {
+  constexpr int L = D / 8;
+  const int g0 = groups == 1 ? 0 : e0 / (D / 2), g1 = groups == 1 ? 0 : e1 / (D / 2);
+  float inv[2], off[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) off[q] = inv[q] = 0.0f;
+  for (int g = 0; g < groups; ++g) {
+    float lo = INFINITY, hi = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if ((i < 4 ? g0 : g1) != g) continue;
+      bad |= !(fabsf(x[i]) < INFINITY);
+      const float c = fminf(fmaxf(x[i], -kMaxF16), kMaxF16);
+      lo = fminf(lo, c);
+      hi = fmaxf(hi, c);
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      bad |= __shfl_xor_sync(0xffffffffu, bad ? 1 : 0, o) != 0;
+    }
+    const __half ho = bad ? __ushort_as_half(0x7fffu) : __float2half_rn(lo);
+    const float fo = __half2float(ho);
+    __half hs = __float2half_rn(__fdiv_rn(__fsub_rn(hi, fo), 15.0f));
+    if (!(__half2float(hs) > 0.0f)) hs = __float2half_rn(1.0f);
+    const float fi = __frcp_rn(__half2float(hs));
+    if (g0 == g) { off[0] = fo; inv[0] = fi; }
+    if (g1 == g) { off[1] = fo; inv[1] = fi; }
+    if (store && threadIdx.x % L == 0)
+      pairs[g] = static_cast<uint32_t>(__half_as_ushort(hs)) | (static_cast<uint32_t>(__half_as_ushort(ho)) << 16);
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float c = fminf(fmaxf(x[4 * q + i], -kMaxF16), kMaxF16);
+      const float r = rintf(__fmul_rn(__fsub_rn(c, off[q]), inv[q]));
+      w |= static_cast<uint32_t>(fminf(fmaxf(r, 0.0f), 15.0f)) << (4 * i);   // NaN: code 0
+    }
+    if (store) *reinterpret_cast<uint16_t*>(codes + (q ? e1 : e0) / 2) = static_cast<uint16_t>(w);
+  }
+}
+
+template <typename T, int D, bool APPEND>
+__global__ void __launch_bounds__(ROPE_THREADS) qk_norm_rope_kernel(const RopeParams p) {
+  constexpr int L = D / 8;
+  const int l = threadIdx.x % L;
+  long long g = (static_cast<long long>(blockIdx.x) * ROPE_THREADS + threadIdx.x) / L;
+  const bool live = g < p.T * p.chunks;
+  if (!live) g = 0;   // stays for the warp's shuffles, stores nothing
+  const long long t = g / p.chunks;
+  const int first = static_cast<int>(g % p.chunks) * UN;
+  const int items = p.heads + (APPEND ? 2 : 1) * p.kv_heads;
+
+  const bool turns = l < p.rot / 8;
+  const int e0 = turns && !p.interleaved ? 4 * l : 8 * l;
+  const int e1 = turns && !p.interleaved ? p.rot / 2 + 4 * l : 8 * l + 4;
+
+  float x[UN][8];
+#pragma unroll
+  for (int u = 0; u < UN; ++u) {
+    const int h = first + u;
+    const T* src = nullptr;
+    if (h < p.heads)
+      src = static_cast<const T*>(p.q) + t * p.q_st + h * p.q_sh;
+    else if (h < p.heads + p.kv_heads)
+      src = static_cast<const T*>(p.k) + t * p.k_st + (h - p.heads) * p.k_sh;
+    else if (APPEND && h < items)
+      src = static_cast<const T*>(p.v) + t * p.v_st + (h - p.heads - p.kv_heads) * p.v_sh;
+    if (src != nullptr) {
+      load_quad<T>(src + e0, p.vec, x[u]);
+      load_quad<T>(src + e1, p.vec, x[u] + 4);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[u][i] = 0.0f;
+    }
+  }
+
+  float cs[4], sn[4];
+  if (turns) {
+    const int f = 4 * l;
+    long long pos = p.positions[t];
+    if (pos < 0 || pos >= p.max_pos) {
+      flag_error(kErrIndex);
+      pos = 0;
+    }
+    if (p.axes == 1) {
+      const float* row = p.cos_sin + pos * p.rot;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        cs[i] = __ldg(row + f + i);
+        sn[i] = __ldg(row + p.rot / 2 + f + i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        long long a = p.positions[(f + i < p.end0 ? 0 : f + i < p.end1 ? 1 : 2) * p.T + t];
+        if (a < 0 || a >= p.max_pos) {
+          flag_error(kErrIndex);
+          a = 0;
+        }
+        cs[i] = __ldg(p.cos_sin + a * p.rot + f + i);
+        sn[i] = __ldg(p.cos_sin + a * p.rot + p.rot / 2 + f + i);
+      }
+    }
+  }
+
+  long long page = 0;
+  int in_page = 0;
+  bool cached = false;
+  if (APPEND) {
+    const long long slot = p.slots[t];
+    cached = live && slot >= 0;
+    if (cached && slot >= p.cache.pages * p.cache.page_size) {
+      flag_error(kErrIndex);
+      cached = false;
+    }
+    if (cached) {
+      page = slot / p.cache.page_size;
+      in_page = static_cast<int>(slot - page * p.cache.page_size);
+    }
+  }
+
+#pragma unroll
+  for (int u = 0; u < UN; ++u) {
+    const int h = first + u;
+    const bool is_q = h < p.heads, is_k = !is_q && h < p.heads + p.kv_heads;
+    const void* w = is_q ? p.qw : is_k ? p.kw : nullptr;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = fmaf(x[u][i], x[u][i], sum);
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (w != nullptr) {
+      const float r = __frcp_rn(__fsqrt_rn(__fadd_rn(sum / D, p.eps)));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int e = (i < 4 ? e0 : e1 - 4) + i;
+        const float wv = p.w_f32 ? static_cast<const float*>(w)[e] : to_f32<T>(static_cast<const T*>(w)[e]);
+        x[u][i] = __fmul_rn(__fmul_rn(x[u][i], r), wv);
+      }
+    }
+    if (turns && (is_q || is_k)) {
+      if (p.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rotate_pair(x[u][2 * i], x[u][2 * i + 1], cs[i], sn[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rotate_pair(x[u][i], x[u][i + 4], cs[i], sn[i]);
+      }
+    }
+    if (is_q || (!APPEND && is_k)) {
+      if (live) {
+        T* dst = is_q ? static_cast<T*>(p.q_out) + (t * p.heads + h) * D
+                      : static_cast<T*>(p.k_out) + (t * p.kv_heads + h - p.heads) * D;
+        store_quad<T>(dst + e0, x[u]);
+        store_quad<T>(dst + e1, x[u] + 4);
+      }
+    }
+    if constexpr (APPEND) {
+      // the lanes of a warp may hold different heads: all of them take part where any has a
+      // key or value head
+      if (__any_sync(0xffffffffu, !is_q && h < items)) {
+        const bool store = cached && !is_q && h < items;
+        const int head = is_k ? h - p.heads : h - p.heads - p.kv_heads;
+        uint8_t* blk = store ? block_ptr(p.cache, page, head, in_page / BLK) : nullptr;
+        const int tok = in_page % BLK;
+        uint8_t* codes = store ? blk + (is_k ? 0 : value_codes_at(D)) + tok * (D / 2) : nullptr;
+        uint32_t* pairs = store ? reinterpret_cast<uint32_t*>(blk + (is_k ? key_pairs_at(D) : value_pairs_at(D, p.groups))) +
+                                      tok * p.groups
+                                : nullptr;
+        quantise_row<D>(x[u], e0, e1, p.groups, store, codes, pairs);
+      }
+    }
+  }
+}
+
+// Cached tokens as T: out [2][n][kv heads][D], keys then values; a negative slot gives zeros.
+// D / 8 lanes per token and head, one word of eight channels each.
+struct GatherParams {
+  const long long* slots;
+  long long n;
+  void* out;
+  CacheView cache;
+  int groups;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_gather_kernel(const GatherParams p) {
+  constexpr int L = D / 8;
+  const long long g = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / L;
+  const int l = threadIdx.x % L;
+  if (g >= p.n * p.cache.kv_heads) return;
+  const long long t = g / p.cache.kv_heads;
+  const int head = static_cast<int>(g - t * p.cache.kv_heads);
+  long long slot = p.slots[t];
+  if (slot >= p.cache.pages * p.cache.page_size) {
+    flag_error(kErrIndex);
+    slot = -1;
+  }
+  uint32_t word[2] = {0, 0}, pair[2] = {0, 0};
+  if (slot >= 0) {
+    const long long page = slot / p.cache.page_size;
+    const int in_page = static_cast<int>(slot - page * p.cache.page_size);
+    const uint8_t* blk = block_ptr(p.cache, page, head, in_page / BLK);
+    const int tok = in_page % BLK;
+    const int grp = l * 8 / (D / p.groups);
+    word[0] = *reinterpret_cast<const uint32_t*>(blk + tok * (D / 2) + 4 * l);
+    word[1] = *reinterpret_cast<const uint32_t*>(blk + value_codes_at(D) + tok * (D / 2) + 4 * l);
+    pair[0] = *reinterpret_cast<const uint32_t*>(blk + key_pairs_at(D) + (tok * p.groups + grp) * 4);
+    pair[1] = *reinterpret_cast<const uint32_t*>(blk + value_pairs_at(D, p.groups) + (tok * p.groups + grp) * 4);
+  }
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const float2 so = __half22float2(*reinterpret_cast<const __half2*>(&pair[s]));
+    uint4 v;
+    uint32_t* vp = &v.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = static_cast<float>((word[s] >> (8 * i)) & 15u), b = static_cast<float>((word[s] >> (8 * i + 4)) & 15u);
+      vp[i] = pack2<T>(__fadd_rn(__fmul_rn(so.x, a), so.y), __fadd_rn(__fmul_rn(so.x, b), so.y));
+    }
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + ((s * p.n + t) * p.cache.kv_heads + head) * D + 8 * l) = v;
+  }
+}
+
+}  // namespace kv4
+}  // namespace w4a16

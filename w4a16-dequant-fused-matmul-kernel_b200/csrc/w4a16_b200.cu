@@ -719,6 +719,7 @@ const char* w4a16_strerror(int status) {
     case W4A16_ERR_SCRATCH_LIMIT:
       return "shape needs more scratch than w4a16_gemm_noalloc's static buffer holds "
              "(use w4a16_gemm with a workspace)";
+    case W4A16_ERR_INDEX: return "a position, slot, page or row in device memory was out of range (device error flag set)";
     default: return "unknown w4a16 status";
   }
 }
@@ -1052,13 +1053,14 @@ int w4a16_check_device_errors(void* stream, uint32_t* flags_out) {
     return W4A16_ERR_LAUNCH;
   }
   if (flags_out != nullptr) *flags_out = flags;
-  if (flags != 0) {
+  if ((flags & kErrWaitTimeout) != 0) {
     // A launch abandoned on a timeout may have left tagged piece words in the
     // allocation-free entry point's static scratch, whose callers cannot clear
     // it themselves: zero it here (a no-op if it was never set up).
     const int zst = noalloc_scratch_zero(s, true);
     if (zst != W4A16_OK) return zst;
   }
+  if (flags == kErrIndex) return W4A16_ERR_INDEX;
   return flags == 0 ? W4A16_OK : W4A16_ERR_TIMEOUT;
 }
 
@@ -1388,3 +1390,6 @@ extern "C" int w4a16_p2p_free(void* ptr) {
   }
   return W4A16_OK;
 }
+
+// The attention path around the GEMMs (4-bit paged cache).
+#include "kv4_abi.cuh"

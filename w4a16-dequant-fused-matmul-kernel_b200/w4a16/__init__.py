@@ -8,6 +8,11 @@ reference package (w4a16-kernel/src/w4a16/__init__.py:18-39):
     w4a16_matmul                                                    (gemm.py)
     W4A16Linear                                                     (linear.py)
 
+Beyond the reference, the attention path between those layers (kv_cache.py): a 4-bit paged
+key/value cache (KV4Cache, KV4Pages), query/key norm and rotation (qk_norm_rope,
+qk_norm_rope_append), attention over the cache (kv4_attention) and page management
+(kv4_reserve, kv4_copy_pages, kv4_fork, kv4_release, kv4_compact).
+
 Tensor-parallel layers (column / row sharding over torch.distributed + NCCL)
 live in ``w4a16.parallel``.
 
@@ -20,6 +25,8 @@ from __future__ import annotations
 from ._lib import W4A16Error, check_device_errors
 from .gemm import (interleave_gate_up, repack_qweight, stage_copy, swiglu, to_fp16, w4a16_matmul,
                    w4a16_matmul_bf16, w4a16_matmul_f32, w4a16_matmul_host, w4a16_matmul_swiglu)
+from .kv_cache import (KV4Cache, KV4Pages, kv4_attention, kv4_compact, kv4_copy_pages, kv4_fork, kv4_gather,
+                       kv4_release, kv4_reserve, qk_norm_rope, qk_norm_rope_append)
 from .linear import W4A16Linear
 from .quant import dequantize_weight, pack_int4, quantize_weight, unpack_int4
 from .reference import dequant_then_matmul, fp16_matmul, reference_w4a16
@@ -45,6 +52,17 @@ __all__ = [
     "w4a16_matmul_host",
     "W4A16Error",
     "check_device_errors",
+    "KV4Cache",
+    "KV4Pages",
+    "qk_norm_rope",
+    "qk_norm_rope_append",
+    "kv4_gather",
+    "kv4_attention",
+    "kv4_reserve",
+    "kv4_copy_pages",
+    "kv4_fork",
+    "kv4_release",
+    "kv4_compact",
 ]
 
 # The reference exported the fused GEMM only when its Triton backend imported

@@ -23,11 +23,30 @@ FLAG_BF16_OUT = 8
 PREFILL_AUTO, PREFILL_SMEM_B, PREFILL_TMEM_A = 0, 1, 2
 W4A16_ERR_TIMEOUT = -5
 W4A16_ERR_WORKSPACE = -6
+W4A16_ERR_INDEX = -8
 DTYPE_CODES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
 
-# Every symbol the header declares, with its ctypes signature.
 _c_i64 = ctypes.c_int64
+_c_int = ctypes.c_int
 _vp = ctypes.c_void_p
+
+
+class KV4CacheStruct(ctypes.Structure):
+    """``w4a16_kv4_cache`` of the header."""
+    _fields_ = [("pool", _vp), ("layers", _c_i64), ("pages", _c_i64), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("page_size", ctypes.c_int32), ("group_size", ctypes.c_int32)]
+
+
+class KV4TablesStruct(ctypes.Structure):
+    """``w4a16_kv4_tables`` of the header."""
+    _fields_ = [("refs", _vp), ("block_table", _vp), ("kv_lens", _vp), ("pages", ctypes.c_int32),
+                ("rows", ctypes.c_int32), ("width", ctypes.c_int32), ("page_size", ctypes.c_int32)]
+
+
+_cache_p = ctypes.POINTER(KV4CacheStruct)
+_tables_p = ctypes.POINTER(KV4TablesStruct)
+
+# Every symbol the header declares, with its ctypes signature.
 SIGNATURES = {
     "w4a16_version": ([], ctypes.c_int),
     "w4a16_strerror": ([ctypes.c_int], ctypes.c_char_p),
@@ -72,6 +91,21 @@ SIGNATURES = {
     "w4a16_p2p_open": ([_vp, ctypes.POINTER(_vp)], ctypes.c_int),
     "w4a16_p2p_close": ([_vp], ctypes.c_int),
     "w4a16_p2p_free": ([_vp], ctypes.c_int),
+    "w4a16_kv4_page_bytes": ([_c_int] * 3 + [ctypes.POINTER(_c_i64)], _c_int),
+    "w4a16_qk_norm_rope": ([_vp, _vp, _c_int, _c_i64] + [_c_int] * 3 + [_c_i64] * 4 + [_vp] + [_c_int] * 3 +
+                           [_vp, _c_i64, _c_int, _c_int, _vp, _vp, _c_int, ctypes.c_float, _vp, _vp, _vp], _c_int),
+    "w4a16_qk_norm_rope_append": ([_vp] * 3 + [_c_int, _c_i64, _c_int] + [_c_i64] * 6 + [_vp] + [_c_int] * 3 +
+                                  [_vp, _c_i64, _c_int, _c_int, _vp, _vp, _c_int, ctypes.c_float, _vp, _cache_p, _c_i64,
+                                   _vp, _vp], _c_int),
+    "w4a16_kv4_gather": ([_cache_p, _c_i64, _vp, _c_i64, _vp, _c_int, _vp], _c_int),
+    "w4a16_kv4_attention": ([_vp, _c_int, _c_i64, _c_int, _c_i64, _c_i64, _cache_p, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64,
+                             _c_i64, ctypes.c_float, _c_int, _vp, _vp, _vp, _c_i64, _vp], _c_int),
+    "w4a16_kv4_attention_workspace_size": ([_cache_p, _c_i64, _c_int, _c_i64, _c_i64, ctypes.POINTER(_c_i64)], _c_int),
+    "w4a16_kv4_copy_pages": ([_cache_p, _vp, _vp, _c_i64, _vp], _c_int),
+    "w4a16_kv4_reserve": ([_tables_p, _vp, _vp, _c_i64, _vp, _vp, _vp], _c_int),
+    "w4a16_kv4_fork": ([_cache_p, _tables_p, _tables_p, _vp, _vp, _c_i64, _vp, _vp, _vp], _c_int),
+    "w4a16_kv4_release": ([_tables_p, _tables_p, _vp, _c_i64, _vp], _c_int),
+    "w4a16_kv4_compact": ([_cache_p, _tables_p, _tables_p, _vp, _vp], _c_int),
 }
 
 _lock = threading.Lock()
@@ -140,8 +174,9 @@ def ptr(t: torch.Tensor | None) -> int | None:
 def check_device_errors(device: torch.device | int | None = None) -> int:
     """Read and clear the device's sticky kernel error flags (synchronises).
 
-    Raises :class:`W4A16Error` if a GEMM kernel's bounded wait expired since
-    the last check; returns 0 otherwise.
+    Raises :class:`W4A16Error` if a kernel's bounded wait expired since the last
+    check, or a cache kernel met a position, slot, page or row out of range; returns
+    0 otherwise.
     """
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(
         "cuda", device) if isinstance(device, int) else device
@@ -160,6 +195,7 @@ def check_device_errors(device: torch.device | int | None = None) -> int:
 # ---------------------------------------------------------------------------
 _ws_lock = threading.Lock()
 _ws_cache: dict[tuple[int, int], torch.Tensor] = {}
+_kv4_ws_cache: dict[tuple[int, int], torch.Tensor] = {}   # attention's, which it does not leave zero
 _ws_retired: list[torch.Tensor] = []
 
 
@@ -196,6 +232,21 @@ def gemm_workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tens
         return ws
 
 
+def kv4_workspace(nbytes: int, device_index: int, stream: int) -> torch.Tensor:
+    """The attention kernels' scratch buffer (zeroed when made) of >= nbytes for this stream."""
+    key = (device_index, stream)
+    ws = _kv4_ws_cache.get(key)
+    if ws is None or ws.numel() < nbytes:
+        with _ws_lock:
+            ws = _kv4_ws_cache.get(key)
+            if ws is None or ws.numel() < nbytes:
+                if ws is not None:
+                    _ws_retired.append(ws)
+                ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device_index)
+                _kv4_ws_cache[key] = ws
+    return ws
+
+
 _ws_for: dict[tuple[int, int, int, int, int, int], tuple[int | None, int]] = {}
 
 
@@ -226,7 +277,7 @@ def reset_workspaces() -> None:
     (after a kernel reported W4A16_ERR_TIMEOUT), on the stream each workspace serves;
     then synchronise those devices."""
     with _ws_lock:
-        items = list(_ws_cache.items())
+        items = list(_ws_cache.items()) + list(_kv4_ws_cache.items())
     devices = set()
     for (dev_index, stream), ws in items:
         with torch.cuda.device(dev_index):
