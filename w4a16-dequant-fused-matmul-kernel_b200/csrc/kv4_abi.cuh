@@ -2,7 +2,7 @@
 // preparation: argument checks and launches. Included once, by w4a16_b200.cu.
 #pragma once
 
-#include "kv4_attend.cuh"
+#include "kv4_decode.cuh"
 #include "kv4_pages.cuh"
 #include "kv4_rope.cuh"
 
@@ -37,6 +37,13 @@ int launched() {
   if (cudaGetLastError() != cudaSuccess) return W4A16_ERR_LAUNCH;
   return W4A16_OK;
 }
+
+// What routing and workspace go by: nothing that lies in device memory.
+struct AttendPlan {
+  long long seqs;
+  int kv_heads;
+  long long rows;          // most query rows of a sequence's kv head
+};
 
 struct RopeArgs {
   const void *q, *k, *v;
@@ -149,6 +156,96 @@ unsigned table_blocks(const w4a16_kv4_tables& t, int threads, const DeviceState&
   return static_cast<unsigned>(std::min<long long>((n + threads - 1) / threads, 4LL * dev.num_sms));
 }
 
+// Decode attention: query rows per tile, warps and blocks per tile of each shape. Eight rows (NT = 1)
+// leave room for 16 warps of 128 registers with two blocks per stage; sixteen rows need 8 warps of
+// twice the registers, which take four blocks per stage so that as many bytes are in flight.
+template <int D, int NG, int NT>
+struct DecodeConfig {
+  static constexpr int W = NT == 1 ? 16 : 8, TB = NT == 1 ? 2 : 4;
+  using Shape = DecodeShape<D, NG, NT, W, TB>;
+  static auto kernel() { return kv4_decode_kernel<D, NG, NT, W, TB>; }
+};
+
+template <typename F>
+int with_decode_config(const w4a16_kv4_cache& c, int nt, F f) {
+  if (c.head_dim == 64) return nt == 1 ? f(DecodeConfig<64, 1, 1>()) : f(DecodeConfig<64, 1, 2>());
+  if (c.group_size == 128) return nt == 1 ? f(DecodeConfig<128, 1, 1>()) : f(DecodeConfig<128, 1, 2>());
+  return nt == 1 ? f(DecodeConfig<128, 2, 1>()) : f(DecodeConfig<128, 2, 2>());
+}
+
+int decode_nt(const AttendPlan& p) { return p.rows <= 8 ? 1 : 2; }
+
+// Warps per team: as many as there are for each segment, a power of two.
+int decode_team_warps(const AttendPlan& p, int W, const DeviceState& dev) {
+  const int rows = 8 * decode_nt(p);
+  const long long segments = std::min<long long>(p.seqs, MAX_SEQS) * p.kv_heads * ((p.rows + rows - 1) / rows);
+  int tw = 1;
+  while (tw < W && 2 * tw * segments <= static_cast<long long>(dev.num_sms) * W) tw *= 2;
+  return tw;
+}
+
+// The workspace begins with the teams' counters, always at the same place: what one call leaves zero
+// the next one finds zero, whatever its shape.
+constexpr int kCounterBytes = 65536;
+
+long long decode_workspace(const w4a16_kv4_cache& c, const AttendPlan& p, const DeviceState& dev) {
+  long long parts = 0;
+  with_decode_config(c, decode_nt(p), [&](auto cfg) {
+    using C = decltype(cfg);
+    parts = static_cast<long long>(dev.num_sms) * (C::W / decode_team_warps(p, C::W, dev)) * 2 * C::Shape::STATE * 4;
+    return 0;
+  });
+  return kCounterBytes + parts;
+}
+
+int launch_decode(const w4a16_kv4_cache& c, const AttendParams& all, const AttendPlan& plan, int bf16, int row_limit,
+                  void* workspace, const DeviceState& dev, cudaStream_t s) {
+  for (int b0 = 0; b0 < all.seqs; b0 += MAX_SEQS) {
+    DecodeParams p = {};
+    p.a = all;
+    p.a.seqs = std::min(all.seqs - b0, MAX_SEQS);
+    p.a.table += static_cast<long long>(b0) * all.width;
+    p.a.lens += b0;
+    if (p.a.cu_q) {
+      p.a.cu_q += b0;
+    } else if (all.seqs > MAX_SEQS) {     // uniform queries: this launch's own
+      const long long each = all.T / all.seqs;
+      p.a.q = static_cast<const uint16_t*>(all.q) + b0 * each * all.q_st;
+      p.a.o = static_cast<uint16_t*>(all.o) + b0 * each * all.heads * c.head_dim;
+      if (all.lse) p.a.lse = all.lse + b0 * each * all.heads;
+      p.a.T = static_cast<int>(each * p.a.seqs);
+    }
+    p.bf16 = bf16;
+    p.row_limit = row_limit;
+    p.wait_ns = g_wait_budget_ns.load(std::memory_order_relaxed);
+    p.counters = static_cast<int*>(workspace);
+    p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
+    const int nt = decode_nt(plan);
+    const int st = with_decode_config(c, nt, [&](auto cfg) {
+      using C = decltype(cfg);
+      const int tw = decode_team_warps(plan, C::W, dev);
+      if (dev.num_sms * (C::W / tw) > kCounterBytes / 4) return W4A16_ERR_DEVICE;
+      p.team_warps = tw;
+      p.teams = dev.num_sms * (C::W / tw);
+      auto k = C::kernel();
+      static std::atomic<uint64_t> ready{0};   // devices whose shared memory limit is set
+      int d = 0;
+      if (cudaGetDevice(&d) != cudaSuccess) return W4A16_ERR_DEVICE;
+      if (!(ready.load(std::memory_order_acquire) >> d & 1)) {
+        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::Shape::SMEM_BYTES) != cudaSuccess) {
+          cudaGetLastError();
+          return W4A16_ERR_LAUNCH;
+        }
+        ready.fetch_or(1ull << d, std::memory_order_release);
+      }
+      k<<<dev.num_sms, C::W * 32, C::Shape::SMEM_BYTES, s>>>(p);
+      return launched();
+    });
+    if (st != W4A16_OK) return st;
+  }
+  return W4A16_OK;
+}
+
 void launch_copy(const w4a16_kv4_cache& c, const int* src, const int* dst, const int* count, int n, const DeviceState& dev,
                  cudaStream_t s) {
   const CacheView v = view_of(c, 0);
@@ -243,6 +340,9 @@ int w4a16_kv4_attention_workspace_size(const w4a16_kv4_cache* cache, int64_t T, 
   if (st != W4A16_OK) return st;
   if (T < 0 || T > 0x7fffffffLL || heads < 1 || heads % cache->kv_heads != 0 || seqs < 0 || max_q < 0)
     return W4A16_ERR_INVALID;
+  if (T == 0 || seqs == 0) return W4A16_OK;
+  const kv4::AttendPlan plan = {seqs, cache->kv_heads, std::min(max_q, T) * (heads / cache->kv_heads)};
+  *bytes_out = kv4::decode_workspace(*cache, plan, *dev);
   return W4A16_OK;
 }
 
@@ -270,21 +370,16 @@ int w4a16_kv4_attention(const void* q, int dtype, int64_t T, int heads, int64_t 
   p.table = block_table; p.width = static_cast<int>(table_width);
   p.lens = kv_lens; p.cu_q = cu_q;
   p.seqs = static_cast<int>(seqs); p.T = static_cast<int>(T);
+  p.max_q = static_cast<int>(std::min<int64_t>(max_q, T));
   p.heads = heads; p.share = heads / cache->kv_heads;
   p.scale = scale; p.window = window;
   p.groups = cache->head_dim / cache->group_size;
-  const long long rows = T * heads;
-  if ((rows + 3) / 4 > 0x7fffffffLL) return W4A16_ERR_INVALID;
-  const unsigned grid = static_cast<unsigned>((rows + 3) / 4);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == W4A16_DTYPE_F16) {
-    if (cache->head_dim == 128) kv4::kv4_attend_simple_kernel<__half, 128><<<grid, 128, 0, s>>>(p);
-    else kv4::kv4_attend_simple_kernel<__half, 64><<<grid, 128, 0, s>>>(p);
-  } else {
-    if (cache->head_dim == 128) kv4::kv4_attend_simple_kernel<__nv_bfloat16, 128><<<grid, 128, 0, s>>>(p);
-    else kv4::kv4_attend_simple_kernel<__nv_bfloat16, 64><<<grid, 128, 0, s>>>(p);
-  }
-  return kv4::launched();
+  const kv4::AttendPlan plan = {seqs, cache->kv_heads, (cu_q ? std::min(max_q, T) : T / seqs) * p.share};
+  const int64_t need = kv4::decode_workspace(*cache, plan, *dev);
+  if (workspace == nullptr || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+    return W4A16_ERR_WORKSPACE;
+  return kv4::launch_decode(*cache, p, plan, dtype == W4A16_DTYPE_BF16, 0x7fffffff, workspace, *dev,
+                            static_cast<cudaStream_t>(stream));
 }
 
 int w4a16_kv4_copy_pages(const w4a16_kv4_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream) {

@@ -1,0 +1,692 @@
+// kv4_decode.cuh -- attention over the 4-bit cache for few query rows per kv head (single new
+// tokens, drafted tokens, the heads that share a kv head): o = softmax(scale q k^T) v.
+//
+// Memory-bound by design: a token of a kv head is D + 8 D / G bytes, read once for all the query
+// rows (query token, head of the group) that share it. What a row costs beside is arithmetic on
+// codes, so codes are never turned into values:
+//   q . k = s_k (q . c) + b_k sum(q)          (per group of G channels; s, b the token's pair)
+//   sum_t p_t v_t = sum_t (p_t s_t) c_t + sum_t p_t b_t
+// A code masked out of its word, (w & 0x000f000f), is a pair of fp16 subnormals c * 2^-24, which
+// the tensor cores multiply exactly: no conversion, one AND per two codes. Nibbles at bits 4-7
+// give 16 c * 2^-24; the queries' fragments for them carry 1/16, and the sums of the values'
+// channels with an odd nibble are divided by 16 at the end.
+//
+// Queries are scaled to a largest magnitude in [1, 2) by a power of two (exact, and any bf16
+// query then fits fp16). p s is the one rounding to 16 bits (2^-11); what it loses, r, would meet
+// codes of 7.5 on average, so 7.5 r is added back in fp32 and only r (c - 7.5) stays: the error
+// of rounding p times a value centred on its group.
+//
+// Both products take the cache as the M side of mma.m16n8k16 (16 tokens, or 16 channels) and
+// eight query rows as its N side, so no row of the tensor core is wasted on padding queries when
+// eight heads share a kv head. S^T comes out with tokens along lanes; movmatrix turns it into the
+// B fragment of the second product.
+//
+// Work: a segment is a kv head of a sequence (and a tile of 8 NT of its rows), a tile TB blocks
+// of 16 tokens. All tiles form one list that N teams of warps split evenly, whatever the lengths;
+// a team that holds a part of a segment leaves (m, l, o) in the workspace and the last of the
+// segment's teams to arrive joins the parts in team order, so results do not depend on timing.
+// Each warp feeds itself: two stages of a tile, filled by bulk copies that its own lanes issue.
+#pragma once
+
+#include "kv4_attend.cuh"
+
+namespace w4a16 {
+namespace kv4 {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNoMax = -1e30f;           // running maximum before any token
+// The running maximum follows only when a score exceeds it by this much (log2): p <= 7.46, and
+// p * s stays finite in fp16 as no scale exceeds (65504 + 65504) / 15 = 8734.
+constexpr float kLazyMax = 2.9f;
+constexpr int MAX_SEQS = 2048;             // sequences per launch (their prefix sums lie in shared memory)
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Bulk copy of `bytes` (a multiple of 16) into shared memory, completing on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+struct DecodeParams {
+  AttendParams a;
+  int bf16;                // q and o bf16, else fp16
+  int row_limit;           // sequences with more rows than this are left to the other kernel
+  int team_warps;          // warps per team: 1, 2, 4, ... W
+  int teams;               // most teams (CTAs * W / team_warps)
+  int* counters;           // [teams] arrivals at a segment that several teams share, by the first of them; left zero
+  float* parts;            // [teams * 2] partial results
+  unsigned long long wait_ns;
+};
+
+template <int D, int NG, int NT, int W, int TB>
+struct DecodeShape {
+  static constexpr int SETS = D / 64;                    // sets of 8 words per token
+  static constexpr int BLOCK = block_bytes(D, NG);
+  static constexpr int STAGE = TB * BLOCK;
+  static constexpr int ACC = SETS * 16 * NT;             // accumulators per lane
+  static constexpr int STATE = (ACC + (4 + 2 * NG) * NT) * 32;   // floats of a warp's state
+  static constexpr int RING_BYTES = W * 2 * STAGE;
+  static constexpr int MERGE_BYTES = W / 2 * STATE * 4;
+  static constexpr int SMEM_BYTES = RING_BYTES + MERGE_BYTES + (MAX_SEQS + 1) * 8 + W * 2 * 8 + W * 8 + 64;
+  static_assert(STAGE % 16 == 0 && SMEM_BYTES <= 227 * 1024, "shared memory budget");
+};
+
+struct Segment {
+  long long start;         // first tile of the segment in the list
+  int n;                   // its tiles
+  int b, kh, rt;           // sequence, kv head, row tile
+  int first, count, len;   // the sequence's queries and cached tokens
+  int tile0;               // the sequence's first tile some query sees
+};
+
+template <int D, int NG, int NT, int W, int TB>
+__global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParams p) {
+  using SH = DecodeShape<D, NG, NT, W, TB>;
+  constexpr int ROWS = 8 * NT, TT = TB * BLK, SETS = SH::SETS;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* ring = smem;
+  float* merge = reinterpret_cast<float*>(smem + SH::RING_BYTES);
+  long long* prefix = reinterpret_cast<long long*>(smem + SH::RING_BYTES + SH::MERGE_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(prefix + MAX_SEQS + 1);
+  long long* scan = reinterpret_cast<long long*>(bars + 2 * W);
+  int* last_flag = reinterpret_cast<int*>(scan);         // one per team, after the prefix sums are done
+
+  const AttendParams& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = lane >> 2, q4 = lane & 3;
+
+  if (lane == 0) {
+    mbar_init(&bars[2 * warp], 1);
+    mbar_init(&bars[2 * warp + 1], 1);
+    mbar_fence_init();
+  }
+
+  // a sequence's tiles and how many segments have them
+  auto extent = [&](int b, Segment& s) {
+    sequence(a, b, s.first, s.count, s.len);
+    s.b = b;
+    const int rows = s.count * a.share;
+    s.tile0 = 0;
+    s.n = 0;
+    if (rows == 0 || rows > p.row_limit) return 0;
+    const int from = a.window ? max(0, s.len - s.count - a.window + 1) : 0;
+    s.tile0 = from / TT;
+    s.n = max(0, (s.len + TT - 1) / TT - s.tile0);
+    return a.cache.kv_heads * ((rows + ROWS - 1) / ROWS);
+  };
+
+  // prefix sums of the sequences' tiles
+  long long total = 0;
+  for (int base = 0; base < a.seqs; base += W * 32) {
+    const int b = base + threadIdx.x;
+    Segment s;
+    long long v = 0;
+    if (b < a.seqs) {
+      const long long h = extent(b, s);
+      v = h * s.n;
+    }
+    long long inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    __syncthreads();
+    if (lane == 31) scan[warp] = inc;
+    __syncthreads();
+    long long before = total;
+    for (int w = 0; w < W; ++w) {
+      const long long x = scan[w];
+      if (w < warp) before += x;
+      total += x;
+    }
+    if (b < a.seqs) prefix[b] = before + inc - v;
+  }
+  if (threadIdx.x == 0) prefix[a.seqs] = total;
+  __syncthreads();
+
+  const int TW = p.team_warps, team_in_cta = warp / TW, wt = warp % TW;
+  const int team = blockIdx.x * (W / TW) + team_in_cta;
+  const int barrier = 1 + team_in_cta;
+  auto team_sync = [&]() {
+    if (TW == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(TW * 32) : "memory");
+  };
+
+  // sequences without a tile: their queries see nothing
+  for (int b = team; b < a.seqs; b += p.teams) {
+    if (prefix[b + 1] != prefix[b]) continue;
+    Segment s;
+    if (extent(b, s) == 0) continue;
+    const long long rows = static_cast<long long>(s.count) * a.heads;
+    uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + static_cast<long long>(s.first) * a.heads * D);
+    for (long long i = wt * 32 + lane; i < rows * (D / 8); i += TW * 32) o[i] = make_uint4(0, 0, 0, 0);
+    if (a.lse)
+      for (long long i = wt * 32 + lane; i < rows; i += TW * 32)
+        a.lse[static_cast<long long>(s.first) * a.heads + i] = -INFINITY;
+  }
+
+  // the team's share of the list: no more teams than give each warp a tile
+  const long long N = min(static_cast<long long>(p.teams), (total + TW - 1) / TW);
+  if (team >= N) return;
+  const long long t0 = total * team / N, t1 = total * (team + 1) / N;
+
+  auto locate = [&](long long t) {
+    int lo = 0, hi = a.seqs - 1;   // last b with prefix[b] <= t: the one that holds t
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (prefix[mid] <= t) lo = mid; else hi = mid - 1;
+    }
+    Segment s;
+    extent(lo, s);
+    const int seg = static_cast<int>((t - prefix[lo]) / s.n);
+    s.kh = seg % a.cache.kv_heads;
+    s.rt = seg / a.cache.kv_heads;
+    s.start = prefix[lo] + static_cast<long long>(seg) * s.n;
+    return s;
+  };
+
+  // ------------------------------ this warp's copies ------------------------------
+  uint8_t* stages = ring + warp * 2 * SH::STAGE;
+  uint64_t* bar = &bars[2 * warp];
+  const bool whole_tiles = a.cache.page_blocks % TB == 0;   // a tile lies in one page
+  Segment ps;                 // segment of the tile to copy next, and that tile's page of this lane's block
+  long long pt = t0 + wt;
+  int ppage = -1, pblocks = 0;
+  auto look_up = [&]() {      // the page of block `lane` of tile pt
+    if (pt >= t1) return;
+    if (pt >= ps.start + ps.n) ps = locate(pt);
+    const int blk = (ps.tile0 + static_cast<int>(pt - ps.start)) * TB;
+    pblocks = min(TB, (ps.len + BLK - 1) / BLK - blk);
+    ppage = -1;
+    if (lane < pblocks) {
+      ppage = a.table[static_cast<long long>(ps.b) * a.width + (blk + lane) / a.cache.page_blocks];
+      if (ppage < 0 || ppage >= a.cache.pages) {
+        flag_error(kErrIndex);
+        ppage = -1;
+      }
+    }
+  };
+  unsigned have = 0;          // blocks of each stage that hold tokens, 8 bits a stage
+  auto issue = [&](int st) {  // copy tile pt into stage st, look up the next
+    if (pt >= t1) return;
+    const unsigned ok = __ballot_sync(0xffffffffu, ppage >= 0);
+    have = (have & ~(0xffu << (8 * st))) | (ok << (8 * st));
+    uint8_t* dst = stages + st * SH::STAGE;
+    if (lane == 0) mbar_arrive_expect_tx(&bar[st], __popc(ok) * SH::BLOCK);
+    __syncwarp();
+    const int blk = (ps.tile0 + static_cast<int>(pt - ps.start)) * TB + lane;
+    if (whole_tiles) {
+      if (lane == 0 && ok) bulk_load(dst, block_ptr(a.cache, ppage, ps.kh, blk % a.cache.page_blocks), pblocks * SH::BLOCK, &bar[st]);
+    } else if (ppage >= 0) {
+      bulk_load(dst + lane * SH::BLOCK, block_ptr(a.cache, ppage, ps.kh, blk % a.cache.page_blocks), SH::BLOCK, &bar[st]);
+    }
+    pt += TW;
+    look_up();
+  };
+  ps.start = 0;
+  ps.n = 0;
+  look_up();
+  int stage = 0;
+  uint32_t phases = 0;
+  issue(0);
+
+  // word of the token's codes that this lane's i-th fragment word is
+  auto key_word = [&](int i) { return NG == 1 ? (D / 32) * q4 + i : (i < 2 ? 2 * q4 + i : 8 + 2 * q4 + i - 2); };
+  constexpr int KW = D / 32;
+  const bool odd = q4 & 1;
+  const uint32_t sel_lo = odd ? 0x1054u : 0x5410u, sel_hi = odd ? 0x3276u : 0x7632u;
+
+  long long g = t0 + wt;
+  for (long long t = t0; t < t1;) {
+    const Segment s = locate(t);
+    const long long end = min(t1, s.start + s.n);
+
+    // ---- the rows' queries as B fragments, their sums, and what a score is scaled by
+    uint32_t qf[NT][KW][4];
+    float f[NT][2], qs[NT][2][NG];
+    int to[NT][2], from[NT][2];       // tokens [from, to) that a row sees
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = s.rt * ROWS + nt * 8 + r;
+      const bool live = row < s.count * a.share;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q);
+      if (live) src += (s.first + row / a.share) * a.q_st + (s.kh * a.share + row % a.share) * a.q_sh;
+      float x[KW][8];
+      float top = 0.0f, sum[NG];
+#pragma unroll
+      for (int i = 0; i < NG; ++i) sum[i] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < KW; ++i) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (live) v = *reinterpret_cast<const uint4*>(src + 8 * key_word(i));
+        const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (p.bf16) {
+            x[i][2 * j] = __uint_as_float(vv[j] << 16);
+            x[i][2 * j + 1] = __uint_as_float(vv[j] & 0xffff0000u);
+          } else {
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&vv[j]));
+            x[i][2 * j] = h.x;
+            x[i][2 * j + 1] = h.y;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          top = fmaxf(top, fabsf(x[i][j]));
+          sum[NG == 1 ? 0 : i / 2] += x[i][j];
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^e <= top < 2^(e+1), kept where 2^-e and 2^e are normal
+      const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
+      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23), up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+      for (int i = 0; i < KW; ++i) {
+        // fragment words: nibbles (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16 of word key_word(i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float by = (j & 1) ? down * 0.0625f : down;
+          const __half2 h = __floats2half2_rn(x[i][j] * by, x[i][j + 4] * by);
+          qf[nt][i][j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+      }
+      const float fr = a.scale * kLog2e * up * 16777216.0f;
+      const int pos = s.len - s.count + row / a.share;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {   // accumulators hold rows 2 q4 and 2 q4 + 1
+        const int src_lane = 4 * (2 * q4 + c);
+        f[nt][c] = __shfl_sync(0xffffffffu, fr, src_lane);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) qs[nt][c][i] = __shfl_sync(0xffffffffu, sum[i] * (a.scale * kLog2e), src_lane);
+        // a row past the last sees everything, so that it makes no tile an edge
+        to[nt][c] = __shfl_sync(0xffffffffu, live ? min(s.len, pos + 1) : s.len, src_lane);
+        from[nt][c] = __shfl_sync(0xffffffffu, live && a.window ? max(0, pos - a.window + 1) : 0, src_lane);
+      }
+    }
+    int all_from = 0, all_to = 0x7fffffff;   // tokens that every row of this warp's tile sees
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        all_from = max(all_from, from[nt][c]);
+        all_to = min(all_to, to[nt][c]);
+      }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      all_from = max(all_from, __shfl_xor_sync(0xffffffffu, all_from, o));
+      all_to = min(all_to, __shfl_xor_sync(0xffffffffu, all_to, o));
+    }
+
+    float acc[NT][SETS * 4][4] = {};
+    float m[NT][2], l[NT][2], corr[NT][2][NG];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        m[nt][c] = kNoMax;
+        l[nt][c] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) corr[nt][c][i] = 0.0f;
+      }
+
+    for (; g < end; g += TW) {
+      const unsigned have_now = have;
+      issue(stage ^ 1);
+      if (!mbar_wait(&bar[stage], (phases >> stage) & 1u, p.wait_ns))
+        mbar_wait(&bar[stage], (phases >> stage) & 1u, kWaitBudgetNs);   // never leave with a copy in flight
+      phases ^= 1u << stage;
+      const uint8_t* tile = stages + stage * SH::STAGE;
+      const unsigned blocks = (stage ? have_now >> 8 : have_now) & 0xffu;
+      const int tok0 = (s.tile0 + static_cast<int>(g - s.start)) * TT;
+      const bool edge = blocks != (1u << TB) - 1u || tok0 < all_from || tok0 + TT > all_to;
+
+      // ---- scores (log2 units)
+      float x[TB][NT][4];
+#pragma unroll
+      for (int k = 0; k < TB; ++k) {
+        const uint8_t* blk = tile + k * SH::BLOCK;
+        uint32_t w0[KW], w1[KW];       // this lane's words of tokens r and r + 8
+        if constexpr (NG == 1 && KW == 4) {
+          *reinterpret_cast<uint4*>(w0) = *reinterpret_cast<const uint4*>(blk + r * (D / 2) + 16 * q4);
+          *reinterpret_cast<uint4*>(w1) = *reinterpret_cast<const uint4*>(blk + (r + 8) * (D / 2) + 16 * q4);
+        } else {
+#pragma unroll
+          for (int i = 0; i < KW; i += 2) {
+            *reinterpret_cast<uint2*>(w0 + i) = *reinterpret_cast<const uint2*>(blk + r * (D / 2) + 4 * key_word(i));
+            *reinterpret_cast<uint2*>(w1 + i) = *reinterpret_cast<const uint2*>(blk + (r + 8) * (D / 2) + 4 * key_word(i));
+          }
+        }
+        const uint32_t* pairs = reinterpret_cast<const uint32_t*>(blk + key_pairs_at(D));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) x[k][nt][c] = 0.0f;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          float d[NT][4] = {};
+#pragma unroll
+          for (int i = gr * (KW / NG); i < (gr + 1) * (KW / NG); ++i) {
+            const uint32_t u0 = w0[i] >> 8, u1 = w1[i] >> 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816(d[nt], w0[i] & 0x000f000fu, w1[i] & 0x000f000fu, w0[i] & 0x00f000f0u, w1[i] & 0x00f000f0u,
+                       qf[nt][i][0], qf[nt][i][1]);
+              mma16816(d[nt], u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qf[nt][i][2],
+                       qf[nt][i][3]);
+            }
+          }
+          const float2 pr0 = __half22float2(*reinterpret_cast<const __half2*>(&pairs[r * NG + gr]));
+          const float2 pr1 = __half22float2(*reinterpret_cast<const __half2*>(&pairs[(r + 8) * NG + gr]));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float sc = c < 2 ? pr0.x : pr1.x, of = c < 2 ? pr0.y : pr1.y;
+              x[k][nt][c] += d[nt][c] * sc * f[nt][c & 1] + of * qs[nt][c & 1][gr];
+            }
+        }
+      }
+      if (edge) {
+#pragma unroll
+        for (int k = 0; k < TB; ++k)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int tok = tok0 + k * BLK + r + (c < 2 ? 0 : 8);
+              if (!((blocks >> k) & 1u) || tok < from[nt][c & 1] || tok >= to[nt][c & 1]) x[k][nt][c] = -INFINITY;
+            }
+      }
+
+      // ---- running maximum
+      float top[NT][2];
+      bool grows = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float v = x[0][nt][c];
+#pragma unroll
+          for (int k = 0; k < TB; ++k) v = fmaxf(v, fmaxf(x[k][nt][c], x[k][nt][c + 2]));
+          top[nt][c] = v;
+          grows |= v > m[nt][c] + kLazyMax;
+        }
+      if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float v = top[nt][c];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+            const float mn = v > m[nt][c] + kLazyMax ? v : m[nt][c];
+            const float by = ex2(m[nt][c] - mn);
+            m[nt][c] = mn;
+            l[nt][c] *= by;
+#pragma unroll
+            for (int i = 0; i < NG; ++i) corr[nt][c][i] *= by;
+#pragma unroll
+            for (int i = 0; i < SETS * 4; ++i) {
+              acc[nt][i][c] *= by;
+              acc[nt][i][c + 2] *= by;
+            }
+          }
+      }
+
+      // ---- probabilities and the second product
+#pragma unroll
+      for (int k = 0; k < TB; ++k) {
+        const uint8_t* blk = tile + k * SH::BLOCK;
+        const uint32_t* pairs = reinterpret_cast<const uint32_t*>(blk + value_pairs_at(D, NG));
+        uint32_t b[NT][NG][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            x[k][nt][c] = ex2(x[k][nt][c] - m[nt][c & 1]);
+            l[nt][c & 1] += x[k][nt][c];
+          }
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          const float2 pr0 = __half22float2(*reinterpret_cast<const __half2*>(&pairs[r * NG + gr]));
+          const float2 pr1 = __half22float2(*reinterpret_cast<const __half2*>(&pairs[(r + 8) * NG + gr]));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            __half h[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float pv = x[k][nt][c];
+              float ps = pv * (c < 2 ? pr0.x : pr1.x), po = pv * (c < 2 ? pr0.y : pr1.y);
+              if (edge && pv == 0.0f) ps = po = 0.0f;     // a token not seen may have any pair, NaN too
+              h[c] = __float2half_rn(ps);
+              corr[nt][c & 1][gr] += po + 7.5f * (ps - __half2float(h[c]));
+            }
+            const __half2 lo = __halves2half2(h[0], h[1]), hi = __halves2half2(h[2], h[3]);
+            b[nt][gr][0] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&lo));
+            b[nt][gr][1] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&hi));
+          }
+        }
+        // channels: set s of this lane's row r is word r + 8 s, nibble j (rows 0-7) and j + 4 (rows 8-15).
+        // Odd q4 load the second token of their pair first, so a load's lanes cover both halves of
+        // the banks (rows of 16 words).
+        const uint8_t* vals = blk + value_codes_at(D);
+        const int ta = 2 * q4 + (odd ? 1 : 0), tb = 2 * q4 + (odd ? 0 : 1);
+#pragma unroll
+        for (int s2 = 0; s2 < SETS; ++s2) {
+          const uint32_t* col = reinterpret_cast<const uint32_t*>(vals) + r + 8 * s2;
+          const uint32_t wa = col[ta * (D / 8)], wb = col[tb * (D / 8)];
+          const uint32_t wc = col[(ta + 8) * (D / 8)], wd = col[(tb + 8) * (D / 8)];
+          const uint32_t y[4] = {prmt(wa, wb, sel_lo), prmt(wa, wb, sel_hi), prmt(wc, wd, sel_lo), prmt(wc, wd, sel_hi)};
+          const uint32_t z[4] = {y[0] >> 8, y[1] >> 8, y[2] >> 8, y[3] >> 8};
+          constexpr int G1 = NG - 1;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint32_t* bb = b[nt][NG == 1 ? 0 : min(s2, G1)];
+            mma16816(acc[nt][4 * s2], y[0] & 0x000f000fu, y[1] & 0x000f000fu, y[2] & 0x000f000fu, y[3] & 0x000f000fu, bb[0], bb[1]);
+            mma16816(acc[nt][4 * s2 + 1], y[0] & 0x00f000f0u, y[1] & 0x00f000f0u, y[2] & 0x00f000f0u, y[3] & 0x00f000f0u, bb[0], bb[1]);
+            mma16816(acc[nt][4 * s2 + 2], z[0] & 0x000f000fu, z[1] & 0x000f000fu, z[2] & 0x000f000fu, z[3] & 0x000f000fu, bb[0], bb[1]);
+            mma16816(acc[nt][4 * s2 + 3], z[0] & 0x00f000f0u, z[1] & 0x00f000f0u, z[2] & 0x00f000f0u, z[3] & 0x00f000f0u, bb[0], bb[1]);
+          }
+        }
+      }
+      __syncwarp();
+      stage ^= 1;
+    }
+
+    // ---- this warp's sums over its lanes of tokens
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], o);
+#pragma unroll
+          for (int i = 0; i < NG; ++i) corr[nt][c][i] += __shfl_xor_sync(0xffffffffu, corr[nt][c][i], o);
+        }
+
+    // a warp's state in memory: float4 [ACC / 4][32], then m, l, corr [NT][2] as [...][32]
+    auto put = [&](float* to_) {
+      float4* q = reinterpret_cast<float4*>(to_) + lane;
+      float* e = to_ + SH::ACC * 32 + lane;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < SETS * 4; ++i) q[(nt * SETS * 4 + i) * 32] = make_float4(acc[nt][i][0], acc[nt][i][1], acc[nt][i][2], acc[nt][i][3]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          e[((nt * 2 + c) * (2 + NG)) * 32] = m[nt][c];
+          e[((nt * 2 + c) * (2 + NG) + 1) * 32] = l[nt][c];
+#pragma unroll
+          for (int i = 0; i < NG; ++i) e[((nt * 2 + c) * (2 + NG) + 2 + i) * 32] = corr[nt][c][i];
+        }
+      }
+    };
+    // ---- the team's warps, by halves
+    for (int half = TW / 2; half > 0; half >>= 1) {
+      float* slot = merge + (team_in_cta * (TW / 2) + (wt & (half - 1))) * SH::STATE;
+      if (wt >= half && wt < 2 * half) put(slot);
+      team_sync();
+      if (wt < half) {
+        const float4* q = reinterpret_cast<const float4*>(slot) + lane;
+        const float* e = slot + SH::ACC * 32 + lane;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float mine[2], theirs[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float* ec = e + ((nt * 2 + c) * (2 + NG)) * 32;
+            const float mo = ec[0], mn = fmaxf(m[nt][c], mo);
+            mine[c] = ex2(m[nt][c] - mn);
+            theirs[c] = ex2(mo - mn);
+            m[nt][c] = mn;
+            l[nt][c] = l[nt][c] * mine[c] + ec[32] * theirs[c];
+#pragma unroll
+            for (int i = 0; i < NG; ++i) corr[nt][c][i] = corr[nt][c][i] * mine[c] + ec[(2 + i) * 32] * theirs[c];
+          }
+#pragma unroll
+          for (int i = 0; i < SETS * 4; ++i) {
+            const float4 v = q[(nt * SETS * 4 + i) * 32];
+            acc[nt][i][0] = acc[nt][i][0] * mine[0] + v.x * theirs[0];
+            acc[nt][i][1] = acc[nt][i][1] * mine[1] + v.y * theirs[1];
+            acc[nt][i][2] = acc[nt][i][2] * mine[0] + v.z * theirs[0];
+            acc[nt][i][3] = acc[nt][i][3] * mine[1] + v.w * theirs[1];
+          }
+        }
+      }
+      team_sync();
+    }
+
+    // one set of eight channels per lane (word r + 8 set) of rows 2 q4 and 2 q4 + 1 of row tile nt:
+    // v[j] the accumulators of nibble pair (j, j + 4)
+    auto emit = [&](int nt, int set, const float (&v)[4][4], const float (&ml)[2], const float (&ll)[2], const float (&cc)[2]) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int row = s.rt * ROWS + nt * 8 + 2 * q4 + c;
+        if (row >= s.count * a.share) continue;
+        const float inv = ll[c] == 0.0f ? 0.0f : 1.0f / ll[c];
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float by = (j & 1) ? 1048576.0f : 16777216.0f;
+          y[j] = (v[j][c] * by + cc[c]) * inv;
+          y[j + 4] = (v[j][c + 2] * by + cc[c]) * inv;
+        }
+        uint4 o;
+        uint32_t* ov = &o.x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          ov[j] = p.bf16 ? pack2<__nv_bfloat16>(y[2 * j], y[2 * j + 1]) : pack2<__half>(y[2 * j], y[2 * j + 1]);
+        const long long at = static_cast<long long>(s.first + row / a.share) * a.heads + s.kh * a.share + row % a.share;
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + at * D + 8 * (r + 8 * set)) = o;
+        if (a.lse && r == 0 && set == 0) a.lse[at] = ll[c] == 0.0f ? -INFINITY : (ml[c] + log2f(ll[c])) * kLn2;
+      }
+    };
+    if (end - t == s.n) {
+      if (wt == 0) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int set = 0; set < SETS; ++set) {
+            const float cc[2] = {corr[nt][0][NG == 1 ? 0 : set], corr[nt][1][NG == 1 ? 0 : set]};
+            float v[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) v[j][c] = acc[nt][4 * set + j][c];
+            emit(nt, set, v, m[nt], l[nt], cc);
+          }
+      }
+    } else {
+      // ---- a part of the segment: leave it, and join the parts if this team is the last
+      const long long first_team = ((s.start + 1) * N - 1) / total, last_team = ((s.start + s.n) * N - 1) / total;
+      if (wt == 0) {
+        put(p.parts + (2 * team + (t == t0 ? 0 : 1)) * static_cast<long long>(SH::STATE));
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) {
+          const int n = atomicAdd(p.counters + first_team, 1);
+          const int last = n == static_cast<int>(last_team - first_team);
+          if (last) p.counters[first_team] = 0;     // every team has arrived: left zero for the next launch
+          last_flag[team_in_cta] = last;
+        }
+      }
+      team_sync();
+      const bool last = last_flag[team_in_cta] != 0;
+      team_sync();
+      if (last) {
+        __threadfence();
+        for (int i = wt; i < NT * SETS; i += TW) {
+          const int nt = i / SETS, set = i % SETS;
+          // a team's part of this segment is its first unless the segment starts inside its range
+          auto part = [&](long long tm) {
+            return p.parts + (2 * tm + (total * tm / N >= s.start ? 0 : 1)) * SH::STATE;
+          };
+          float mm[2] = {kNoMax, kNoMax};
+          for (long long tm = first_team; tm <= last_team; ++tm) {
+            const float* e = part(tm) + SH::ACC * 32 + lane + nt * 2 * (2 + NG) * 32;
+            mm[0] = fmaxf(mm[0], __ldcg(e));
+            mm[1] = fmaxf(mm[1], __ldcg(e + (2 + NG) * 32));
+          }
+          float v[4][4] = {}, ll[2] = {0.0f, 0.0f}, cc[2] = {0.0f, 0.0f};
+#pragma unroll 4
+          for (long long tm = first_team; tm <= last_team; ++tm) {
+            const float* base = part(tm);
+            const float* e = base + SH::ACC * 32 + lane + nt * 2 * (2 + NG) * 32;
+            float by[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float* ec = e + c * (2 + NG) * 32;
+              by[c] = ex2(__ldcg(ec) - mm[c]);
+              ll[c] += by[c] * __ldcg(ec + 32);
+              cc[c] += by[c] * __ldcg(ec + (2 + (NG == 1 ? 0 : set)) * 32);
+            }
+            const float4* q = reinterpret_cast<const float4*>(base) + lane + (nt * SETS + set) * 4 * 32;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float4 w = __ldcg(q + j * 32);
+              v[j][0] += by[0] * w.x;
+              v[j][1] += by[1] * w.y;
+              v[j][2] += by[0] * w.z;
+              v[j][3] += by[1] * w.w;
+            }
+          }
+          emit(nt, set, v, mm, ll, cc);
+        }
+      }
+    }
+    t = end;
+  }
+}
+
+}  // namespace kv4
+}  // namespace w4a16
