@@ -11,10 +11,11 @@
 // give 16 c * 2^-24; the queries' fragments for them carry 1/16, and the sums of the values'
 // channels with an odd nibble are divided by 16 at the end.
 //
-// Queries are scaled to a largest magnitude in [1, 2) by a power of two (exact, and any bf16
-// query then fits fp16). p s is the one rounding to 16 bits (2^-11); what it loses, r, would meet
-// codes of 7.5 on average, so 7.5 r is added back in fp32 and only r (c - 7.5) stays: the error
-// of rounding p times a value centred on its group.
+// The tile's queries are scaled to a largest magnitude in [1, 2) by a power of two (exact, and any
+// bf16 query then fits fp16). p s is the one rounding to 16 bits, h (2^-11). Rounded against codes of
+// 7.5 on average it would cost more than a rounding of p against centred values, so the sum is
+// taken as sum h (c - 7.5) + sum p (b + 7.5 s), the second term in fp32; the sum of h comes from one
+// more product, with ones.
 //
 // Both products take the cache as the M side of mma.m16n8k16 (16 tokens, or 16 channels) and
 // eight query rows as its N side, so no row of the tensor core is wasted on padding queries when
@@ -22,8 +23,8 @@
 // B fragment of the second product.
 //
 // Work: a segment is a kv head of a sequence (and a tile of 8 NT of its rows), a tile TB blocks
-// of 16 tokens. All tiles form one list that N teams of warps split evenly, whatever the lengths;
-// a team that holds a part of a segment leaves (m, l, o) in the workspace and the last of the
+// of 16 tokens. All tiles form one list that N teams of warps split evenly, whatever the lengths
+// (a segment counts `seg_cost` tiles more than it has, for its queries and its epilogue); a team that holds a part of a segment leaves (m, l, o) in the workspace and the last of the
 // segment's teams to arrive joins the parts in team order, so results do not depend on timing.
 // Each warp feeds itself: two stages of a tile, filled by bulk copies that its own lanes issue.
 #pragma once
@@ -73,6 +74,8 @@ struct DecodeParams {
   int bf16;                // q and o bf16, else fp16
   int row_limit;           // sequences with more rows than this are left to the other kernel
   int team_warps;          // warps per team: 1, 2, 4, ... W
+  int seg_cost;            // tiles that a segment counts more than it has
+  int page_shift;          // log2 of blocks per page, or -1
   int teams;               // most teams (CTAs * W / team_warps)
   int* counters;           // [teams] arrivals at a segment that several teams share, by the first of them; left zero
   float* parts;            // [teams * 2] partial results
@@ -93,7 +96,7 @@ struct DecodeShape {
 };
 
 struct Segment {
-  long long start;         // first tile of the segment in the list
+  long long start;         // its first tile's place in the list (after the seg_cost places without a tile)
   int n;                   // its tiles
   int b, kh, rt;           // sequence, kv head, row tile
   int first, count, len;   // the sequence's queries and cached tokens
@@ -144,7 +147,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     long long v = 0;
     if (b < a.seqs) {
       const long long h = extent(b, s);
-      v = h * s.n;
+      v = s.n ? h * (s.n + p.seg_cost) : 0;
     }
     long long inc = v;
 #pragma unroll
@@ -200,53 +203,59 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     }
     Segment s;
     extent(lo, s);
-    const int seg = static_cast<int>((t - prefix[lo]) / s.n);
+    const int seg = static_cast<int>((t - prefix[lo]) / (s.n + p.seg_cost));
     s.kh = seg % a.cache.kv_heads;
     s.rt = seg / a.cache.kv_heads;
-    s.start = prefix[lo] + static_cast<long long>(seg) * s.n;
+    s.start = prefix[lo] + static_cast<long long>(seg) * (s.n + p.seg_cost) + p.seg_cost;
     return s;
   };
 
   // ------------------------------ this warp's copies ------------------------------
+  // Lane j < TB copies block j of a tile, and looks its page up one tile ahead.
   uint8_t* stages = ring + warp * 2 * SH::STAGE;
   uint64_t* bar = &bars[2 * warp];
-  const bool whole_tiles = a.cache.page_blocks % TB == 0;   // a tile lies in one page
-  Segment ps;                 // segment of the tile to copy next, and that tile's page of this lane's block
-  long long pt = t0 + wt;
-  int ppage = -1, pblocks = 0;
-  auto look_up = [&]() {      // the page of block `lane` of tile pt
-    if (pt >= t1) return;
-    if (pt >= ps.start + ps.n) ps = locate(pt);
-    const int blk = (ps.tile0 + static_cast<int>(pt - ps.start)) * TB;
-    pblocks = min(TB, (ps.len + BLK - 1) / BLK - blk);
-    ppage = -1;
-    if (lane < pblocks) {
-      ppage = a.table[static_cast<long long>(ps.b) * a.width + (blk + lane) / a.cache.page_blocks];
-      if (ppage < 0 || ppage >= a.cache.pages) {
-        flag_error(kErrIndex);
-        ppage = -1;
+  const long long page_stride = a.cache.kv_heads * a.cache.page_bytes;
+  long long pt = t0 + wt, pend = t0;   // the next tile to copy, and the end of its segment
+  int pblk = 0, plast = 0;             // its block of this lane, and the sequence's blocks
+  const int* prow = nullptr;           // the sequence's row of the table
+  const uint8_t* phead = nullptr;      // its kv head in page 0
+  const uint8_t* psrc = nullptr;       // the block's bytes, or null
+  auto look_up = [&]() {
+    while (pt >= pend && pt < t1) {    // on to the segment that holds pt, past places without a tile
+      const Segment s = locate(pt);
+      if (pt < s.start) {
+        pt += (s.start - pt + TW - 1) / TW * TW;
+        pend = s.start;
+        if (pt >= s.start + s.n) continue;
       }
+      pend = s.start + s.n;
+      pblk = (s.tile0 + static_cast<int>(pt - s.start)) * TB + lane;
+      plast = (s.len + BLK - 1) / BLK;
+      prow = a.table + static_cast<long long>(s.b) * a.width;
+      phead = a.cache.pool + s.kh * a.cache.page_bytes;
+    }
+    psrc = nullptr;
+    if (pt < t1 && lane < TB && pblk < plast) {
+      const int col = p.page_shift >= 0 ? pblk >> p.page_shift : pblk / a.cache.page_blocks;
+      const int page = prow[col];
+      if (static_cast<unsigned>(page) < static_cast<unsigned>(a.cache.pages))
+        psrc = phead + page * page_stride + (pblk - col * a.cache.page_blocks) * SH::BLOCK;
+      else
+        flag_error(kErrIndex);
     }
   };
   unsigned have = 0;          // blocks of each stage that hold tokens, 8 bits a stage
   auto issue = [&](int st) {  // copy tile pt into stage st, look up the next
     if (pt >= t1) return;
-    const unsigned ok = __ballot_sync(0xffffffffu, ppage >= 0);
-    have = (have & ~(0xffu << (8 * st))) | (ok << (8 * st));
-    uint8_t* dst = stages + st * SH::STAGE;
+    const unsigned ok = __ballot_sync(0xffffffffu, psrc != nullptr);
+    have = st ? (have & 0xffu) | (ok << 8) : (have & 0xff00u) | ok;
     if (lane == 0) mbar_arrive_expect_tx(&bar[st], __popc(ok) * SH::BLOCK);
     __syncwarp();
-    const int blk = (ps.tile0 + static_cast<int>(pt - ps.start)) * TB + lane;
-    if (whole_tiles) {
-      if (lane == 0 && ok) bulk_load(dst, block_ptr(a.cache, ppage, ps.kh, blk % a.cache.page_blocks), pblocks * SH::BLOCK, &bar[st]);
-    } else if (ppage >= 0) {
-      bulk_load(dst + lane * SH::BLOCK, block_ptr(a.cache, ppage, ps.kh, blk % a.cache.page_blocks), SH::BLOCK, &bar[st]);
-    }
+    if (psrc != nullptr) bulk_load(stages + st * SH::STAGE + lane * SH::BLOCK, psrc, SH::BLOCK, &bar[st]);
     pt += TW;
+    pblk += TW * TB;
     look_up();
   };
-  ps.start = 0;
-  ps.n = 0;
   look_up();
   int stage = 0;
   uint32_t phases = 0;
@@ -258,23 +267,26 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
   const bool odd = q4 & 1;
   const uint32_t sel_lo = odd ? 0x1054u : 0x5410u, sel_hi = odd ? 0x3276u : 0x7632u;
 
-  long long g = t0 + wt;
   for (long long t = t0; t < t1;) {
     const Segment s = locate(t);
+    if (t < s.start) {
+      t = s.start;
+      if (t >= t1) break;
+    }
     const long long end = min(t1, s.start + s.n);
 
     // ---- the rows' queries as B fragments, their sums, and what a score is scaled by
     uint32_t qf[NT][KW][4];
-    float f[NT][2], qs[NT][2][NG];
+    float qs[NT][2][NG];
     int to[NT][2], from[NT][2];       // tokens [from, to) that a row sees
+    float x[NT][KW][8], top = 0.0f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = s.rt * ROWS + nt * 8 + r;
       const bool live = row < s.count * a.share;
       const uint16_t* src = static_cast<const uint16_t*>(a.q);
       if (live) src += (s.first + row / a.share) * a.q_st + (s.kh * a.share + row % a.share) * a.q_sh;
-      float x[KW][8];
-      float top = 0.0f, sum[NG];
+      float sum[NG];
 #pragma unroll
       for (int i = 0; i < NG; ++i) sum[i] = 0.0f;
 #pragma unroll
@@ -285,33 +297,18 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (p.bf16) {
-            x[i][2 * j] = __uint_as_float(vv[j] << 16);
-            x[i][2 * j + 1] = __uint_as_float(vv[j] & 0xffff0000u);
+            x[nt][i][2 * j] = __uint_as_float(vv[j] << 16);
+            x[nt][i][2 * j + 1] = __uint_as_float(vv[j] & 0xffff0000u);
           } else {
             const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&vv[j]));
-            x[i][2 * j] = h.x;
-            x[i][2 * j + 1] = h.y;
+            x[nt][i][2 * j] = h.x;
+            x[nt][i][2 * j + 1] = h.y;
           }
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          top = fmaxf(top, fabsf(x[i][j]));
-          sum[NG == 1 ? 0 : i / 2] += x[i][j];
-        }
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^e <= top < 2^(e+1), kept where 2^-e and 2^e are normal
-      const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
-      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23), up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-#pragma unroll
-      for (int i = 0; i < KW; ++i) {
-        // fragment words: nibbles (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16 of word key_word(i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float by = (j & 1) ? down * 0.0625f : down;
-          const __half2 h = __floats2half2_rn(x[i][j] * by, x[i][j + 4] * by);
-          qf[nt][i][j] = *reinterpret_cast<const uint32_t*>(&h);
+          top = fmaxf(top, fabsf(x[nt][i][j]));
+          sum[NG == 1 ? 0 : i / 2] += x[nt][i][j];
         }
       }
 #pragma unroll
@@ -319,12 +316,10 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
       }
-      const float fr = a.scale * kLog2e * up * 16777216.0f;
       const int pos = s.len - s.count + row / a.share;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {   // accumulators hold rows 2 q4 and 2 q4 + 1
         const int src_lane = 4 * (2 * q4 + c);
-        f[nt][c] = __shfl_sync(0xffffffffu, fr, src_lane);
 #pragma unroll
         for (int i = 0; i < NG; ++i) qs[nt][c][i] = __shfl_sync(0xffffffffu, sum[i] * (a.scale * kLog2e), src_lane);
         // a row past the last sees everything, so that it makes no tile an edge
@@ -332,6 +327,23 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
         from[nt][c] = __shfl_sync(0xffffffffu, live && a.window ? max(0, pos - a.window + 1) : 0, src_lane);
       }
     }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // 2^e <= top < 2^(e+1), kept where 2^-e and 2^e are normal
+    const int e2 = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
+    const float f = a.scale * kLog2e * 16777216.0f * __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < KW; ++i)
+        // fragment words: nibbles (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16 of word key_word(i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float by = (j & 1) ? down * 0.0625f : down;
+          const __half2 h = __floats2half2_rn(x[nt][i][j] * by, x[nt][i][j + 4] * by);
+          qf[nt][i][j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
     int all_from = 0, all_to = 0x7fffffff;   // tokens that every row of this warp's tile sees
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -346,31 +358,35 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
       all_to = min(all_to, __shfl_xor_sync(0xffffffffu, all_to, o));
     }
 
-    float acc[NT][SETS * 4][4] = {};
+    float acc[NT][SETS * 4][4] = {}, hsum[NT][NG][4] = {};
     float m[NT][2], l[NT][2], corr[NT][2][NG];
+    unsigned fresh = (1u << (2 * NT)) - 1u;    // rows that have seen no token yet (their m is 0 until then)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        m[nt][c] = kNoMax;
+        m[nt][c] = 0.0f;
         l[nt][c] = 0.0f;
 #pragma unroll
         for (int i = 0; i < NG; ++i) corr[nt][c][i] = 0.0f;
       }
 
-    for (; g < end; g += TW) {
-      const unsigned have_now = have;
+    // this warp's tiles of the piece: those at t0 + wt + k TW
+    int g = static_cast<int>(t - t0);
+    g = static_cast<int>(t - s.start) + ((wt - g) & (TW - 1));
+    const int stop = static_cast<int>(end - s.start);
+    for (; g < stop; g += TW) {
+      const unsigned blocks = (stage ? have >> 8 : have) & 0xffu;
       issue(stage ^ 1);
       if (!mbar_wait(&bar[stage], (phases >> stage) & 1u, p.wait_ns))
         mbar_wait(&bar[stage], (phases >> stage) & 1u, kWaitBudgetNs);   // never leave with a copy in flight
       phases ^= 1u << stage;
       const uint8_t* tile = stages + stage * SH::STAGE;
-      const unsigned blocks = (stage ? have_now >> 8 : have_now) & 0xffu;
-      const int tok0 = (s.tile0 + static_cast<int>(g - s.start)) * TT;
+      const int tok0 = (s.tile0 + g) * TT;
       const bool edge = blocks != (1u << TB) - 1u || tok0 < all_from || tok0 + TT > all_to;
 
-      // ---- scores (log2 units)
-      float x[TB][NT][4];
+      // ---- scores over the running maximum, log2 units
+      float y[TB][NT][4];
 #pragma unroll
       for (int k = 0; k < TB; ++k) {
         const uint8_t* blk = tile + k * SH::BLOCK;
@@ -389,7 +405,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) x[k][nt][c] = 0.0f;
+          for (int c = 0; c < 4; ++c) y[k][nt][c] = -m[nt][c & 1];
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
           float d[NT][4] = {};
@@ -406,13 +422,12 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
           }
           const float2 pr0 = __half22float2(*reinterpret_cast<const __half2*>(&pairs[r * NG + gr]));
           const float2 pr1 = __half22float2(*reinterpret_cast<const __half2*>(&pairs[(r + 8) * NG + gr]));
+          const float s0 = pr0.x * f, s1 = pr1.x * f;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const float sc = c < 2 ? pr0.x : pr1.x, of = c < 2 ? pr0.y : pr1.y;
-              x[k][nt][c] += d[nt][c] * sc * f[nt][c & 1] + of * qs[nt][c & 1][gr];
-            }
+            for (int c = 0; c < 4; ++c)
+              y[k][nt][c] = fmaf(d[nt][c], c < 2 ? s0 : s1, fmaf(c < 2 ? pr0.y : pr1.y, qs[nt][c & 1][gr], y[k][nt][c]));
         }
       }
       if (edge) {
@@ -423,37 +438,48 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const int tok = tok0 + k * BLK + r + (c < 2 ? 0 : 8);
-              if (!((blocks >> k) & 1u) || tok < from[nt][c & 1] || tok >= to[nt][c & 1]) x[k][nt][c] = -INFINITY;
+              if (!((blocks >> k) & 1u) || tok < from[nt][c & 1] || tok >= to[nt][c & 1]) y[k][nt][c] = -INFINITY;
             }
       }
 
       // ---- running maximum
-      float top[NT][2];
-      bool grows = false;
+      float top_y[NT][2];
+      bool grows = fresh != 0;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float v = x[0][nt][c];
+          float v = fmaxf(y[0][nt][c], y[0][nt][c + 2]);
 #pragma unroll
-          for (int k = 0; k < TB; ++k) v = fmaxf(v, fmaxf(x[k][nt][c], x[k][nt][c + 2]));
-          top[nt][c] = v;
-          grows |= v > m[nt][c] + kLazyMax;
+          for (int k = 1; k < TB; ++k) v = fmaxf(v, fmaxf(y[k][nt][c], y[k][nt][c + 2]));
+          top_y[nt][c] = v;
+          grows |= v > kLazyMax;
         }
       if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float v = top[nt][c];
+            float v = top_y[nt][c];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-            const float mn = v > m[nt][c] + kLazyMax ? v : m[nt][c];
-            const float by = ex2(m[nt][c] - mn);
-            m[nt][c] = mn;
+            const unsigned bit = 1u << (2 * nt + c);
+            const bool first = (fresh & bit) != 0;
+            const float up = v > (first ? -INFINITY : kLazyMax) ? v : 0.0f;
+            const float by = first ? 1.0f : ex2(-up);      // nothing to scale yet
+            if (v > -INFINITY) fresh &= ~bit;
+            m[nt][c] += up;
             l[nt][c] *= by;
 #pragma unroll
-            for (int i = 0; i < NG; ++i) corr[nt][c][i] *= by;
+            for (int k = 0; k < TB; ++k) {
+              y[k][nt][c] -= up;
+              y[k][nt][c + 2] -= up;
+            }
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+              corr[nt][c][i] *= by;
+              hsum[nt][i][c] *= by;
+            }
 #pragma unroll
             for (int i = 0; i < SETS * 4; ++i) {
               acc[nt][i][c] *= by;
@@ -472,27 +498,34 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            x[k][nt][c] = ex2(x[k][nt][c] - m[nt][c & 1]);
-            l[nt][c & 1] += x[k][nt][c];
+            y[k][nt][c] = ex2(y[k][nt][c]);
+            l[nt][c & 1] += y[k][nt][c];
           }
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
           const float2 pr0 = __half22float2(*reinterpret_cast<const __half2*>(&pairs[r * NG + gr]));
           const float2 pr1 = __half22float2(*reinterpret_cast<const __half2*>(&pairs[(r + 8) * NG + gr]));
+          const float o0 = fmaf(7.5f, pr0.x, pr0.y), o1 = fmaf(7.5f, pr1.x, pr1.y);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            __half h[4];
+            float ps[4];
+            if (edge) {            // a token that is not seen may have any pair, NaN too
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const float pv = x[k][nt][c];
-              float ps = pv * (c < 2 ? pr0.x : pr1.x), po = pv * (c < 2 ? pr0.y : pr1.y);
-              if (edge && pv == 0.0f) ps = po = 0.0f;     // a token not seen may have any pair, NaN too
-              h[c] = __float2half_rn(ps);
-              corr[nt][c & 1][gr] += po + 7.5f * (ps - __half2float(h[c]));
+              for (int c = 0; c < 4; ++c) {
+                const float pv = y[k][nt][c];
+                ps[c] = pv == 0.0f ? 0.0f : pv * (c < 2 ? pr0.x : pr1.x);
+                if (pv != 0.0f) corr[nt][c & 1][gr] = fmaf(pv, c < 2 ? o0 : o1, corr[nt][c & 1][gr]);
+              }
+            } else {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                ps[c] = y[k][nt][c] * (c < 2 ? pr0.x : pr1.x);
+                corr[nt][c & 1][gr] = fmaf(y[k][nt][c], c < 2 ? o0 : o1, corr[nt][c & 1][gr]);
+              }
             }
-            const __half2 lo = __halves2half2(h[0], h[1]), hi = __halves2half2(h[2], h[3]);
-            b[nt][gr][0] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&lo));
-            b[nt][gr][1] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&hi));
+            b[nt][gr][0] = movmatrix_trans(pack2<__half>(ps[0], ps[1]));
+            b[nt][gr][1] = movmatrix_trans(pack2<__half>(ps[2], ps[3]));
+            mma16816(hsum[nt][gr], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, b[nt][gr][0], b[nt][gr][1]);
           }
         }
         // channels: set s of this lane's row r is word r + 8 s, nibble j (rows 0-7) and j + 4 (rows 8-15).
@@ -505,14 +538,13 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
           const uint32_t* col = reinterpret_cast<const uint32_t*>(vals) + r + 8 * s2;
           const uint32_t wa = col[ta * (D / 8)], wb = col[tb * (D / 8)];
           const uint32_t wc = col[(ta + 8) * (D / 8)], wd = col[(tb + 8) * (D / 8)];
-          const uint32_t y[4] = {prmt(wa, wb, sel_lo), prmt(wa, wb, sel_hi), prmt(wc, wd, sel_lo), prmt(wc, wd, sel_hi)};
-          const uint32_t z[4] = {y[0] >> 8, y[1] >> 8, y[2] >> 8, y[3] >> 8};
-          constexpr int G1 = NG - 1;
+          const uint32_t v[4] = {prmt(wa, wb, sel_lo), prmt(wa, wb, sel_hi), prmt(wc, wd, sel_lo), prmt(wc, wd, sel_hi)};
+          const uint32_t z[4] = {v[0] >> 8, v[1] >> 8, v[2] >> 8, v[3] >> 8};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            const uint32_t* bb = b[nt][NG == 1 ? 0 : min(s2, G1)];
-            mma16816(acc[nt][4 * s2], y[0] & 0x000f000fu, y[1] & 0x000f000fu, y[2] & 0x000f000fu, y[3] & 0x000f000fu, bb[0], bb[1]);
-            mma16816(acc[nt][4 * s2 + 1], y[0] & 0x00f000f0u, y[1] & 0x00f000f0u, y[2] & 0x00f000f0u, y[3] & 0x00f000f0u, bb[0], bb[1]);
+            const uint32_t* bb = b[nt][NG == 1 ? 0 : s2];
+            mma16816(acc[nt][4 * s2], v[0] & 0x000f000fu, v[1] & 0x000f000fu, v[2] & 0x000f000fu, v[3] & 0x000f000fu, bb[0], bb[1]);
+            mma16816(acc[nt][4 * s2 + 1], v[0] & 0x00f000f0u, v[1] & 0x00f000f0u, v[2] & 0x00f000f0u, v[3] & 0x00f000f0u, bb[0], bb[1]);
             mma16816(acc[nt][4 * s2 + 2], z[0] & 0x000f000fu, z[1] & 0x000f000fu, z[2] & 0x000f000fu, z[3] & 0x000f000fu, bb[0], bb[1]);
             mma16816(acc[nt][4 * s2 + 3], z[0] & 0x00f000f0u, z[1] & 0x00f000f0u, z[2] & 0x00f000f0u, z[3] & 0x00f000f0u, bb[0], bb[1]);
           }
@@ -533,6 +565,14 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
 #pragma unroll
           for (int i = 0; i < NG; ++i) corr[nt][c][i] += __shfl_xor_sync(0xffffffffu, corr[nt][c][i], o);
         }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if ((fresh >> (2 * nt + c)) & 1u) m[nt][c] = kNoMax;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) corr[nt][c][i] = fmaf(-7.5f, hsum[nt][i][c], corr[nt][c][i]);
+      }
 
     // a warp's state in memory: float4 [ACC / 4][32], then m, l, corr [NT][2] as [...][32]
     auto put = [&](float* to_) {
@@ -630,7 +670,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
       // ---- a part of the segment: leave it, and join the parts if this team is the last
       const long long first_team = ((s.start + 1) * N - 1) / total, last_team = ((s.start + s.n) * N - 1) / total;
       if (wt == 0) {
-        put(p.parts + (2 * team + (t == t0 ? 0 : 1)) * static_cast<long long>(SH::STATE));
+        put(p.parts + (2 * team + (t0 >= s.start ? 0 : 1)) * static_cast<long long>(SH::STATE));
         __threadfence();
         __syncwarp();
         if (lane == 0) {
