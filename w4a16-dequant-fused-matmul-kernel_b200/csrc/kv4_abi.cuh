@@ -227,9 +227,6 @@ int launch_decode(const w4a16_kv4_cache& c, const AttendParams& all, const Atten
       if (dev.num_sms * (C::W / tw) > kCounterBytes / 4) return W4A16_ERR_DEVICE;
       p.team_warps = tw;
       p.seg_cost = tw;
-      p.page_shift = -1;
-      for (int i = 0; i < 12; ++i)
-        if (p.a.cache.page_blocks == 1 << i) p.page_shift = i;
       p.teams = dev.num_sms * (C::W / tw);
       auto k = C::kernel();
       static std::atomic<uint64_t> ready{0};   // devices whose shared memory limit is set

@@ -29,6 +29,8 @@
 // Each warp feeds itself: two stages of a tile, filled by bulk copies that its own lanes issue.
 #pragma once
 
+#include <type_traits>
+
 #include "kv4_attend.cuh"
 
 namespace w4a16 {
@@ -50,7 +52,7 @@ __device__ __forceinline__ float ex2(float x) {
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 
@@ -59,6 +61,14 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same with accumulators that start at zero.
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // Bulk copy of `bytes` (a multiple of 16) into shared memory, completing on `bar`.
@@ -75,7 +85,6 @@ struct DecodeParams {
   int row_limit;           // sequences with more rows than this are left to the other kernel
   int team_warps;          // warps per team: 1, 2, 4, ... W
   int seg_cost;            // tiles that a segment counts more than it has
-  int page_shift;          // log2 of blocks per page, or -1
   int teams;               // most teams (CTAs * W / team_warps)
   int* counters;           // [teams] arrivals at a segment that several teams share, by the first of them; left zero
   float* parts;            // [teams * 2] partial results
@@ -211,52 +220,74 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
   };
 
   // ------------------------------ this warp's copies ------------------------------
-  // Lane j < TB copies block j of a tile, and looks its page up one tile ahead.
+  // A tile arrives with one copy where it lies in one page (`whole_tiles`), else block by block. The
+  // sources of the next 32 copies are looked up together, one per lane; lane 0 issues them in turn.
   uint8_t* stages = ring + warp * 2 * SH::STAGE;
   uint64_t* bar = &bars[2 * warp];
-  const long long page_stride = a.cache.kv_heads * a.cache.page_bytes;
-  long long pt = t0 + wt, pend = t0;   // the next tile to copy, and the end of its segment
-  int pblk = 0, plast = 0;             // its block of this lane, and the sequence's blocks
+  const bool whole_tiles = a.cache.page_blocks % TB == 0;
+  const int per_tile = whole_tiles ? 1 : TB;
+  long long pt = t0 + wt;              // the next tile to copy
+  int pleft = 0, ptaken = 32;          // tiles of its segment left for this warp, and sources used
+  int pblk = 0, plast = 0;             // its first block, and the sequence's blocks
   const int* prow = nullptr;           // the sequence's row of the table
   const uint8_t* phead = nullptr;      // its kv head in page 0
-  const uint8_t* psrc = nullptr;       // the block's bytes, or null
-  auto look_up = [&]() {
-    while (pt >= pend && pt < t1) {    // on to the segment that holds pt, past places without a tile
+  unsigned long long psrc = 0;         // this lane's source (0: none)
+  unsigned have = 0;                   // blocks of each stage that hold tokens, 8 bits a stage
+  auto refill = [&]() {                // called with every lane, at a new segment or after 32 sources
+    while (pleft == 0 && pt < t1) {    // on to the segment that holds pt, past places without a tile
       const Segment s = locate(pt);
       if (pt < s.start) {
         pt += (s.start - pt + TW - 1) / TW * TW;
-        pend = s.start;
         if (pt >= s.start + s.n) continue;
       }
-      pend = s.start + s.n;
-      pblk = (s.tile0 + static_cast<int>(pt - s.start)) * TB + lane;
+      if (pt >= t1) break;
+      pleft = static_cast<int>((min(t1, s.start + s.n) - pt + TW - 1) / TW);
+      pblk = (s.tile0 + static_cast<int>(pt - s.start)) * TB;
       plast = (s.len + BLK - 1) / BLK;
       prow = a.table + static_cast<long long>(s.b) * a.width;
       phead = a.cache.pool + s.kh * a.cache.page_bytes;
     }
-    psrc = nullptr;
-    if (pt < t1 && lane < TB && pblk < plast) {
-      const int col = p.page_shift >= 0 ? pblk >> p.page_shift : pblk / a.cache.page_blocks;
-      const int page = prow[col];
+    ptaken = 0;
+    psrc = 0;
+    const int tile = lane / per_tile, blk = pblk + tile * TW * TB + lane % per_tile;
+    if (tile < pleft && blk < plast) {
+      const int col = blk / a.cache.page_blocks, page = prow[col];
       if (static_cast<unsigned>(page) < static_cast<unsigned>(a.cache.pages))
-        psrc = phead + page * page_stride + (pblk - col * a.cache.page_blocks) * SH::BLOCK;
+        psrc = reinterpret_cast<unsigned long long>(phead + page * (a.cache.kv_heads * a.cache.page_bytes) +
+                                                    (blk - col * a.cache.page_blocks) * SH::BLOCK);
       else
         flag_error(kErrIndex);
     }
-  };
-  unsigned have = 0;          // blocks of each stage that hold tokens, 8 bits a stage
-  auto issue = [&](int st) {  // copy tile pt into stage st, look up the next
-    if (pt >= t1) return;
-    const unsigned ok = __ballot_sync(0xffffffffu, psrc != nullptr);
-    have = st ? (have & 0xffu) | (ok << 8) : (have & 0xff00u) | ok;
-    if (lane == 0) mbar_arrive_expect_tx(&bar[st], __popc(ok) * SH::BLOCK);
     __syncwarp();
-    if (psrc != nullptr) bulk_load(stages + st * SH::STAGE + lane * SH::BLOCK, psrc, SH::BLOCK, &bar[st]);
-    pt += TW;
-    pblk += TW * TB;
-    look_up();
   };
-  look_up();
+  auto issue = [&](int st) {           // copy the next tile into stage st
+    if (pleft == 0 || ptaken + per_tile > 32) refill();
+    if (pleft == 0) return;
+    const int blocks = min(TB, plast - pblk);
+    uint8_t* dst = stages + st * SH::STAGE;
+    unsigned ok = 0;
+    if (whole_tiles) {
+      const unsigned long long src = __shfl_sync(0xffffffffu, psrc, ptaken);
+      if (src) ok = (1u << blocks) - 1u;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bar[st], src ? blocks * SH::BLOCK : 0);
+        if (src) bulk_load(dst, reinterpret_cast<const void*>(src), blocks * SH::BLOCK, &bar[st]);
+      }
+    } else {
+      ok = (__ballot_sync(0xffffffffu, psrc != 0) >> ptaken) & ((1u << TB) - 1u);
+      if (lane == 0) mbar_arrive_expect_tx(&bar[st], __popc(ok) * SH::BLOCK);
+#pragma unroll 1
+      for (int j = 0; j < TB; ++j) {
+        const unsigned long long src = __shfl_sync(0xffffffffu, psrc, ptaken + j);
+        if (lane == 0 && src) bulk_load(dst + j * SH::BLOCK, reinterpret_cast<const void*>(src), SH::BLOCK, &bar[st]);
+      }
+    }
+    have = st ? (have & 0xffu) | (ok << 8) : (have & 0xff00u) | ok;
+    ptaken += per_tile;
+    pblk += TW * TB;
+    pt += TW;
+    --pleft;
+  };
   int stage = 0;
   uint32_t phases = 0;
   issue(0);
@@ -375,16 +406,15 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     int g = static_cast<int>(t - t0);
     g = static_cast<int>(t - s.start) + ((wt - g) & (TW - 1));
     const int stop = static_cast<int>(end - s.start);
-    for (; g < stop; g += TW) {
-      const unsigned blocks = (stage ? have >> 8 : have) & 0xffu;
-      issue(stage ^ 1);
-      if (!mbar_wait(&bar[stage], (phases >> stage) & 1u, p.wait_ns))
-        mbar_wait(&bar[stage], (phases >> stage) & 1u, kWaitBudgetNs);   // never leave with a copy in flight
-      phases ^= 1u << stage;
-      const uint8_t* tile = stages + stage * SH::STAGE;
-      const int tok0 = (s.tile0 + g) * TT;
-      const bool edge = blocks != (1u << TB) - 1u || tok0 < all_from || tok0 + TT > all_to;
+    // tiles [inside_lo, inside_hi) of the segment lie within what every row sees
+    const int inside_lo = (all_from + TT - 1) / TT - s.tile0, inside_hi = all_to / TT - s.tile0;
+    const uint32_t lane_k = (NG == 1 && KW == 4) ? r * (D / 2) + 16 * q4 : r * (D / 2);
+    const uint32_t lane_va = value_codes_at(D) + (2 * q4 + (odd ? 1 : 0)) * (D / 2) + 4 * r;
+    const uint32_t lane_vb = value_codes_at(D) + (2 * q4 + (odd ? 0 : 1)) * (D / 2) + 4 * r;
 
+    // One tile. EDGE: some row may not see some token of it.
+    auto step = [&](auto edge_tag, const uint8_t* tile, unsigned blocks, int tok0) {
+      constexpr bool EDGE = decltype(edge_tag)::value;
       // ---- scores over the running maximum, log2 units
       float y[TB][NT][4];
 #pragma unroll
@@ -392,13 +422,13 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
         const uint8_t* blk = tile + k * SH::BLOCK;
         uint32_t w0[KW], w1[KW];       // this lane's words of tokens r and r + 8
         if constexpr (NG == 1 && KW == 4) {
-          *reinterpret_cast<uint4*>(w0) = *reinterpret_cast<const uint4*>(blk + r * (D / 2) + 16 * q4);
-          *reinterpret_cast<uint4*>(w1) = *reinterpret_cast<const uint4*>(blk + (r + 8) * (D / 2) + 16 * q4);
+          *reinterpret_cast<uint4*>(w0) = *reinterpret_cast<const uint4*>(blk + lane_k);
+          *reinterpret_cast<uint4*>(w1) = *reinterpret_cast<const uint4*>(blk + lane_k + 4 * D);
         } else {
 #pragma unroll
           for (int i = 0; i < KW; i += 2) {
-            *reinterpret_cast<uint2*>(w0 + i) = *reinterpret_cast<const uint2*>(blk + r * (D / 2) + 4 * key_word(i));
-            *reinterpret_cast<uint2*>(w1 + i) = *reinterpret_cast<const uint2*>(blk + (r + 8) * (D / 2) + 4 * key_word(i));
+            *reinterpret_cast<uint2*>(w0 + i) = *reinterpret_cast<const uint2*>(blk + lane_k + 4 * key_word(i));
+            *reinterpret_cast<uint2*>(w1 + i) = *reinterpret_cast<const uint2*>(blk + lane_k + 4 * D + 4 * key_word(i));
           }
         }
         const uint32_t* pairs = reinterpret_cast<const uint32_t*>(blk + key_pairs_at(D));
@@ -408,14 +438,18 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
           for (int c = 0; c < 4; ++c) y[k][nt][c] = -m[nt][c & 1];
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
-          float d[NT][4] = {};
+          float d[NT][4];
 #pragma unroll
           for (int i = gr * (KW / NG); i < (gr + 1) * (KW / NG); ++i) {
             const uint32_t u0 = w0[i] >> 8, u1 = w1[i] >> 8;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma16816(d[nt], w0[i] & 0x000f000fu, w1[i] & 0x000f000fu, w0[i] & 0x00f000f0u, w1[i] & 0x00f000f0u,
-                       qf[nt][i][0], qf[nt][i][1]);
+              if (i == gr * (KW / NG))
+                mma16816_first(d[nt], w0[i] & 0x000f000fu, w1[i] & 0x000f000fu, w0[i] & 0x00f000f0u, w1[i] & 0x00f000f0u,
+                               qf[nt][i][0], qf[nt][i][1]);
+              else
+                mma16816(d[nt], w0[i] & 0x000f000fu, w1[i] & 0x000f000fu, w0[i] & 0x00f000f0u, w1[i] & 0x00f000f0u,
+                         qf[nt][i][0], qf[nt][i][1]);
               mma16816(d[nt], u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qf[nt][i][2],
                        qf[nt][i][3]);
             }
@@ -430,7 +464,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
               y[k][nt][c] = fmaf(d[nt][c], c < 2 ? s0 : s1, fmaf(c < 2 ? pr0.y : pr1.y, qs[nt][c & 1][gr], y[k][nt][c]));
         }
       }
-      if (edge) {
+      if constexpr (EDGE) {
 #pragma unroll
         for (int k = 0; k < TB; ++k)
 #pragma unroll
@@ -509,7 +543,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float ps[4];
-            if (edge) {            // a token that is not seen may have any pair, NaN too
+            if constexpr (EDGE) {            // a token that is not seen may have any pair, NaN too
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
                 const float pv = y[k][nt][c];
@@ -531,13 +565,12 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
         // channels: set s of this lane's row r is word r + 8 s, nibble j (rows 0-7) and j + 4 (rows 8-15).
         // Odd q4 load the second token of their pair first, so a load's lanes cover both halves of
         // the banks (rows of 16 words).
-        const uint8_t* vals = blk + value_codes_at(D);
-        const int ta = 2 * q4 + (odd ? 1 : 0), tb = 2 * q4 + (odd ? 0 : 1);
 #pragma unroll
         for (int s2 = 0; s2 < SETS; ++s2) {
-          const uint32_t* col = reinterpret_cast<const uint32_t*>(vals) + r + 8 * s2;
-          const uint32_t wa = col[ta * (D / 8)], wb = col[tb * (D / 8)];
-          const uint32_t wc = col[(ta + 8) * (D / 8)], wd = col[(tb + 8) * (D / 8)];
+          const uint32_t wa = *reinterpret_cast<const uint32_t*>(blk + lane_va + 32 * s2);
+          const uint32_t wb = *reinterpret_cast<const uint32_t*>(blk + lane_vb + 32 * s2);
+          const uint32_t wc = *reinterpret_cast<const uint32_t*>(blk + lane_va + 4 * D + 32 * s2);
+          const uint32_t wd = *reinterpret_cast<const uint32_t*>(blk + lane_vb + 4 * D + 32 * s2);
           const uint32_t v[4] = {prmt(wa, wb, sel_lo), prmt(wa, wb, sel_hi), prmt(wc, wd, sel_lo), prmt(wc, wd, sel_hi)};
           const uint32_t z[4] = {v[0] >> 8, v[1] >> 8, v[2] >> 8, v[3] >> 8};
 #pragma unroll
@@ -550,6 +583,20 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
           }
         }
       }
+    };
+    for (; g < stop; g += TW) {
+      const unsigned blocks = (stage ? have >> 8 : have) & 0xffu;
+      issue(stage ^ 1);
+      if (!mbar_try_wait(&bar[stage], (phases >> stage) & 1u)) {
+        if (!mbar_wait(&bar[stage], (phases >> stage) & 1u, p.wait_ns))
+          mbar_wait(&bar[stage], (phases >> stage) & 1u, kWaitBudgetNs);   // never leave with a copy in flight
+      }
+      phases ^= 1u << stage;
+      const uint8_t* tile = stages + stage * SH::STAGE;
+      if (blocks == (1u << TB) - 1u && g >= inside_lo && g < inside_hi)
+        step(std::false_type(), tile, blocks, 0);
+      else
+        step(std::true_type(), tile, blocks, (s.tile0 + g) * TT);
       __syncwarp();
       stage ^= 1;
     }
