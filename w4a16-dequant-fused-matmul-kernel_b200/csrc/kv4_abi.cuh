@@ -192,7 +192,7 @@ long long decode_workspace(const w4a16_kv4_cache& c, const AttendPlan& p, const 
   long long parts = 0;
   with_decode_config(c, decode_nt(p), [&](auto cfg) {
     using C = decltype(cfg);
-    parts = static_cast<long long>(dev.num_sms) * (C::W / decode_team_warps(p, C::W, dev)) * 2 * C::Shape::STATE * 4;
+    parts = static_cast<long long>(dev.num_sms) * (C::W / decode_team_warps(p, C::W, dev)) * 2 * C::Shape::PART * 4;
     return 0;
   });
   return kCounterBytes + parts;
@@ -200,51 +200,58 @@ long long decode_workspace(const w4a16_kv4_cache& c, const AttendPlan& p, const 
 
 int launch_decode(const w4a16_kv4_cache& c, const AttendParams& all, const AttendPlan& plan, int bf16, int row_limit,
                   void* workspace, const DeviceState& dev, cudaStream_t s) {
-  for (int b0 = 0; b0 < all.seqs; b0 += MAX_SEQS) {
-    DecodeParams p = {};
-    p.a = all;
-    p.a.seqs = std::min(all.seqs - b0, MAX_SEQS);
-    p.a.table += static_cast<long long>(b0) * all.width;
-    p.a.lens += b0;
-    if (p.a.cu_q) {
-      p.a.cu_q += b0;
-    } else if (all.seqs > MAX_SEQS) {     // uniform queries: this launch's own
-      const long long each = all.T / all.seqs;
-      p.a.q = static_cast<const uint16_t*>(all.q) + b0 * each * all.q_st;
-      p.a.o = static_cast<uint16_t*>(all.o) + b0 * each * all.heads * c.head_dim;
-      if (all.lse) p.a.lse = all.lse + b0 * each * all.heads;
-      p.a.T = static_cast<int>(each * p.a.seqs);
-    }
-    p.bf16 = bf16;
-    p.row_limit = row_limit;
-    p.wait_ns = g_wait_budget_ns.load(std::memory_order_relaxed);
-    p.counters = static_cast<int*>(workspace);
-    p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
-    const int nt = decode_nt(plan);
-    const int st = with_decode_config(c, nt, [&](auto cfg) {
-      using C = decltype(cfg);
-      const int tw = decode_team_warps(plan, C::W, dev);
-      if (dev.num_sms * (C::W / tw) > kCounterBytes / 4) return W4A16_ERR_DEVICE;
-      p.team_warps = tw;
-      p.seg_cost = tw;
-      p.teams = dev.num_sms * (C::W / tw);
-      auto k = C::kernel();
-      static std::atomic<uint64_t> ready{0};   // devices whose shared memory limit is set
-      int d = 0;
-      if (cudaGetDevice(&d) != cudaSuccess) return W4A16_ERR_DEVICE;
-      if (!(ready.load(std::memory_order_acquire) >> d & 1)) {
-        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::Shape::SMEM_BYTES) != cudaSuccess) {
-          cudaGetLastError();
-          return W4A16_ERR_LAUNCH;
-        }
-        ready.fetch_or(1ull << d, std::memory_order_release);
+  const int nt = decode_nt(plan);
+  return with_decode_config(c, nt, [&](auto cfg) {
+    using C = decltype(cfg);
+    const int tw = decode_team_warps(plan, C::W, dev);
+    if (dev.num_sms * (C::W / tw) > kCounterBytes / 4) return W4A16_ERR_DEVICE;
+    auto k = C::kernel();
+    static std::atomic<uint64_t> ready{0};   // devices whose shared memory limit is set
+    int d = 0;
+    if (cudaGetDevice(&d) != cudaSuccess) return W4A16_ERR_DEVICE;
+    if (!(ready.load(std::memory_order_acquire) >> d & 1)) {
+      if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::Shape::SMEM_BYTES) != cudaSuccess) {
+        cudaGetLastError();
+        return W4A16_ERR_LAUNCH;
       }
+      ready.fetch_or(1ull << d, std::memory_order_release);
+    }
+    // places in a launch's list of tiles fit 31 bits: as many sequences per launch as that allows
+    const long long row_tiles = (std::min<long long>(plan.rows, row_limit) + 8 * nt - 1) / (8 * nt);
+    const long long tiles = static_cast<long long>(all.width) * all.cache.page_size / (C::TB * BLK) + 1 + 3 * tw;
+    if (plan.kv_heads * row_tiles > 0x7fffffffLL / tiles) return W4A16_ERR_INVALID;
+    const int step = static_cast<int>(std::min<long long>(MAX_SEQS, 0x7fffffffLL / (plan.kv_heads * row_tiles * tiles)));
+    for (int b0 = 0; b0 < all.seqs; b0 += step) {
+      DecodeParams p = {};
+      p.a = all;
+      p.a.seqs = std::min(all.seqs - b0, step);
+      p.a.table += static_cast<long long>(b0) * all.width;
+      p.a.lens += b0;
+      if (p.a.cu_q) {
+        p.a.cu_q += b0;
+      } else if (p.a.seqs < all.seqs) {     // uniform queries: this launch's own
+        const long long each = all.T / all.seqs;
+        p.a.q = static_cast<const uint16_t*>(all.q) + b0 * each * all.q_st;
+        p.a.o = static_cast<uint16_t*>(all.o) + b0 * each * all.heads * c.head_dim;
+        if (all.lse) p.a.lse = all.lse + b0 * each * all.heads;
+        p.a.T = static_cast<int>(each * p.a.seqs);
+      }
+      p.bf16 = bf16;
+      p.row_limit = row_limit;
+      p.team_warps = tw;
+      // a piece's queries and end cost a team about what three tiles of each of its warps do (6 us
+      // where a tile takes 2)
+      p.seg_cost = 3 * tw;
+      p.teams = dev.num_sms * (C::W / tw);
+      p.wait_ns = g_wait_budget_ns.load(std::memory_order_relaxed);
+      p.counters = static_cast<int*>(workspace);
+      p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
       k<<<dev.num_sms, C::W * 32, C::Shape::SMEM_BYTES, s>>>(p);
-      return launched();
-    });
-    if (st != W4A16_OK) return st;
-  }
-  return W4A16_OK;
+      const int st = launched();
+      if (st != W4A16_OK) return st;
+    }
+    return static_cast<int>(W4A16_OK);
+  });
 }
 
 void launch_copy(const w4a16_kv4_cache& c, const int* src, const int* dst, const int* count, int n, const DeviceState& dev,

@@ -24,9 +24,11 @@
 //
 // Work: a segment is a kv head of a sequence (and a tile of 8 NT of its rows), a tile TB blocks
 // of 16 tokens. All tiles form one list that N teams of warps split evenly, whatever the lengths
-// (a segment counts `seg_cost` tiles more than it has, for its queries and its epilogue); a team that holds a part of a segment leaves (m, l, o) in the workspace and the last of the
-// segment's teams to arrive joins the parts in team order, so results do not depend on timing.
-// Each warp feeds itself: two stages of a tile, filled by bulk copies that its own lanes issue.
+// (a segment counts `seg_cost` tiles more than it has, for its queries and its epilogue); a team that holds a part of a segment leaves (m, l, o) in the workspace and, when all its
+// tiles are done, the last of the segment's teams to arrive joins the parts in team order, so
+// results do not depend on timing. Each warp feeds itself: two stages of a tile, filled by copies
+// that its own lane 0 issues. A piece's end passes through shared memory once: each warp leaves its
+// sums in the stage it has just read, and each then adds up some rows over all warps.
 #pragma once
 
 #include <type_traits>
@@ -96,33 +98,71 @@ struct DecodeShape {
   static constexpr int SETS = D / 64;                    // sets of 8 words per token
   static constexpr int BLOCK = block_bytes(D, NG);
   static constexpr int STAGE = TB * BLOCK;
-  static constexpr int ACC = SETS * 16 * NT;             // accumulators per lane
-  static constexpr int STATE = (ACC + (4 + 2 * NG) * NT) * 32;   // floats of a warp's state
+  static constexpr int R4 = NT * SETS * 4;               // rows of 32 float4: a warp's (or team's) sums
+  static constexpr int SMALL = 8 * NT * (2 + NG);        // and for each query row m, l, corr [NG]
+  static constexpr int PART = R4 * 128 + SMALL;          // floats of a part in the workspace
   static constexpr int RING_BYTES = W * 2 * STAGE;
-  static constexpr int MERGE_BYTES = W / 2 * STATE * 4;
-  static constexpr int SMEM_BYTES = RING_BYTES + MERGE_BYTES + (MAX_SEQS + 1) * 8 + W * 2 * 8 + W * 8 + 64;
-  static_assert(STAGE % 16 == 0 && SMEM_BYTES <= 227 * 1024, "shared memory budget");
+  static constexpr int SMEM_BYTES = RING_BYTES + W * SMALL * 4 + MAX_SEQS * 16 + W * 2 * 8 + W * 16 + 64;
+  static_assert(STAGE % 16 == 0 && STAGE >= R4 * 512, "a stage holds a warp's sums");
+  static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+};
+
+// A sequence as the list of tiles has it: where its tiles begin, its queries (none: it has no tile in
+// this launch) and cached tokens.
+struct Sequence {
+  int prefix, first, count, len;
 };
 
 struct Segment {
-  long long start;         // its first tile's place in the list (after the seg_cost places without a tile)
+  int start;               // its first tile's place in the list (after the seg_cost places without a tile)
   int n;                   // its tiles
   int b, kh, rt;           // sequence, kv head, row tile
   int first, count, len;   // the sequence's queries and cached tokens
   int tile0;               // the sequence's first tile some query sees
 };
 
+// Waits for a copy that takes longer than a try; whatever happens, not without it.
+__device__ __noinline__ void wait_for_copy(uint64_t* bar, uint32_t parity, uint64_t budget_ns) {
+  if (!mbar_wait(bar, parity, budget_ns)) mbar_wait(bar, parity, kWaitBudgetNs);
+}
+
+// Row i of a segment's sums, divided and rounded: channels 8 (r + 8 set) + j and + 4 of query rows
+// 2 q4 and 2 q4 + 1 of row tile nt, i = (nt SETS + set) 4 + j.
+template <int D, int NG, int NT>
+__device__ __forceinline__ void finish_row(const DecodeParams& p, const Segment& s, int i, int r, int q4, const float4& v,
+                                           const float (&mm)[2], const float (&ll)[2], const float (&cc)[2][NG]) {
+  constexpr int SETS = D / 64;
+  const AttendParams& a = p.a;
+  const int nt = i / (SETS * 4), set = i / 4 % SETS, j = i % 4;
+  const float by = (j & 1) ? 1048576.0f : 16777216.0f;     // codes are c 2^-24, 16 c 2^-24 where j is odd
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int row = s.rt * 8 * NT + nt * 8 + 2 * q4 + c;
+    if (row >= s.count * a.share) continue;
+    const float inv = ll[c] == 0.0f ? 0.0f : 1.0f / ll[c];
+    const float add = NG == 1 || set == 0 ? cc[c][0] : cc[c][NG - 1];
+    const float y0 = ((c ? v.y : v.x) * by + add) * inv, y1 = ((c ? v.w : v.z) * by + add) * inv;
+    const long long at = static_cast<long long>(s.first + row / a.share) * a.heads + s.kh * a.share + row % a.share;
+    const uint32_t both = p.bf16 ? pack2<__nv_bfloat16>(y0, y1) : pack2<__half>(y0, y1);
+    uint16_t* o = static_cast<uint16_t*>(a.o) + at * D + 8 * (r + 8 * set) + j;
+    o[0] = static_cast<uint16_t>(both);
+    o[4] = static_cast<uint16_t>(both >> 16);
+    if (a.lse && r == 0 && set == 0 && j == 0) a.lse[at] = ll[c] == 0.0f ? -INFINITY : (mm[c] + log2f(ll[c])) * kLn2;
+  }
+}
+
 template <int D, int NG, int NT, int W, int TB>
 __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParams p) {
   using SH = DecodeShape<D, NG, NT, W, TB>;
   constexpr int ROWS = 8 * NT, TT = TB * BLK, SETS = SH::SETS;
+  constexpr int R4 = SH::R4, SMALL = SH::SMALL;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* ring = smem;
-  float* merge = reinterpret_cast<float*>(smem + SH::RING_BYTES);
-  long long* prefix = reinterpret_cast<long long*>(smem + SH::RING_BYTES + SH::MERGE_BYTES);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(prefix + MAX_SEQS + 1);
-  long long* scan = reinterpret_cast<long long*>(bars + 2 * W);
-  int* last_flag = reinterpret_cast<int*>(scan);         // one per team, after the prefix sums are done
+  float* smalls = reinterpret_cast<float*>(smem + SH::RING_BYTES);
+  Sequence* seqs = reinterpret_cast<Sequence*>(smalls + W * SMALL);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(seqs + MAX_SEQS);
+  int* scan = reinterpret_cast<int*>(bars + 2 * W);
+  int* flags = scan + W;                                 // two per team, then each warp's stage with its sums
 
   const AttendParams& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -134,88 +174,87 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     mbar_fence_init();
   }
 
-  // a sequence's tiles and how many segments have them
-  auto extent = [&](int b, Segment& s) {
-    sequence(a, b, s.first, s.count, s.len);
-    s.b = b;
-    const int rows = s.count * a.share;
-    s.tile0 = 0;
-    s.n = 0;
-    if (rows == 0 || rows > p.row_limit) return 0;
-    const int from = a.window ? max(0, s.len - s.count - a.window + 1) : 0;
-    s.tile0 = from / TT;
-    s.n = max(0, (s.len + TT - 1) / TT - s.tile0);
-    return a.cache.kv_heads * ((rows + ROWS - 1) / ROWS);
-  };
+  // the first tile that some query of a sequence sees, how many there are, and its segments
+  auto tile0_of = [&](int count, int len) { return a.window ? max(0, len - count - a.window + 1) / TT : 0; };
+  auto tiles_of = [&](int count, int len) { return count ? max(0, (len + TT - 1) / TT - tile0_of(count, len)) : 0; };
+  auto segments_of = [&](int count) { return a.cache.kv_heads * ((count * a.share + ROWS - 1) / ROWS); };
 
   // prefix sums of the sequences' tiles
-  long long total = 0;
+  int total = 0;
   for (int base = 0; base < a.seqs; base += W * 32) {
     const int b = base + threadIdx.x;
-    Segment s;
-    long long v = 0;
+    Sequence q = {0, 0, 0, 0};
+    int v = 0;
     if (b < a.seqs) {
-      const long long h = extent(b, s);
-      v = s.n ? h * (s.n + p.seg_cost) : 0;
+      sequence(a, b, q.first, q.count, q.len);
+      if (static_cast<long long>(q.count) * a.share > p.row_limit) q.count = 0;
+      const int n = tiles_of(q.count, q.len);
+      v = n ? segments_of(q.count) * (n + p.seg_cost) : 0;
     }
-    long long inc = v;
+    int inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+      const int x = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += x;
     }
-    __syncthreads();
+    if (base) __syncthreads();
     if (lane == 31) scan[warp] = inc;
     __syncthreads();
-    long long before = total;
+    q.prefix = total + inc - v;
+#pragma unroll
     for (int w = 0; w < W; ++w) {
-      const long long x = scan[w];
-      if (w < warp) before += x;
+      const int x = scan[w];
+      if (w < warp) q.prefix += x;
       total += x;
     }
-    if (b < a.seqs) prefix[b] = before + inc - v;
+    if (b < a.seqs) seqs[b] = q;
   }
-  if (threadIdx.x == 0) prefix[a.seqs] = total;
   __syncthreads();
 
   const int TW = p.team_warps, team_in_cta = warp / TW, wt = warp % TW;
   const int team = blockIdx.x * (W / TW) + team_in_cta;
-  const int barrier = 1 + team_in_cta;
   auto team_sync = [&]() {
     if (TW == 1) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(TW * 32) : "memory");
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + team_in_cta), "r"(TW * 32) : "memory");
   };
 
   // sequences without a tile: their queries see nothing
   for (int b = team; b < a.seqs; b += p.teams) {
-    if (prefix[b + 1] != prefix[b]) continue;
-    Segment s;
-    if (extent(b, s) == 0) continue;
-    const long long rows = static_cast<long long>(s.count) * a.heads;
-    uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + static_cast<long long>(s.first) * a.heads * D);
+    const Sequence q = seqs[b];
+    if (q.count == 0 || tiles_of(q.count, q.len) != 0) continue;
+    const long long rows = static_cast<long long>(q.count) * a.heads, at = static_cast<long long>(q.first) * a.heads;
+    uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + at * D);
     for (long long i = wt * 32 + lane; i < rows * (D / 8); i += TW * 32) o[i] = make_uint4(0, 0, 0, 0);
     if (a.lse)
-      for (long long i = wt * 32 + lane; i < rows; i += TW * 32)
-        a.lse[static_cast<long long>(s.first) * a.heads + i] = -INFINITY;
+      for (long long i = wt * 32 + lane; i < rows; i += TW * 32) a.lse[at + i] = -INFINITY;
   }
 
-  // the team's share of the list: no more teams than give each warp a tile
-  const long long N = min(static_cast<long long>(p.teams), (total + TW - 1) / TW);
+  // The team's share [t0, t1) of the list: no more teams than give each warp a tile; the first
+  // `more` teams have one place more than the others.
+  const int N = min(p.teams, (total + TW - 1) / TW);
   if (team >= N) return;
-  const long long t0 = total * team / N, t1 = total * (team + 1) / N;
+  const int each = total / N, more = total - each * N;
+  const int t0 = team * each + min(team, more), t1 = t0 + each + (team < more ? 1 : 0);
+  auto team_of = [&](int t) { return t < more * (each + 1) ? t / (each + 1) : more + (t - more * (each + 1)) / each; };
 
-  auto locate = [&](long long t) {
-    int lo = 0, hi = a.seqs - 1;   // last b with prefix[b] <= t: the one that holds t
+  auto locate = [&](int t) {
+    int lo = 0, hi = a.seqs - 1;   // last b with prefix <= t: the one that holds t
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (prefix[mid] <= t) lo = mid; else hi = mid - 1;
+      if (seqs[mid].prefix <= t) lo = mid; else hi = mid - 1;
     }
+    const Sequence q = seqs[lo];
     Segment s;
-    extent(lo, s);
-    const int seg = static_cast<int>((t - prefix[lo]) / (s.n + p.seg_cost));
-    s.kh = seg % a.cache.kv_heads;
+    s.b = lo;
+    s.first = q.first;
+    s.count = q.count;
+    s.len = q.len;
+    s.tile0 = tile0_of(q.count, q.len);
+    s.n = tiles_of(q.count, q.len);
+    const int seg = (t - q.prefix) / (s.n + p.seg_cost);
     s.rt = seg / a.cache.kv_heads;
-    s.start = prefix[lo] + static_cast<long long>(seg) * (s.n + p.seg_cost) + p.seg_cost;
+    s.kh = seg - s.rt * a.cache.kv_heads;
+    s.start = q.prefix + seg * (s.n + p.seg_cost) + p.seg_cost;
     return s;
   };
 
@@ -226,7 +265,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
   uint64_t* bar = &bars[2 * warp];
   const bool whole_tiles = a.cache.page_blocks % TB == 0;
   const int per_tile = whole_tiles ? 1 : TB;
-  long long pt = t0 + wt;              // the next tile to copy
+  int pt = t0 + wt;                    // the next tile to copy
   int pleft = 0, ptaken = 32;          // tiles of its segment left for this warp, and sources used
   int pblk = 0, plast = 0;             // its first block, and the sequence's blocks
   const int* prow = nullptr;           // the sequence's row of the table
@@ -241,8 +280,8 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
         if (pt >= s.start + s.n) continue;
       }
       if (pt >= t1) break;
-      pleft = static_cast<int>((min(t1, s.start + s.n) - pt + TW - 1) / TW);
-      pblk = (s.tile0 + static_cast<int>(pt - s.start)) * TB;
+      pleft = (min(t1, s.start + s.n) - pt + TW - 1) / TW;
+      pblk = (s.tile0 + pt - s.start) * TB;
       plast = (s.len + BLK - 1) / BLK;
       prow = a.table + static_cast<long long>(s.b) * a.width;
       phead = a.cache.pool + s.kh * a.cache.page_bytes;
@@ -298,13 +337,13 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
   const bool odd = q4 & 1;
   const uint32_t sel_lo = odd ? 0x1054u : 0x5410u, sel_hi = odd ? 0x3276u : 0x7632u;
 
-  for (long long t = t0; t < t1;) {
+  for (int t = t0; t < t1;) {
     const Segment s = locate(t);
     if (t < s.start) {
       t = s.start;
       if (t >= t1) break;
     }
-    const long long end = min(t1, s.start + s.n);
+    const int end = min(t1, s.start + s.n);
 
     // ---- the rows' queries as B fragments, their sums, and what a score is scaled by
     uint32_t qf[NT][KW][4];
@@ -403,9 +442,8 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
       }
 
     // this warp's tiles of the piece: those at t0 + wt + k TW
-    int g = static_cast<int>(t - t0);
-    g = static_cast<int>(t - s.start) + ((wt - g) & (TW - 1));
-    const int stop = static_cast<int>(end - s.start);
+    int g = t - s.start + ((wt - (t - t0)) & (TW - 1));
+    const int stop = end - s.start;
     // tiles [inside_lo, inside_hi) of the segment lie within what every row sees
     const int inside_lo = (all_from + TT - 1) / TT - s.tile0, inside_hi = all_to / TT - s.tile0;
     const uint32_t lane_k = (NG == 1 && KW == 4) ? r * (D / 2) + 16 * q4 : r * (D / 2);
@@ -587,10 +625,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     for (; g < stop; g += TW) {
       const unsigned blocks = (stage ? have >> 8 : have) & 0xffu;
       issue(stage ^ 1);
-      if (!mbar_try_wait(&bar[stage], (phases >> stage) & 1u)) {
-        if (!mbar_wait(&bar[stage], (phases >> stage) & 1u, p.wait_ns))
-          mbar_wait(&bar[stage], (phases >> stage) & 1u, kWaitBudgetNs);   // never leave with a copy in flight
-      }
+      if (!mbar_try_wait(&bar[stage], (phases >> stage) & 1u)) wait_for_copy(&bar[stage], (phases >> stage) & 1u, p.wait_ns);
       phases ^= 1u << stage;
       const uint8_t* tile = stages + stage * SH::STAGE;
       if (blocks == (1u << TB) - 1u && g >= inside_lo && g < inside_hi)
@@ -621,157 +656,151 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
         for (int i = 0; i < NG; ++i) corr[nt][c][i] = fmaf(-7.5f, hsum[nt][i][c], corr[nt][c][i]);
       }
 
-    // a warp's state in memory: float4 [ACC / 4][32], then m, l, corr [NT][2] as [...][32]
-    auto put = [&](float* to_) {
-      float4* q = reinterpret_cast<float4*>(to_) + lane;
-      float* e = to_ + SH::ACC * 32 + lane;
+    // ---- the warp's sums into the stage it has just read, the rest beside
+    {
+      float4* sums = reinterpret_cast<float4*>(stages + (stage ^ 1) * SH::STAGE) + lane;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int i = 0; i < SETS * 4; ++i) q[(nt * SETS * 4 + i) * 32] = make_float4(acc[nt][i][0], acc[nt][i][1], acc[nt][i][2], acc[nt][i][3]);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          e[((nt * 2 + c) * (2 + NG)) * 32] = m[nt][c];
-          e[((nt * 2 + c) * (2 + NG) + 1) * 32] = l[nt][c];
-#pragma unroll
-          for (int i = 0; i < NG; ++i) e[((nt * 2 + c) * (2 + NG) + 2 + i) * 32] = corr[nt][c][i];
-        }
-      }
-    };
-    // ---- the team's warps, by halves
-    for (int half = TW / 2; half > 0; half >>= 1) {
-      float* slot = merge + (team_in_cta * (TW / 2) + (wt & (half - 1))) * SH::STATE;
-      if (wt >= half && wt < 2 * half) put(slot);
-      team_sync();
-      if (wt < half) {
-        const float4* q = reinterpret_cast<const float4*>(slot) + lane;
-        const float* e = slot + SH::ACC * 32 + lane;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float mine[2], theirs[2];
+        for (int i = 0; i < SETS * 4; ++i)
+          sums[(nt * SETS * 4 + i) * 32] = make_float4(acc[nt][i][0], acc[nt][i][1], acc[nt][i][2], acc[nt][i][3]);
+        if (r == 0) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float* ec = e + ((nt * 2 + c) * (2 + NG)) * 32;
-            const float mo = ec[0], mn = fmaxf(m[nt][c], mo);
-            mine[c] = ex2(m[nt][c] - mn);
-            theirs[c] = ex2(mo - mn);
-            m[nt][c] = mn;
-            l[nt][c] = l[nt][c] * mine[c] + ec[32] * theirs[c];
+            float* e = smalls + warp * SMALL + (nt * 8 + 2 * q4 + c) * (2 + NG);
+            e[0] = m[nt][c];
+            e[1] = l[nt][c];
 #pragma unroll
-            for (int i = 0; i < NG; ++i) corr[nt][c][i] = corr[nt][c][i] * mine[c] + ec[(2 + i) * 32] * theirs[c];
-          }
-#pragma unroll
-          for (int i = 0; i < SETS * 4; ++i) {
-            const float4 v = q[(nt * SETS * 4 + i) * 32];
-            acc[nt][i][0] = acc[nt][i][0] * mine[0] + v.x * theirs[0];
-            acc[nt][i][1] = acc[nt][i][1] * mine[1] + v.y * theirs[1];
-            acc[nt][i][2] = acc[nt][i][2] * mine[0] + v.z * theirs[0];
-            acc[nt][i][3] = acc[nt][i][3] * mine[1] + v.w * theirs[1];
+            for (int i = 0; i < NG; ++i) e[2 + i] = corr[nt][c][i];
           }
         }
       }
-      team_sync();
+      if (lane == 0) flags[2 * W + warp] = stage ^ 1;
     }
-
-    // one set of eight channels per lane (word r + 8 set) of rows 2 q4 and 2 q4 + 1 of row tile nt:
-    // v[j] the accumulators of nibble pair (j, j + 4)
-    auto emit = [&](int nt, int set, const float (&v)[4][4], const float (&ml)[2], const float (&ll)[2], const float (&cc)[2]) {
+    team_sync();
+    // ---- row i of the sums over the team's warps: finished, or left as a part
+    const bool whole = end - t == s.n;
+    float* part = p.parts + (2 * team + (t0 >= s.start ? 0 : 1)) * static_cast<long long>(SH::PART);
+    for (int i = wt; i < R4; i += TW) {
+      const int col = i / (SETS * 4) * 8 + 2 * q4;
+      const float* e = smalls + team_in_cta * TW * SMALL + col * (2 + NG);
+      float mm[2] = {kNoMax, kNoMax}, ll[2] = {0.0f, 0.0f}, cc[2][NG] = {};
+      for (int w = 0; w < TW; ++w) {
+        mm[0] = fmaxf(mm[0], e[w * SMALL]);
+        mm[1] = fmaxf(mm[1], e[w * SMALL + 2 + NG]);
+      }
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int w = 0; w < TW; ++w) {
+        float by[2];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int row = s.rt * ROWS + nt * 8 + 2 * q4 + c;
-        if (row >= s.count * a.share) continue;
-        const float inv = ll[c] == 0.0f ? 0.0f : 1.0f / ll[c];
-        float y[8];
+        for (int c = 0; c < 2; ++c) {
+          const float* ec = e + w * SMALL + c * (2 + NG);
+          by[c] = ex2(ec[0] - mm[c]);
+          ll[c] = fmaf(by[c], ec[1], ll[c]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float by = (j & 1) ? 1048576.0f : 16777216.0f;
-          y[j] = (v[j][c] * by + cc[c]) * inv;
-          y[j + 4] = (v[j][c + 2] * by + cc[c]) * inv;
+          for (int k = 0; k < NG; ++k) cc[c][k] = fmaf(by[c], ec[2 + k], cc[c][k]);
         }
-        uint4 o;
-        uint32_t* ov = &o.x;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          ov[j] = p.bf16 ? pack2<__nv_bfloat16>(y[2 * j], y[2 * j + 1]) : pack2<__half>(y[2 * j], y[2 * j + 1]);
-        const long long at = static_cast<long long>(s.first + row / a.share) * a.heads + s.kh * a.share + row % a.share;
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + at * D + 8 * (r + 8 * set)) = o;
-        if (a.lse && r == 0 && set == 0) a.lse[at] = ll[c] == 0.0f ? -INFINITY : (ml[c] + log2f(ll[c])) * kLn2;
+        const int from_warp = team_in_cta * TW + w;
+        const float4 x = *(reinterpret_cast<const float4*>(ring + (2 * from_warp + flags[2 * W + from_warp]) * SH::STAGE) + i * 32 + lane);
+        v.x = fmaf(by[0], x.x, v.x);
+        v.y = fmaf(by[1], x.y, v.y);
+        v.z = fmaf(by[0], x.z, v.z);
+        v.w = fmaf(by[1], x.w, v.w);
       }
-    };
-    if (end - t == s.n) {
-      if (wt == 0) {
+      if (whole) {
+        finish_row<D, NG, NT>(p, s, i, r, q4, v, mm, ll, cc);
+      } else {
+        reinterpret_cast<float4*>(part)[i * 32 + lane] = v;
+        if (i % (SETS * 4) == 0 && r == 0) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int c = 0; c < 2; ++c) {
+            float* ec = part + R4 * 128 + (col + c) * (2 + NG);
+            ec[0] = mm[c];
+            ec[1] = ll[c];
 #pragma unroll
-          for (int set = 0; set < SETS; ++set) {
-            const float cc[2] = {corr[nt][0][NG == 1 ? 0 : set], corr[nt][1][NG == 1 ? 0 : set]};
-            float v[4][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) v[j][c] = acc[nt][4 * set + j][c];
-            emit(nt, set, v, m[nt], l[nt], cc);
+            for (int k = 0; k < NG; ++k) ec[2 + k] = cc[c][k];
           }
-      }
-    } else {
-      // ---- a part of the segment: leave it, and join the parts if this team is the last
-      const long long first_team = ((s.start + 1) * N - 1) / total, last_team = ((s.start + s.n) * N - 1) / total;
-      if (wt == 0) {
-        put(p.parts + (2 * team + (t0 >= s.start ? 0 : 1)) * static_cast<long long>(SH::STATE));
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) {
-          const int n = atomicAdd(p.counters + first_team, 1);
-          const int last = n == static_cast<int>(last_team - first_team);
-          if (last) p.counters[first_team] = 0;     // every team has arrived: left zero for the next launch
-          last_flag[team_in_cta] = last;
-        }
-      }
-      team_sync();
-      const bool last = last_flag[team_in_cta] != 0;
-      team_sync();
-      if (last) {
-        __threadfence();
-        for (int i = wt; i < NT * SETS; i += TW) {
-          const int nt = i / SETS, set = i % SETS;
-          // a team's part of this segment is its first unless the segment starts inside its range
-          auto part = [&](long long tm) {
-            return p.parts + (2 * tm + (total * tm / N >= s.start ? 0 : 1)) * SH::STATE;
-          };
-          float mm[2] = {kNoMax, kNoMax};
-          for (long long tm = first_team; tm <= last_team; ++tm) {
-            const float* e = part(tm) + SH::ACC * 32 + lane + nt * 2 * (2 + NG) * 32;
-            mm[0] = fmaxf(mm[0], __ldcg(e));
-            mm[1] = fmaxf(mm[1], __ldcg(e + (2 + NG) * 32));
-          }
-          float v[4][4] = {}, ll[2] = {0.0f, 0.0f}, cc[2] = {0.0f, 0.0f};
-#pragma unroll 4
-          for (long long tm = first_team; tm <= last_team; ++tm) {
-            const float* base = part(tm);
-            const float* e = base + SH::ACC * 32 + lane + nt * 2 * (2 + NG) * 32;
-            float by[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const float* ec = e + c * (2 + NG) * 32;
-              by[c] = ex2(__ldcg(ec) - mm[c]);
-              ll[c] += by[c] * __ldcg(ec + 32);
-              cc[c] += by[c] * __ldcg(ec + (2 + (NG == 1 ? 0 : set)) * 32);
-            }
-            const float4* q = reinterpret_cast<const float4*>(base) + lane + (nt * SETS + set) * 4 * 32;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float4 w = __ldcg(q + j * 32);
-              v[j][0] += by[0] * w.x;
-              v[j][1] += by[1] * w.y;
-              v[j][2] += by[0] * w.z;
-              v[j][3] += by[1] * w.w;
-            }
-          }
-          emit(nt, set, v, mm, ll, cc);
         }
       }
     }
+    fence_proxy_async_smem();   // the stages are copied into again
+    team_sync();
     t = end;
+  }
+
+  // ---- parts: the segment the team starts in, and the one it ends in
+  auto shared_segment = [&](int k, Segment& s) {
+    s = locate(k ? t1 - 1 : t0);
+    if (k ? s.start <= t0 || s.start >= t1 : s.start > t0) return false;
+    return s.start < t0 || s.start + s.n > t1;
+  };
+  {
+    __threadfence();
+    team_sync();
+    if (wt == 0 && lane < 2) {
+      Segment s;
+      int last = 0;
+      if (shared_segment(lane, s)) {
+        const int first = team_of(s.start), all = team_of(s.start + s.n - 1) - first;
+        last = atomicAdd(p.counters + first, 1) == all;
+        if (last) p.counters[first] = 0;     // every team has arrived: left zero for the next launch
+      }
+      flags[2 * team_in_cta + lane] = last;
+    }
+    team_sync();
+  }
+  for (int k = 0; k < 2; ++k) {
+    if (!flags[2 * team_in_cta + k]) continue;
+    __threadfence();
+    Segment s;
+    shared_segment(k, s);
+    const int first = team_of(s.start), count = team_of(s.start + s.n - 1) - first + 1;
+    const int first_t0 = first * each + min(first, more);
+    // the first team's part is its second unless its own share starts at the segment's
+    const float* part0 = p.parts + (2 * first + (first_t0 >= s.start ? 0 : 1)) * static_cast<long long>(SH::PART);
+    const float* rest = p.parts + 2 * first * static_cast<long long>(SH::PART);
+    // RUN rows at a time, which share the query rows' m, l and corr; the maximum runs along, so that
+    // all loads of four parts are in flight together
+    constexpr int RUN = 4;
+    const int rows = max(1, R4 / TW);
+    for (int i0 = wt * rows; i0 < min(R4, (wt + 1) * rows); i0 += RUN) {
+      const int col = i0 / (SETS * 4) * 8 + 2 * q4, n = min(RUN, rows);
+      float mm[2] = {kNoMax, kNoMax}, ll[2] = {0.0f, 0.0f}, cc[2][NG] = {};
+      float4 v[RUN];
+#pragma unroll
+      for (int j = 0; j < RUN; ++j) v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+      for (int w = 0; w < count; ++w) {
+        const float* base = w ? rest + 2 * w * static_cast<long long>(SH::PART) : part0;
+        const float* e = base + R4 * 128 + col * (2 + NG);
+        float4 x[RUN];
+#pragma unroll
+        for (int j = 0; j < RUN; ++j)
+          x[j] = j < n ? __ldcg(reinterpret_cast<const float4*>(base) + (i0 + j) * 32 + lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float mine[2], theirs[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float* ec = e + c * (2 + NG);
+          const float mo = __ldcg(ec), mn = fmaxf(mm[c], mo);
+          mine[c] = ex2(mm[c] - mn);
+          theirs[c] = ex2(mo - mn);
+          mm[c] = mn;
+          ll[c] = fmaf(theirs[c], __ldcg(ec + 1), ll[c] * mine[c]);
+#pragma unroll
+          for (int j = 0; j < NG; ++j) cc[c][j] = fmaf(theirs[c], __ldcg(ec + 2 + j), cc[c][j] * mine[c]);
+        }
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) {
+          v[j].x = fmaf(theirs[0], x[j].x, v[j].x * mine[0]);
+          v[j].y = fmaf(theirs[1], x[j].y, v[j].y * mine[1]);
+          v[j].z = fmaf(theirs[0], x[j].z, v[j].z * mine[0]);
+          v[j].w = fmaf(theirs[1], x[j].w, v[j].w * mine[1]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < RUN; ++j)
+        if (j < n) finish_row<D, NG, NT>(p, s, i0 + j, r, q4, v[j], mm, ll, cc);
+    }
   }
 }
 
