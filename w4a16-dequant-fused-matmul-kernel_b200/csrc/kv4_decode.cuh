@@ -26,7 +26,9 @@
 // of 16 tokens. All tiles form one list that N teams of warps split evenly, whatever the lengths
 // (a segment counts `seg_cost` tiles more than it has, for its queries and its epilogue); a team that holds a part of a segment leaves (m, l, o) in the workspace and, when all its
 // tiles are done, the last of the segment's teams to arrive joins the parts in team order, so
-// results do not depend on timing. Each warp feeds itself: two stages of a tile, filled by copies
+// results do not depend on timing. (Where there are teams enough and every segment is short, each
+// team takes one whole segment: joining parts costs about 5 us, eight tiles of each warp.) Each warp
+// feeds itself: two stages of a tile, filled by copies
 // that its own lane 0 issues. A piece's end passes through shared memory once: each warp leaves its
 // sums in the stage it has just read, and each then adds up some rows over all warps.
 #pragma once
@@ -102,16 +104,17 @@ struct DecodeShape {
   static constexpr int SMALL = 8 * NT * (2 + NG);        // and for each query row m, l, corr [NG]
   static constexpr int PART = R4 * 128 + SMALL;          // floats of a part in the workspace
   static constexpr int RING_BYTES = W * 2 * STAGE;
-  static constexpr int SMEM_BYTES = RING_BYTES + W * SMALL * 4 + MAX_SEQS * 16 + W * 2 * 8 + W * 16 + 64;
+  static constexpr int SMEM_BYTES = RING_BYTES + W * SMALL * 4 + MAX_SEQS * 20 + 16 + W * 2 * 8 + W * 16 + 64;
   static_assert(STAGE % 16 == 0 && STAGE >= R4 * 512, "a stage holds a warp's sums");
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
 };
 
-// A sequence as the list of tiles has it: where its tiles begin, its queries (none: it has no tile in
-// this launch) and cached tokens.
+// A sequence as the list of tiles has it: where its tiles and its segments begin, its queries (none:
+// it has no tile in this launch) and cached tokens.
 struct Sequence {
-  int prefix, first, count, len;
+  int prefix, segments, first, count, len;
 };
+constexpr int kWholeTiles = 8;             // a segment of at most so many tiles per warp is one team's
 
 struct Segment {
   int start;               // its first tile's place in the list (after the seg_cost places without a tile)
@@ -160,9 +163,9 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
   uint8_t* ring = smem;
   float* smalls = reinterpret_cast<float*>(smem + SH::RING_BYTES);
   Sequence* seqs = reinterpret_cast<Sequence*>(smalls + W * SMALL);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(seqs + MAX_SEQS);
-  int* scan = reinterpret_cast<int*>(bars + 2 * W);
-  int* flags = scan + W;                                 // two per team, then each warp's stage with its sums
+  uint64_t* bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(seqs + MAX_SEQS) + 15) & ~static_cast<uintptr_t>(15));
+  unsigned long long* scan = reinterpret_cast<unsigned long long*>(bars + 2 * W);
+  int* flags = reinterpret_cast<int*>(scan);             // two per team, then each warp's stage with its sums
 
   const AttendParams& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -179,39 +182,49 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
   auto tiles_of = [&](int count, int len) { return count ? max(0, (len + TT - 1) / TT - tile0_of(count, len)) : 0; };
   auto segments_of = [&](int count) { return a.cache.kv_heads * ((count * a.share + ROWS - 1) / ROWS); };
 
-  // prefix sums of the sequences' tiles
-  int total = 0;
+  const int TW = p.team_warps;
+  // prefix sums of the sequences' tiles (low half) and segments (high half)
+  unsigned long long sums = 0;
+  bool longer = false;               // some segment is longer than one team should take
   for (int base = 0; base < a.seqs; base += W * 32) {
     const int b = base + threadIdx.x;
-    Sequence q = {0, 0, 0, 0};
-    int v = 0;
+    Sequence q = {0, 0, 0, 0, 0};
+    unsigned long long v = 0;
+    bool more = false;
     if (b < a.seqs) {
       sequence(a, b, q.first, q.count, q.len);
       if (static_cast<long long>(q.count) * a.share > p.row_limit) q.count = 0;
       const int n = tiles_of(q.count, q.len);
-      v = n ? segments_of(q.count) * (n + p.seg_cost) : 0;
+      if (n) {
+        const unsigned h = segments_of(q.count);
+        v = (static_cast<unsigned long long>(h) << 32) | h * (n + p.seg_cost);
+      }
+      more = n > kWholeTiles * TW;
     }
-    int inc = v;
+    unsigned long long inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, inc, o);
+      const unsigned long long x = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += x;
     }
     if (base) __syncthreads();
     if (lane == 31) scan[warp] = inc;
-    __syncthreads();
-    q.prefix = total + inc - v;
+    longer |= __syncthreads_or(more) != 0;
+    unsigned long long before = sums + inc - v;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const int x = scan[w];
-      if (w < warp) q.prefix += x;
-      total += x;
+      const unsigned long long x = scan[w];
+      if (w < warp) before += x;
+      sums += x;
     }
+    q.prefix = static_cast<int>(before);
+    q.segments = static_cast<int>(before >> 32);
     if (b < a.seqs) seqs[b] = q;
   }
   __syncthreads();
+  const int total = static_cast<int>(sums), segments = static_cast<int>(sums >> 32);
 
-  const int TW = p.team_warps, team_in_cta = warp / TW, wt = warp % TW;
+  const int team_in_cta = warp / TW, wt = warp % TW;
   const int team = blockIdx.x * (W / TW) + team_in_cta;
   auto team_sync = [&]() {
     if (TW == 1) __syncwarp();
@@ -231,17 +244,18 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
 
   // The team's share [t0, t1) of the list: no more teams than give each warp a tile; the first
   // `more` teams have one place more than the others.
-  const int N = min(p.teams, (total + TW - 1) / TW);
+  const bool direct = !longer && segments <= p.teams;    // or team i takes segment i
+  const int N = direct ? segments : min(p.teams, (total + TW - 1) / TW);
   if (team >= N) return;
   const int each = total / N, more = total - each * N;
-  const int t0 = team * each + min(team, more), t1 = t0 + each + (team < more ? 1 : 0);
+  int t0 = team * each + min(team, more), t1 = t0 + each + (team < more ? 1 : 0);
   auto team_of = [&](int t) { return t < more * (each + 1) ? t / (each + 1) : more + (t - more * (each + 1)) / each; };
 
   auto locate = [&](int t) {
-    int lo = 0, hi = a.seqs - 1;   // last b with prefix <= t: the one that holds t
+    int lo = 0, hi = a.seqs - 1;   // last b that begins at or before t: the one that holds t
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (seqs[mid].prefix <= t) lo = mid; else hi = mid - 1;
+      if ((direct ? seqs[mid].segments : seqs[mid].prefix) <= (direct ? team : t)) lo = mid; else hi = mid - 1;
     }
     const Sequence q = seqs[lo];
     Segment s;
@@ -251,12 +265,16 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     s.len = q.len;
     s.tile0 = tile0_of(q.count, q.len);
     s.n = tiles_of(q.count, q.len);
-    const int seg = (t - q.prefix) / (s.n + p.seg_cost);
+    const int seg = direct ? team - q.segments : (t - q.prefix) / (s.n + p.seg_cost);
     s.rt = seg / a.cache.kv_heads;
     s.kh = seg - s.rt * a.cache.kv_heads;
-    s.start = q.prefix + seg * (s.n + p.seg_cost) + p.seg_cost;
+    s.start = direct ? 0 : q.prefix + seg * (s.n + p.seg_cost) + p.seg_cost;
     return s;
   };
+  if (direct) {
+    t0 = 0;
+    t1 = locate(0).n;
+  }
 
   // ------------------------------ this warp's copies ------------------------------
   // A tile arrives with one copy where it lies in one page (`whole_tiles`), else block by block. The
@@ -337,6 +355,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
   const bool odd = q4 & 1;
   const uint32_t sel_lo = odd ? 0x1054u : 0x5410u, sel_hi = odd ? 0x3276u : 0x7632u;
 
+  bool parts = false;         // some piece was part of a segment
   for (int t = t0; t < t1;) {
     const Segment s = locate(t);
     if (t < s.start) {
@@ -680,6 +699,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     team_sync();
     // ---- row i of the sums over the team's warps: finished, or left as a part
     const bool whole = end - t == s.n;
+    parts |= !whole;
     float* part = p.parts + (2 * team + (t0 >= s.start ? 0 : 1)) * static_cast<long long>(SH::PART);
     for (int i = wt; i < R4; i += TW) {
       const int col = i / (SETS * 4) * 8 + 2 * q4;
@@ -734,6 +754,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     if (k ? s.start <= t0 || s.start >= t1 : s.start > t0) return false;
     return s.start < t0 || s.start + s.n > t1;
   };
+  if (!parts) return;
   {
     __threadfence();
     team_sync();

@@ -13,7 +13,6 @@ An index the device finds out of range (a position, slot, page or row) is skippe
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 from torch import Tensor
@@ -27,6 +26,7 @@ _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
 _CODES = {torch.float16: _lib.DTYPE_CODES[torch.float16], torch.bfloat16: _lib.DTYPE_CODES[torch.bfloat16]}
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 _raw_stream = _lib.stream_of_index
+_CONTIGUOUS = torch.contiguous_format
 
 
 class KV4Cache:
@@ -167,7 +167,7 @@ def _ptr(t: Tensor | None):
 
 def _out_like(q: Tensor, out: Tensor | None, name: str = "out") -> Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return torch.empty_like(q, memory_format=_CONTIGUOUS)
     assert out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and out.device == q.device, (
         f"{name} must be a contiguous {q.dtype} {list(q.shape)} tensor on q's device")
     return out
@@ -271,19 +271,19 @@ def kv4_attention(q: Tensor, cache: KV4Cache, layer: int, block_table: Tensor, k
     Returns:
         [T, heads, D] of q's type, or (that, lse).
     """
-    _check_heads("q", q)
-    T, H, D = q.shape
-    d = q.get_device()
-    cache._check_layer(layer)
-    assert D == cache.head_dim and H > 0 and H % cache.num_kv_heads == 0, (
-        f"q must have a multiple of the cache's {cache.num_kv_heads} kv heads, of {cache.head_dim} channels")
-    assert cache._index == d, "the cache must be on q's device"
-    assert block_table.dtype is _I32 and block_table.dim() == 2 and block_table.is_contiguous() and (
-        block_table.get_device() == d), "block_table must be a contiguous int32 [sequences, pages] tensor on q's device"
-    B, width = block_table.shape
-    assert kv_lens.dtype is _I32 and kv_lens.shape == (B,) and kv_lens.is_contiguous() and kv_lens.get_device() == d, (
-        f"kv_lens must be a contiguous int32 [{B}] tensor on q's device")
-    assert window >= 0, f"window={window} must not be negative"
+    # The common case in one expression; anything else goes through the checks one by one, which say
+    # what is wrong.
+    d, dt, qh, th = q.get_device(), q.dtype, q.shape, block_table.shape
+    if not (d == cache._index and dt in _CODES and len(qh) == 3 and qh[2] == cache.head_dim and len(th) == 2
+            and 0 <= layer < cache.num_layers and qh[1] > 0 and qh[1] % cache.num_kv_heads == 0
+            and block_table.dtype is _I32 and block_table.get_device() == d and block_table.is_contiguous()
+            and kv_lens.dtype is _I32 and kv_lens.get_device() == d and kv_lens.shape == th[:1] and kv_lens.is_contiguous()
+            and window >= 0):
+        _check_attention(q, cache, layer, block_table, kv_lens, window)
+    T, H, D = qh
+    B, width = th
+    qt, qs, qc = q.stride()
+    assert qc == 1 or q.numel() == 0, "q must be [tokens, heads, head_dim] with contiguous channels"
     if cu_q is None:
         assert T == 0 or (B > 0 and T % B == 0), f"{T} queries do not divide into {B} sequences: cu_q is needed"
         max_q = T // B if B else 0
@@ -292,8 +292,8 @@ def kv4_attention(q: Tensor, cache: KV4Cache, layer: int, block_table: Tensor, k
             f"cu_q must be a contiguous int32 [{B + 1}] tensor on q's device")
         max_q = T if max_q is None else max_q
         assert max_q >= 0, f"max_q={max_q} must not be negative"
-    o = _out_like(q, out)
-    lse = torch.empty((T, H), dtype=_F32, device=q.device) if return_lse else None
+    o = torch.empty_like(q, memory_format=_CONTIGUOUS) if out is None else _out_like(q, out)
+    lse = q.new_empty((T, H), dtype=_F32) if return_lse else None
     key = (T, H, B, max_q)
     need = cache._ws_sizes.get(key)
     if need is None:
@@ -303,12 +303,28 @@ def kv4_attention(q: Tensor, cache: KV4Cache, layer: int, block_table: Tensor, k
                        "w4a16_kv4_attention_workspace_size")
         need = cache._ws_sizes[key] = size.value
     ws = _lib.kv4_workspace(need, d, _raw_stream(d)) if need else None
-    qs = q.stride()
-    _on(d, _lib.lib().w4a16_kv4_attention, q.data_ptr(), _CODES[q.dtype], T, H, qs[0], qs[1], cache._ref, layer,
-        block_table.data_ptr(), width, kv_lens.data_ptr(), _ptr(cu_q), B, max_q,
-        1.0 / math.sqrt(D) if scale is None else scale, window, o.data_ptr(), _ptr(lse), _ptr(ws),
-        0 if ws is None else ws.numel())
+    _on(d, _lib.lib().w4a16_kv4_attention, q.data_ptr(), _CODES[dt], T, H, qt, qs, cache._ref, layer,
+        block_table.data_ptr(), width, kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), B, max_q,
+        D ** -0.5 if scale is None else scale, window, o.data_ptr(), None if lse is None else lse.data_ptr(),
+        None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
     return (o, lse) if return_lse else o
+
+
+def _check_attention(q: Tensor, cache: KV4Cache, layer: int, block_table: Tensor, kv_lens: Tensor, window: int) -> None:
+    """kv4_attention's checks, one by one, so a bad call fails with the specific message."""
+    _check_heads("q", q)
+    _, H, D = q.shape
+    d = q.get_device()
+    cache._check_layer(layer)
+    assert D == cache.head_dim and H > 0 and H % cache.num_kv_heads == 0, (
+        f"q must have a multiple of the cache's {cache.num_kv_heads} kv heads, of {cache.head_dim} channels")
+    assert cache._index == d, "the cache must be on q's device"
+    assert block_table.dtype is _I32 and block_table.dim() == 2 and block_table.is_contiguous() and (
+        block_table.get_device() == d), "block_table must be a contiguous int32 [sequences, pages] tensor on q's device"
+    B = block_table.shape[0]
+    assert kv_lens.dtype is _I32 and kv_lens.shape == (B,) and kv_lens.is_contiguous() and kv_lens.get_device() == d, (
+        f"kv_lens must be a contiguous int32 [{B}] tensor on q's device")
+    assert window >= 0, f"window={window} must not be negative"
 
 
 def _ints(name: str, t: Tensor, n: int, device_index: int) -> None:
