@@ -2,7 +2,7 @@
 // preparation: argument checks and launches. Included once, by w4a16_b200.cu.
 #pragma once
 
-#include "kv4_decode.cuh"
+#include "kv4_prefill.cuh"
 #include "kv4_pages.cuh"
 #include "kv4_rope.cuh"
 
@@ -254,6 +254,43 @@ int launch_decode(const w4a16_kv4_cache& c, const AttendParams& all, const Atten
   });
 }
 
+// Sequences with more query rows (new tokens x heads of a group) per kv head than this take the
+// tensor-memory kernel, whose blocks of 256 rows each read the cache once; the others the decode
+// kernel, which reads it once per 16 rows but splits it over all SMs.
+constexpr int kDecodeRows = 64;
+
+template <int D, int NG>
+int launch_prefill_as(const PrefillParams& p, long long blocks, cudaStream_t s) {
+  auto k = kv4_prefill_kernel<D, NG>;
+  constexpr int bytes = PrefillShape<D, NG>::SMEM_BYTES;
+  static std::atomic<uint64_t> ready{0};
+  int d = 0;
+  if (cudaGetDevice(&d) != cudaSuccess) return W4A16_ERR_DEVICE;
+  if (!(ready.load(std::memory_order_acquire) >> d & 1)) {
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+      cudaGetLastError();
+      return W4A16_ERR_LAUNCH;
+    }
+    ready.fetch_or(1ull << d, std::memory_order_release);
+  }
+  k<<<static_cast<unsigned>(blocks), PF_THREADS, bytes, s>>>(p);
+  return launched();
+}
+
+int launch_prefill(const w4a16_kv4_cache& c, const AttendParams& a, const AttendPlan& plan, int bf16, cudaStream_t s) {
+  PrefillParams p = {};
+  p.a = a;
+  p.bf16 = bf16;
+  p.row_limit = kDecodeRows;
+  p.wait_ns = g_wait_budget_ns.load(std::memory_order_relaxed);
+  const long long tiles = (plan.rows + PF_ROWS - 1) / PF_ROWS;
+  if (plan.seqs * plan.kv_heads > 0x7fffffffLL / tiles) return W4A16_ERR_INVALID;
+  const long long blocks = tiles * plan.seqs * plan.kv_heads;
+  if (c.head_dim == 64) return launch_prefill_as<64, 1>(p, blocks, s);
+  if (c.group_size == 128) return launch_prefill_as<128, 1>(p, blocks, s);
+  return launch_prefill_as<128, 2>(p, blocks, s);
+}
+
 void launch_copy(const w4a16_kv4_cache& c, const int* src, const int* dst, const int* count, int n, const DeviceState& dev,
                  cudaStream_t s) {
   const CacheView v = view_of(c, 0);
@@ -349,7 +386,8 @@ int w4a16_kv4_attention_workspace_size(const w4a16_kv4_cache* cache, int64_t T, 
   if (T < 0 || T > 0x7fffffffLL || heads < 1 || heads % cache->kv_heads != 0 || seqs < 0 || max_q < 0)
     return W4A16_ERR_INVALID;
   if (T == 0 || seqs == 0) return W4A16_OK;
-  const kv4::AttendPlan plan = {seqs, cache->kv_heads, std::min(max_q, T) * (heads / cache->kv_heads)};
+  const kv4::AttendPlan plan = {seqs, cache->kv_heads,
+                                std::min<long long>(std::min(max_q, T) * (heads / cache->kv_heads), kv4::kDecodeRows)};
   *bytes_out = kv4::decode_workspace(*cache, plan, *dev);
   return W4A16_OK;
 }
@@ -364,7 +402,7 @@ int w4a16_kv4_attention(const void* q, int dtype, int64_t T, int heads, int64_t 
   if (T < 0 || T > 0x7fffffffLL || (dtype != W4A16_DTYPE_F16 && dtype != W4A16_DTYPE_BF16) || heads < 1 ||
       heads > 65535 || heads % cache->kv_heads != 0 || layer < 0 || layer >= cache->layers || seqs < 0 ||
       seqs > 0x7fffffffLL || table_width < 0 || max_q < 0 || window < 0 || workspace_bytes < 0 || !(scale == scale) ||
-      table_width * cache->page_size > 0x7fffffffLL)
+      table_width * cache->page_size > 0x7fffffffLL || T * (heads / cache->kv_heads) > (1LL << 30))
     return W4A16_ERR_INVALID;
   if (T == 0 || seqs == 0) return T == 0 ? W4A16_OK : W4A16_ERR_INVALID;
   if (cu_q == nullptr && T % seqs != 0) return W4A16_ERR_INVALID;
@@ -383,11 +421,19 @@ int w4a16_kv4_attention(const void* q, int dtype, int64_t T, int heads, int64_t 
   p.scale = scale; p.window = window;
   p.groups = cache->head_dim / cache->group_size;
   const kv4::AttendPlan plan = {seqs, cache->kv_heads, (cu_q ? std::min(max_q, T) : T / seqs) * p.share};
-  const int64_t need = kv4::decode_workspace(*cache, plan, *dev);
+  kv4::AttendPlan few = plan;      // the sequences that the decode kernel takes
+  few.rows = std::min<long long>(plan.rows, kv4::kDecodeRows);
+  const int64_t need = kv4::decode_workspace(*cache, few, *dev);
   if (workspace == nullptr || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return W4A16_ERR_WORKSPACE;
-  return kv4::launch_decode(*cache, p, plan, dtype == W4A16_DTYPE_BF16, 0x7fffffff, workspace, *dev,
-                            static_cast<cudaStream_t>(stream));
+  const int bf16 = dtype == W4A16_DTYPE_BF16;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (plan.rows > kv4::kDecodeRows) {
+    const int st2 = kv4::launch_prefill(*cache, p, plan, bf16, s);
+    if (st2 != W4A16_OK || cu_q == nullptr) return st2;
+  }
+  // sequences with few rows (every one, unless the batch is mixed)
+  return kv4::launch_decode(*cache, p, few, bf16, kv4::kDecodeRows, workspace, *dev, s);
 }
 
 int w4a16_kv4_copy_pages(const w4a16_kv4_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream) {
