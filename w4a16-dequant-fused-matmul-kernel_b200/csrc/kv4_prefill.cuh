@@ -38,7 +38,7 @@ namespace w4a16 {
 namespace kv4 {
 
 constexpr int PF_ROWS = 256;         // query rows per block (two tiles)
-constexpr int PF_THREADS = 13 * 32;
+constexpr int PF_THREADS = 16 * 32;  // warps 13-15 only complete the fourth group of four (register split)
 constexpr int PF_TILE = 128 * 128;   // bytes of a [128][64] fp16 tile
 constexpr int PF_PARS = 4;           // steps whose pairs are kept
 
@@ -54,6 +54,19 @@ __device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t smem_addr, uint3
   return d;
 }
 constexpr uint32_t kTransposeB = 1u << 16;   // instruction descriptor: B's N index contiguous
+
+// Registers per thread of a group of four warps from here on. The block is launched with 512 x 128;
+// 2 x 184 + 104 + 40 is the same for each scheduler's four warps.
+constexpr int PF_SOFTMAX_REGS = 184, PF_CACHE_REGS = 104, PF_MMA_REGS = 40;
+static_assert(2 * PF_SOFTMAX_REGS + PF_CACHE_REGS + PF_MMA_REGS <= 512, "register split");
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 struct PrefillParams {
   AttendParams a;
@@ -88,6 +101,13 @@ __device__ __forceinline__ uint4 centred_word(uint32_t w) {
                     hadd2_u32(lop3_and_or(u, 0x00F000F0u, 0x54005400u), 0xD480D480u));
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
+}
+
 __device__ __forceinline__ uint8_t* swizzled(uint8_t* tile, int row, int chunk) {
   return tile + row * 128 + ((chunk ^ (row & 7)) << 4);
 }
@@ -114,7 +134,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   const bool two = row0 + 128 <= last_row;
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  // an offset, not a cast: the compiler then knows its loads to be from shared memory
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* qtile = smem;
   uint8_t* ktile = qtile + SH::Q_BYTES;                   // two buffers, then V's two
   uint8_t* vtile = ktile + 2 * SH::KV_BYTES;
@@ -213,62 +234,80 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 12) {
+  if (warp >= 12) {
+    fewer_registers<PF_MMA_REGS>();
     // ------------------------------ products ------------------------------
-    if (lane == 0) {
-      const uint32_t qk_desc = umma_idesc_f16_f32(128, TOK), pv_desc = umma_idesc_f16_f32(128, D / NG) | kTransposeB;
+    // The whole warp runs along, and one lane of it issues: what the instructions take is then uniform
+    // and lies in uniform registers, where a branch on the lane would have every descriptor moved there
+    // (16 products took 3.9k cycles to issue that way).
+    if (warp == 12) {
+      const bool leader = elect_one();
+      constexpr uint32_t qk_desc = umma_idesc_f16_f32(128, TOK), pv_desc = umma_idesc_f16_f32(128, D / NG) | kTransposeB;
+      const uint64_t qd0 = umma_desc_sw128(smem_u32(qtile)), kd0 = umma_desc_sw128(smem_u32(ktile));
+      const uint64_t vd0 = umma_desc_sw128_mn(smem_u32(vtile), SH::BLOCK_BYTES);
       auto qk = [&](int t, int j) {
-        const uint8_t* q = qtile + t * KB * PF_TILE;
-        const uint8_t* k = ktile + (j & 1) * SH::KV_BYTES;
+        const uint64_t qd = qd0 + static_cast<uint64_t>(t * KB * (PF_TILE >> 4)), kd = kd0 + static_cast<uint64_t>((j & 1) * (SH::KV_BYTES >> 4));
+        if (leader) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          const uint64_t qd = umma_desc_sw128(smem_u32(q + kb * PF_TILE)), kd = umma_desc_sw128(smem_u32(k + kb * SH::BLOCK_BYTES));
-          const int g = NG == 2 ? kb : 0;
+          for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma_f16(tmem + t * 128 + g * TOK, qd + kk * 2, kd + kk * 2, qk_desc, (NG == 1 && kb) || kk);
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma_f16(tmem + t * 128 + (NG == 2 ? kb * TOK : 0), qd + kb * (PF_TILE >> 4) + kk * 2,
+                         kd + kb * (SH::BLOCK_BYTES >> 4) + kk * 2, qk_desc, (NG == 1 && kb) || kk);
+          tc_commit(&sfull[t]);
         }
-        tc_commit(&sfull[t]);
       };
-      bool ok = true;
-      if (steps > 0) {
-        ok = mbar_wait(&kfull[0], 0, p.wait_ns);
-        tc_fence_after();
-        if (ok) {
-          qk(0, 0);
-          if (two) qk(1, 0);
-          tc_commit(&kempty[0]);
-        }
-      }
-      for (int j = 0; ok && j < steps; ++j) {
-        for (int t = 0; ok && t < (two ? 2 : 1); ++t) {
-          ok = (t || mbar_wait(&vfull[j & 1], (j >> 1) & 1, p.wait_ns)) && mbar_wait(&pfull[t], j & 1, p.wait_ns);
-          if (!ok) break;
-          tc_fence_after();
+      auto pv = [&](int t, int j) {
+        const uint64_t vd = vd0 + static_cast<uint64_t>((j & 1) * (SH::KV_BYTES >> 4));
+        if (leader) {
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const uint64_t vd = umma_desc_sw128_mn(smem_u32(vtile + (j & 1) * SH::KV_BYTES + g * SH::BLOCK_BYTES), SH::BLOCK_BYTES);
+          for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int kk = 0; kk < TOK / 16; ++kk)
-              tc_mma_f16_ts(tmem + 256 + t * 128 + g * 64, tmem + t * 128 + g * TOK + kk * 8, vd + kk * 128, pv_desc, j || kk);
-          }
+              tc_mma_f16_ts(tmem + 256 + t * 128 + g * 64, tmem + t * 128 + g * TOK + kk * 8,
+                            vd + g * (SH::BLOCK_BYTES >> 4) + kk * 128, pv_desc, j || kk);
           tc_commit(&pvdone[t]);
-          if (t == 1 || !two) tc_commit(&vempty[j & 1]);
-          if (j + 1 < steps) {
-            if (t == 0) {
-              ok = mbar_wait(&kfull[(j + 1) & 1], ((j + 1) >> 1) & 1, p.wait_ns);
-              if (!ok) break;
-              tc_fence_after();
-            }
-            qk(t, j + 1);
-            if (t == 1 || !two) tc_commit(&kempty[(j + 1) & 1]);
-          }
+        }
+      };
+      auto signal = [&](uint64_t* bar) {
+        if (leader) tc_commit(bar);
+      };
+      bool ok = steps == 0 || mbar_wait(&kfull[0], 0, p.wait_ns);
+      if (ok && steps > 0) {
+        tc_fence_after();
+        qk(0, 0);
+        if (two) qk(1, 0);
+        signal(&kempty[0]);
+      }
+      for (int j = 0; ok && j < steps; ++j) {
+        ok = mbar_wait(&vfull[j & 1], (j >> 1) & 1, p.wait_ns) && mbar_wait(&pfull[0], j & 1, p.wait_ns);
+        if (!ok) break;
+        tc_fence_after();
+        pv(0, j);
+        if (!two) signal(&vempty[j & 1]);
+        if (j + 1 < steps) {
+          ok = mbar_wait(&kfull[(j + 1) & 1], ((j + 1) >> 1) & 1, p.wait_ns);
+          if (!ok) break;
+          tc_fence_after();
+          qk(0, j + 1);
+          if (!two) signal(&kempty[(j + 1) & 1]);
+        }
+        if (!two) continue;
+        ok = mbar_wait(&pfull[1], j & 1, p.wait_ns);
+        if (!ok) break;
+        tc_fence_after();
+        pv(1, j);
+        signal(&vempty[j & 1]);
+        if (j + 1 < steps) {
+          qk(1, j + 1);
+          signal(&kempty[(j + 1) & 1]);
         }
       }
-      tc_commit(drain);
+      signal(drain);
     }
   } else if (warp >= 8) {
     // ------------------------------ the cache ------------------------------
+    fewer_registers<PF_CACHE_REGS>();
     constexpr int CPT = CHUNKS / NG;                     // eights of channels per thread: one group's
     const int tok = (threadIdx.x - 256) % TOK, g = (threadIdx.x - 256) / TOK;
     uint4 kc[CPT / 4], vc[CPT / 4];
@@ -342,9 +381,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       expand(vtile + (j & 1) * SH::KV_BYTES, vc1, true);
       if (lane == 0) mbar_arrive(&vfull[j & 1]);
     }
-  } else if (warp < 4 || two) {
+  } else {
     // ------------------------------ softmax ------------------------------
+    more_registers<PF_SOFTMAX_REGS>();
     const int t = warp >> 2;
+    const int n = t == 0 || two ? steps : 0;             // a tile without rows has no products
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
     const bool live = row <= last_row;
@@ -368,43 +409,41 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       l_add = 0.0f;
 #pragma unroll
       for (int g = 0; g < NG; ++g) c_add[g] = 0.0f;
+      uint32_t x[2][32];       // 64 columns: the half's tokens, or 32 of each group
 #pragma unroll
-      for (int c = 0; c < HT; c += 32) {
-        uint32_t x[NG][32];
+      for (int i = 0; i < 2; ++i) tmem_ld_32x32b_x32(s_half + (NG == 1 ? 32 * i : TOK * i), x[i]);
+      tmem_ld_wait();
 #pragma unroll
-        for (int g = 0; g < NG; ++g) tmem_ld_32x32b_x32(s_half + g * TOK + c, x[g]);
-        tmem_ld_wait();
+      for (int i = 0; i < HT; i += 2) {
+        float ps[NG][2];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float ps[NG][2];
+        for (int k = 0; k < 2; ++k) {
+          float4 q[NG];
+          float y = -m;
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float4 q[NG];
-            float y = -m;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-              q[g] = par[g * TOK + c + i + k];
-              y = fmaf(q[g].y, qs[g], y);
-            }
-#pragma unroll
-            for (int g = 0; g < NG; ++g) y = fmaf(__uint_as_float(x[g][i + k]), q[g].x, y);
-            if (EDGE && (tok0 + c + i + k < see_from || tok0 + c + i + k >= see_to)) y = -INFINITY;
-            top = fmaxf(top, y);
-            const float e = ex2(y);
-            l_add += e;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-              if (EDGE && e == 0.0f) {     // a token that is not seen may have any pair, NaN too
-                ps[g][k] = 0.0f;
-              } else {
-                ps[g][k] = e * q[g].z;
-                c_add[g] = fmaf(e, q[g].w, c_add[g]);
-              }
-            }
+          for (int g = 0; g < NG; ++g) {
+            q[g] = par[g * TOK + i + k];
+            y = fmaf(q[g].y, qs[g], y);
           }
 #pragma unroll
-          for (int g = 0; g < NG; ++g) h[g][(c + i) / 2] = pack2<__half>(ps[g][0], ps[g][1]);
+          for (int g = 0; g < NG; ++g)
+            y = fmaf(__uint_as_float(NG == 1 ? x[(i + k) / 32][(i + k) % 32] : x[g][(i + k) % 32]), q[g].x, y);
+          if (EDGE && (tok0 + i + k < see_from || tok0 + i + k >= see_to)) y = -INFINITY;
+          top = fmaxf(top, y);
+          const float e = ex2(y);
+          l_add += e;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            if (EDGE && e == 0.0f) {     // a token that is not seen may have any pair, NaN too
+              ps[g][k] = 0.0f;
+            } else {
+              ps[g][k] = e * q[g].z;
+              c_add[g] = fmaf(e, q[g].w, c_add[g]);
+            }
+          }
         }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) h[g][i / 2] = pack2<__half>(ps[g][0], ps[g][1]);
       }
       return top;
     };
@@ -417,7 +456,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
         tmem_st_32x32b_x16(at + c, r);
       }
     };
-    for (int j = 0; ok && j < steps; ++j) {
+    for (int j = 0; ok && j < n; ++j) {
       ok = mbar_wait(&sfull[t], j & 1, p.wait_ns) && mbar_wait(&parfull[j % PF_PARS], (j / PF_PARS) & 1, p.wait_ns);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -491,7 +530,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       if (lane == 0) mbar_arrive(&pfull[t]);
     }
     // ---- the row's result
-    if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&pvdone[t], (steps - 1) & 1, p.wait_ns));
+    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&pvdone[t], (steps - 1) & 1, p.wait_ns));
     tc_fence_after();
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const long long at = static_cast<long long>(first + row / a.share) * a.heads + kh * a.share + row % a.share;
@@ -500,7 +539,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
     for (int c = 0; c < D; c += 16) {
       uint32_t x[16];
       __syncwarp();
-      if (steps > 0) {
+      if (n > 0) {
         tmem_ld_32x32b_x16(o_at + c, x);
         tmem_ld_wait();
       }
@@ -509,7 +548,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
         float y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)     // column order 0 4 1 5 2 6 3 7
-          y[(i >> 1) + (i & 1) * 4] = steps > 0 && l != 0.0f ? (__uint_as_float(x[8 * k + i]) + (c < D / NG ? corr[0] : corr[NG - 1])) * inv : 0.0f;
+          y[(i >> 1) + (i & 1) * 4] = n > 0 && l != 0.0f ? (__uint_as_float(x[8 * k + i]) + (c < D / NG ? corr[0] : corr[NG - 1])) * inv : 0.0f;
         uint4 o;
         uint32_t* ow = &o.x;
 #pragma unroll
