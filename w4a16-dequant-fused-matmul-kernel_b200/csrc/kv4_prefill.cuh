@@ -101,6 +101,32 @@ __device__ __forceinline__ uint4 centred_word(uint32_t w) {
                     hadd2_u32(lop3_and_or(u, 0x00F000F0u, 0x54005400u), 0xD480D480u));
 }
 
+// Two fp32 values in one 64-bit register and the instructions that take both at once.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair_of(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void halves_of(f32x2 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t yes;
@@ -139,8 +165,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   uint8_t* qtile = smem;
   uint8_t* ktile = qtile + SH::Q_BYTES;                   // two buffers, then V's two
   uint8_t* vtile = ktile + 2 * SH::KV_BYTES;
-  float4* pars = reinterpret_cast<float4*>(vtile + 2 * SH::KV_BYTES);   // [PF_PARS][NG][TOK]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(pars + PF_PARS * 128);
+  // [PF_PARS][NG][TOK / 2][8]: of a pair of tokens the keys' scales (times f) and offsets, the values'
+  // scales and offset + 8 scale
+  float* pars = reinterpret_cast<float*>(vtile + 2 * SH::KV_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(pars + PF_PARS * 128 * 4);
   uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6;
   uint64_t *sfull = bars + 8, *pfull = bars + 10, *pvdone = bars + 12, *drain = bars + 14;
   uint64_t* parfull = bars + 15;
@@ -367,7 +395,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       page = page_of(j + 2);
       // the pairs of step j - PF_PARS have been read: its products were done before step j - 2's V tile
       // was written over
-      pars[((j % PF_PARS) * NG + g) * TOK + tok] = make_float4(ks.x * f, ks.y, vs.x, fmaf(8.0f, vs.x, vs.y));
+      float* par = pars + (((j % PF_PARS) * NG + g) * TOK + (tok & ~1)) * 4 + (tok & 1);
+      par[0] = ks.x * f;
+      par[2] = ks.y;
+      par[4] = vs.x;
+      par[6] = fmaf(8.0f, vs.x, vs.y);
       __syncwarp();
       if (lane == 0) mbar_arrive(&parfull[j % PF_PARS]);
       ok = mbar_wait_backoff(&kempty[j & 1], ((j >> 1) & 1) ^ 1u, p.wait_ns, 64);
@@ -396,54 +428,73 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
     const int all_to = min(len, len - count + (row0 + t * 128) / a.share + 1);
     const int all_from = a.window ? max(0, len - count + tile_last / a.share - a.window + 1) : 0;
     constexpr int HT = 64 / NG;                          // tokens of half a step
+    f32x2 qs2[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) qs2[g] = pair_of(qs[g], qs[g]);
     float m = 0.0f, l = 0.0f, corr[NG];                  // l = sum p, corr = sum p (b + 8 s)
 #pragma unroll
     for (int g = 0; g < NG; ++g) corr[g] = 0.0f;
     bool fresh = true, ok = true;
     // The probabilities of half a step with the maximum m: h = p s in fp16, packed by token pairs, and
     // what l and corr gain; returns the largest score over m.
-    auto half_step = [&](auto edge_tag, const float4* par, uint32_t s_half, int tok0, uint32_t (&h)[NG][HT / 2],
+    auto half_step = [&](auto edge_tag, const float* par, uint32_t s_half, int tok0, uint32_t (&h)[NG][HT / 2],
                          float& l_add, float (&c_add)[NG]) {
       constexpr bool EDGE = decltype(edge_tag)::value;
       float top = -INFINITY;
-      l_add = 0.0f;
+      const f32x2 minus_m = pair_of(-m, -m);
+      f32x2 l2 = 0, c2[NG];
 #pragma unroll
-      for (int g = 0; g < NG; ++g) c_add[g] = 0.0f;
+      for (int g = 0; g < NG; ++g) c2[g] = 0;
       uint32_t x[2][32];       // 64 columns: the half's tokens, or 32 of each group
 #pragma unroll
       for (int i = 0; i < 2; ++i) tmem_ld_32x32b_x32(s_half + (NG == 1 ? 32 * i : TOK * i), x[i]);
       tmem_ld_wait();
 #pragma unroll
       for (int i = 0; i < HT; i += 2) {
-        float ps[NG][2];
+        ulonglong2 kq[NG], vq[NG];      // (scale, offset) of the pair's keys, then of its values
+        f32x2 y = minus_m;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float4 q[NG];
-          float y = -m;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            q[g] = par[g * TOK + i + k];
-            y = fmaf(q[g].y, qs[g], y);
-          }
-#pragma unroll
-          for (int g = 0; g < NG; ++g)
-            y = fmaf(__uint_as_float(NG == 1 ? x[(i + k) / 32][(i + k) % 32] : x[g][(i + k) % 32]), q[g].x, y);
-          if (EDGE && (tok0 + i + k < see_from || tok0 + i + k >= see_to)) y = -INFINITY;
-          top = fmaxf(top, y);
-          const float e = ex2(y);
-          l_add += e;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            if (EDGE && e == 0.0f) {     // a token that is not seen may have any pair, NaN too
-              ps[g][k] = 0.0f;
-            } else {
-              ps[g][k] = e * q[g].z;
-              c_add[g] = fmaf(e, q[g].w, c_add[g]);
-            }
-          }
+        for (int g = 0; g < NG; ++g) {
+          const ulonglong2* at = reinterpret_cast<const ulonglong2*>(par + (g * TOK + i) * 4);
+          kq[g] = at[0];
+          vq[g] = at[1];
+          y = fma2(kq[g].y, qs2[g], y);
         }
 #pragma unroll
-        for (int g = 0; g < NG; ++g) h[g][i / 2] = pack2<__half>(ps[g][0], ps[g][1]);
+        for (int g = 0; g < NG; ++g) {
+          const uint32_t* xs = NG == 1 ? &x[i / 32][i % 32] : &x[g][i];
+          y = fma2(pair_of(__uint_as_float(xs[0]), __uint_as_float(xs[1])), kq[g].x, y);
+        }
+        float y0, y1;
+        halves_of(y, y0, y1);
+        if (EDGE && (tok0 + i < see_from || tok0 + i >= see_to)) y0 = -INFINITY;
+        if (EDGE && (tok0 + i + 1 < see_from || tok0 + i + 1 >= see_to)) y1 = -INFINITY;
+        top = fmaxf(top, fmaxf(y0, y1));
+        const float e0 = ex2(y0), e1 = ex2(y1);
+        const f32x2 e = pair_of(e0, e1);
+        l2 = add2(l2, e);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          if (EDGE) {                  // a token that is not seen may have any pair, NaN too
+            float s0, s1, o0, o1;
+            halves_of(vq[g].x, s0, s1);
+            halves_of(vq[g].y, o0, o1);
+            vq[g].x = pair_of(e0 == 0.0f ? 0.0f : s0, e1 == 0.0f ? 0.0f : s1);
+            vq[g].y = pair_of(e0 == 0.0f ? 0.0f : o0, e1 == 0.0f ? 0.0f : o1);
+          }
+          float p0, p1;
+          halves_of(mul2(e, vq[g].x), p0, p1);
+          h[g][i / 2] = pack2<__half>(p0, p1);
+          c2[g] = fma2(e, vq[g].y, c2[g]);
+        }
+      }
+      float lo, hi;
+      halves_of(l2, lo, hi);
+      l_add = lo + hi;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        halves_of(c2[g], lo, hi);
+        c_add[g] = lo + hi;
       }
       return top;
     };
@@ -465,7 +516,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       const bool edge = tok0 < all_from || tok0 + TOK > all_to;
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
-        const float4* par = pars + (j % PF_PARS) * NG * TOK + half * HT;
+        const float* par = pars + ((j % PF_PARS) * NG * TOK + half * HT) * 4;
         uint32_t h[NG][HT / 2];
         float l_add, c_add[NG];
         auto take = [&]() {
