@@ -38,7 +38,7 @@ namespace w4a16 {
 namespace kv4 {
 
 constexpr int PF_ROWS = 256;         // query rows per block (two tiles)
-constexpr int PF_THREADS = 16 * 32;  // warps 13-15 only complete the fourth group of four (register split)
+constexpr int PF_THREADS = 13 * 32;
 constexpr int PF_TILE = 128 * 128;   // bytes of a [128][64] fp16 tile
 constexpr int PF_PARS = 4;           // steps whose pairs are kept
 
@@ -54,19 +54,6 @@ __device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t smem_addr, uint3
   return d;
 }
 constexpr uint32_t kTransposeB = 1u << 16;   // instruction descriptor: B's N index contiguous
-
-// Registers per thread of a group of four warps from here on. The block is launched with 512 x 128;
-// 2 x 184 + 104 + 40 is the same for each scheduler's four warps.
-constexpr int PF_SOFTMAX_REGS = 184, PF_CACHE_REGS = 104, PF_MMA_REGS = 40;
-static_assert(2 * PF_SOFTMAX_REGS + PF_CACHE_REGS + PF_MMA_REGS <= 512, "register split");
-template <int N>
-__device__ __forceinline__ void more_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void fewer_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
 
 struct PrefillParams {
   AttendParams a;
@@ -101,39 +88,6 @@ __device__ __forceinline__ uint4 centred_word(uint32_t w) {
                     hadd2_u32(lop3_and_or(u, 0x00F000F0u, 0x54005400u), 0xD480D480u));
 }
 
-// Two fp32 values in one 64-bit register and the instructions that take both at once.
-using f32x2 = unsigned long long;
-__device__ __forceinline__ f32x2 pair_of(float lo, float hi) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void halves_of(f32x2 v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
-// One lane of a converged warp.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t yes;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
-  return yes != 0;
-}
-
 __device__ __forceinline__ uint8_t* swizzled(uint8_t* tile, int row, int chunk) {
   return tile + row * 128 + ((chunk ^ (row & 7)) << 4);
 }
@@ -165,10 +119,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   uint8_t* qtile = smem;
   uint8_t* ktile = qtile + SH::Q_BYTES;                   // two buffers, then V's two
   uint8_t* vtile = ktile + 2 * SH::KV_BYTES;
-  // [PF_PARS][NG][TOK / 2][8]: of a pair of tokens the keys' scales (times f) and offsets, the values'
-  // scales and offset + 8 scale
-  float* pars = reinterpret_cast<float*>(vtile + 2 * SH::KV_BYTES);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(pars + PF_PARS * 128 * 4);
+  float4* pars = reinterpret_cast<float4*>(vtile + 2 * SH::KV_BYTES);   // [PF_PARS][NG][TOK]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(pars + PF_PARS * 128);
   uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6;
   uint64_t *sfull = bars + 8, *pfull = bars + 10, *pvdone = bars + 12, *drain = bars + 14;
   uint64_t* parfull = bars + 15;
@@ -262,80 +214,62 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 12) {
-    fewer_registers<PF_MMA_REGS>();
+  if (warp == 12) {
     // ------------------------------ products ------------------------------
-    // The whole warp runs along, and one lane of it issues: what the instructions take is then uniform
-    // and lies in uniform registers, where a branch on the lane would have every descriptor moved there
-    // (16 products took 3.9k cycles to issue that way).
-    if (warp == 12) {
-      const bool leader = elect_one();
-      constexpr uint32_t qk_desc = umma_idesc_f16_f32(128, TOK), pv_desc = umma_idesc_f16_f32(128, D / NG) | kTransposeB;
-      const uint64_t qd0 = umma_desc_sw128(smem_u32(qtile)), kd0 = umma_desc_sw128(smem_u32(ktile));
-      const uint64_t vd0 = umma_desc_sw128_mn(smem_u32(vtile), SH::BLOCK_BYTES);
+    if (lane == 0) {
+      const uint32_t qk_desc = umma_idesc_f16_f32(128, TOK), pv_desc = umma_idesc_f16_f32(128, D / NG) | kTransposeB;
       auto qk = [&](int t, int j) {
-        const uint64_t qd = qd0 + static_cast<uint64_t>(t * KB * (PF_TILE >> 4)), kd = kd0 + static_cast<uint64_t>((j & 1) * (SH::KV_BYTES >> 4));
-        if (leader) {
+        const uint8_t* q = qtile + t * KB * PF_TILE;
+        const uint8_t* k = ktile + (j & 1) * SH::KV_BYTES;
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
+        for (int kb = 0; kb < KB; ++kb) {
+          const uint64_t qd = umma_desc_sw128(smem_u32(q + kb * PF_TILE)), kd = umma_desc_sw128(smem_u32(k + kb * SH::BLOCK_BYTES));
+          const int g = NG == 2 ? kb : 0;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc_mma_f16(tmem + t * 128 + (NG == 2 ? kb * TOK : 0), qd + kb * (PF_TILE >> 4) + kk * 2,
-                         kd + kb * (SH::BLOCK_BYTES >> 4) + kk * 2, qk_desc, (NG == 1 && kb) || kk);
-          tc_commit(&sfull[t]);
+          for (int kk = 0; kk < 4; ++kk)
+            tc_mma_f16(tmem + t * 128 + g * TOK, qd + kk * 2, kd + kk * 2, qk_desc, (NG == 1 && kb) || kk);
         }
+        tc_commit(&sfull[t]);
       };
-      auto pv = [&](int t, int j) {
-        const uint64_t vd = vd0 + static_cast<uint64_t>((j & 1) * (SH::KV_BYTES >> 4));
-        if (leader) {
-#pragma unroll
-          for (int g = 0; g < NG; ++g)
-#pragma unroll
-            for (int kk = 0; kk < TOK / 16; ++kk)
-              tc_mma_f16_ts(tmem + 256 + t * 128 + g * 64, tmem + t * 128 + g * TOK + kk * 8,
-                            vd + g * (SH::BLOCK_BYTES >> 4) + kk * 128, pv_desc, j || kk);
-          tc_commit(&pvdone[t]);
-        }
-      };
-      auto signal = [&](uint64_t* bar) {
-        if (leader) tc_commit(bar);
-      };
-      bool ok = steps == 0 || mbar_wait(&kfull[0], 0, p.wait_ns);
-      if (ok && steps > 0) {
+      bool ok = true;
+      if (steps > 0) {
+        ok = mbar_wait(&kfull[0], 0, p.wait_ns);
         tc_fence_after();
-        qk(0, 0);
-        if (two) qk(1, 0);
-        signal(&kempty[0]);
+        if (ok) {
+          qk(0, 0);
+          if (two) qk(1, 0);
+          tc_commit(&kempty[0]);
+        }
       }
       for (int j = 0; ok && j < steps; ++j) {
-        ok = mbar_wait(&vfull[j & 1], (j >> 1) & 1, p.wait_ns) && mbar_wait(&pfull[0], j & 1, p.wait_ns);
-        if (!ok) break;
-        tc_fence_after();
-        pv(0, j);
-        if (!two) signal(&vempty[j & 1]);
-        if (j + 1 < steps) {
-          ok = mbar_wait(&kfull[(j + 1) & 1], ((j + 1) >> 1) & 1, p.wait_ns);
+        for (int t = 0; ok && t < (two ? 2 : 1); ++t) {
+          ok = (t || mbar_wait(&vfull[j & 1], (j >> 1) & 1, p.wait_ns)) && mbar_wait(&pfull[t], j & 1, p.wait_ns);
           if (!ok) break;
           tc_fence_after();
-          qk(0, j + 1);
-          if (!two) signal(&kempty[(j + 1) & 1]);
-        }
-        if (!two) continue;
-        ok = mbar_wait(&pfull[1], j & 1, p.wait_ns);
-        if (!ok) break;
-        tc_fence_after();
-        pv(1, j);
-        signal(&vempty[j & 1]);
-        if (j + 1 < steps) {
-          qk(1, j + 1);
-          signal(&kempty[(j + 1) & 1]);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const uint64_t vd = umma_desc_sw128_mn(smem_u32(vtile + (j & 1) * SH::KV_BYTES + g * SH::BLOCK_BYTES), SH::BLOCK_BYTES);
+#pragma unroll
+            for (int kk = 0; kk < TOK / 16; ++kk)
+              tc_mma_f16_ts(tmem + 256 + t * 128 + g * 64, tmem + t * 128 + g * TOK + kk * 8, vd + kk * 128, pv_desc, j || kk);
+          }
+          tc_commit(&pvdone[t]);
+          if (t == 1 || !two) tc_commit(&vempty[j & 1]);
+          if (j + 1 < steps) {
+            if (t == 0) {
+              ok = mbar_wait(&kfull[(j + 1) & 1], ((j + 1) >> 1) & 1, p.wait_ns);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            qk(t, j + 1);
+            if (t == 1 || !two) tc_commit(&kempty[(j + 1) & 1]);
+          }
         }
       }
-      signal(drain);
+      tc_commit(drain);
     }
   } else if (warp >= 8) {
     // ------------------------------ the cache ------------------------------
-    fewer_registers<PF_CACHE_REGS>();
     constexpr int CPT = CHUNKS / NG;                     // eights of channels per thread: one group's
     const int tok = (threadIdx.x - 256) % TOK, g = (threadIdx.x - 256) / TOK;
     uint4 kc[CPT / 4], vc[CPT / 4];
@@ -395,11 +329,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       page = page_of(j + 2);
       // the pairs of step j - PF_PARS have been read: its products were done before step j - 2's V tile
       // was written over
-      float* par = pars + (((j % PF_PARS) * NG + g) * TOK + (tok & ~1)) * 4 + (tok & 1);
-      par[0] = ks.x * f;
-      par[2] = ks.y;
-      par[4] = vs.x;
-      par[6] = fmaf(8.0f, vs.x, vs.y);
+      pars[((j % PF_PARS) * NG + g) * TOK + tok] = make_float4(ks.x * f, ks.y, vs.x, fmaf(8.0f, vs.x, vs.y));
       __syncwarp();
       if (lane == 0) mbar_arrive(&parfull[j % PF_PARS]);
       ok = mbar_wait_backoff(&kempty[j & 1], ((j >> 1) & 1) ^ 1u, p.wait_ns, 64);
@@ -413,11 +343,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       expand(vtile + (j & 1) * SH::KV_BYTES, vc1, true);
       if (lane == 0) mbar_arrive(&vfull[j & 1]);
     }
-  } else {
+  } else if (warp < 4 || two) {
     // ------------------------------ softmax ------------------------------
-    more_registers<PF_SOFTMAX_REGS>();
     const int t = warp >> 2;
-    const int n = t == 0 || two ? steps : 0;             // a tile without rows has no products
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
     const bool live = row <= last_row;
@@ -428,73 +356,56 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
     const int all_to = min(len, len - count + (row0 + t * 128) / a.share + 1);
     const int all_from = a.window ? max(0, len - count + tile_last / a.share - a.window + 1) : 0;
     constexpr int HT = 64 / NG;                          // tokens of half a step
-    f32x2 qs2[NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) qs2[g] = pair_of(qs[g], qs[g]);
     float m = 0.0f, l = 0.0f, corr[NG];                  // l = sum p, corr = sum p (b + 8 s)
 #pragma unroll
     for (int g = 0; g < NG; ++g) corr[g] = 0.0f;
     bool fresh = true, ok = true;
     // The probabilities of half a step with the maximum m: h = p s in fp16, packed by token pairs, and
     // what l and corr gain; returns the largest score over m.
-    auto half_step = [&](auto edge_tag, const float* par, uint32_t s_half, int tok0, uint32_t (&h)[NG][HT / 2],
+    auto half_step = [&](auto edge_tag, const float4* par, uint32_t s_half, int tok0, uint32_t (&h)[NG][HT / 2],
                          float& l_add, float (&c_add)[NG]) {
       constexpr bool EDGE = decltype(edge_tag)::value;
       float top = -INFINITY;
-      const f32x2 minus_m = pair_of(-m, -m);
-      f32x2 l2 = 0, c2[NG];
+      l_add = 0.0f;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) c2[g] = 0;
-      uint32_t x[2][32];       // 64 columns: the half's tokens, or 32 of each group
+      for (int g = 0; g < NG; ++g) c_add[g] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) tmem_ld_32x32b_x32(s_half + (NG == 1 ? 32 * i : TOK * i), x[i]);
-      tmem_ld_wait();
+      for (int c = 0; c < HT; c += 32) {
+        uint32_t x[NG][32];
 #pragma unroll
-      for (int i = 0; i < HT; i += 2) {
-        ulonglong2 kq[NG], vq[NG];      // (scale, offset) of the pair's keys, then of its values
-        f32x2 y = minus_m;
+        for (int g = 0; g < NG; ++g) tmem_ld_32x32b_x32(s_half + g * TOK + c, x[g]);
+        tmem_ld_wait();
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const ulonglong2* at = reinterpret_cast<const ulonglong2*>(par + (g * TOK + i) * 4);
-          kq[g] = at[0];
-          vq[g] = at[1];
-          y = fma2(kq[g].y, qs2[g], y);
-        }
+        for (int i = 0; i < 32; i += 2) {
+          float ps[NG][2];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const uint32_t* xs = NG == 1 ? &x[i / 32][i % 32] : &x[g][i];
-          y = fma2(pair_of(__uint_as_float(xs[0]), __uint_as_float(xs[1])), kq[g].x, y);
-        }
-        float y0, y1;
-        halves_of(y, y0, y1);
-        if (EDGE && (tok0 + i < see_from || tok0 + i >= see_to)) y0 = -INFINITY;
-        if (EDGE && (tok0 + i + 1 < see_from || tok0 + i + 1 >= see_to)) y1 = -INFINITY;
-        top = fmaxf(top, fmaxf(y0, y1));
-        const float e0 = ex2(y0), e1 = ex2(y1);
-        const f32x2 e = pair_of(e0, e1);
-        l2 = add2(l2, e);
+          for (int k = 0; k < 2; ++k) {
+            float4 q[NG];
+            float y = -m;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          if (EDGE) {                  // a token that is not seen may have any pair, NaN too
-            float s0, s1, o0, o1;
-            halves_of(vq[g].x, s0, s1);
-            halves_of(vq[g].y, o0, o1);
-            vq[g].x = pair_of(e0 == 0.0f ? 0.0f : s0, e1 == 0.0f ? 0.0f : s1);
-            vq[g].y = pair_of(e0 == 0.0f ? 0.0f : o0, e1 == 0.0f ? 0.0f : o1);
+            for (int g = 0; g < NG; ++g) {
+              q[g] = par[g * TOK + c + i + k];
+              y = fmaf(q[g].y, qs[g], y);
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) y = fmaf(__uint_as_float(x[g][i + k]), q[g].x, y);
+            if (EDGE && (tok0 + c + i + k < see_from || tok0 + c + i + k >= see_to)) y = -INFINITY;
+            top = fmaxf(top, y);
+            const float e = ex2(y);
+            l_add += e;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              if (EDGE && e == 0.0f) {     // a token that is not seen may have any pair, NaN too
+                ps[g][k] = 0.0f;
+              } else {
+                ps[g][k] = e * q[g].z;
+                c_add[g] = fmaf(e, q[g].w, c_add[g]);
+              }
+            }
           }
-          float p0, p1;
-          halves_of(mul2(e, vq[g].x), p0, p1);
-          h[g][i / 2] = pack2<__half>(p0, p1);
-          c2[g] = fma2(e, vq[g].y, c2[g]);
-        }
-      }
-      float lo, hi;
-      halves_of(l2, lo, hi);
-      l_add = lo + hi;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        halves_of(c2[g], lo, hi);
-        c_add[g] = lo + hi;
+          for (int g = 0; g < NG; ++g) h[g][(c + i) / 2] = pack2<__half>(ps[g][0], ps[g][1]);
+        }
       }
       return top;
     };
@@ -507,7 +418,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
         tmem_st_32x32b_x16(at + c, r);
       }
     };
-    for (int j = 0; ok && j < n; ++j) {
+    for (int j = 0; ok && j < steps; ++j) {
       ok = mbar_wait(&sfull[t], j & 1, p.wait_ns) && mbar_wait(&parfull[j % PF_PARS], (j / PF_PARS) & 1, p.wait_ns);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -516,7 +427,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       const bool edge = tok0 < all_from || tok0 + TOK > all_to;
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
-        const float* par = pars + ((j % PF_PARS) * NG * TOK + half * HT) * 4;
+        const float4* par = pars + (j % PF_PARS) * NG * TOK + half * HT;
         uint32_t h[NG][HT / 2];
         float l_add, c_add[NG];
         auto take = [&]() {
@@ -581,7 +492,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       if (lane == 0) mbar_arrive(&pfull[t]);
     }
     // ---- the row's result
-    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&pvdone[t], (steps - 1) & 1, p.wait_ns));
+    if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&pvdone[t], (steps - 1) & 1, p.wait_ns));
     tc_fence_after();
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const long long at = static_cast<long long>(first + row / a.share) * a.heads + kh * a.share + row % a.share;
@@ -590,7 +501,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
     for (int c = 0; c < D; c += 16) {
       uint32_t x[16];
       __syncwarp();
-      if (n > 0) {
+      if (steps > 0) {
         tmem_ld_32x32b_x16(o_at + c, x);
         tmem_ld_wait();
       }
@@ -599,7 +510,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
         float y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)     // column order 0 4 1 5 2 6 3 7
-          y[(i >> 1) + (i & 1) * 4] = n > 0 && l != 0.0f ? (__uint_as_float(x[8 * k + i]) + (c < D / NG ? corr[0] : corr[NG - 1])) * inv : 0.0f;
+          y[(i >> 1) + (i & 1) * 4] = steps > 0 && l != 0.0f ? (__uint_as_float(x[8 * k + i]) + (c < D / NG ? corr[0] : corr[NG - 1])) * inv : 0.0f;
         uint4 o;
         uint32_t* ow = &o.x;
 #pragma unroll
