@@ -457,7 +457,8 @@ int w4a16_kv4_page_bytes(int head_dim, int page_size, int group_size, int64_t* b
  * token and head strides, in elements): RMS norm of each head (x / sqrt(mean(x^2) + eps) *
  * weight; a null weight skips it), then the rotation of the first `rot` channels (a multiple
  * of 8): pairs (i, i + rot/2), or (2i, 2i+1) when interleaved, by the angle whose cosine and
- * sine are cos_sin[position][i] and cos_sin[position][rot/2 + i] (fp32 [max_position, rot]).
+ * sine are cos_sin[position][i] and cos_sin[position][rot/2 + i] (fp32 [max_position, rot], 16-byte
+ * aligned).
  * positions: [T] (axes 1), or [3, T] (axes 3): frequencies i < axis0_end turn by the first
  * row's position, i < axis1_end by the second's, the others by the third's. fp32 arithmetic,
  * one rounding. q_out, k_out: dense, 16-byte aligned. weight_dtype: dtype, or fp32.

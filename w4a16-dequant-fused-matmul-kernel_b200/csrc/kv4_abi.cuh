@@ -99,7 +99,7 @@ int rope(const RopeArgs& a, void* q_out, void* k_out, const w4a16_kv4_cache* cac
       (a.kv_heads && !append && k_out == nullptr) || (append && (a.v == nullptr || slots == nullptr)) ||
       (a.rot && (a.positions == nullptr || a.cos_sin == nullptr)))
     return W4A16_ERR_INVALID;
-  if (!aligned16(q_out) || (!append && !aligned16(k_out))) return W4A16_ERR_ALIGNMENT;
+  if (!aligned16(q_out) || (!append && !aligned16(k_out)) || !aligned16(a.cos_sin)) return W4A16_ERR_ALIGNMENT;
   p.q = a.q; p.k = a.k; p.v = a.v;
   p.q_st = a.q_st; p.q_sh = a.q_sh; p.k_st = a.k_st; p.k_sh = a.k_sh; p.v_st = a.v_st; p.v_sh = a.v_sh;
   p.q_out = q_out; p.k_out = k_out;
@@ -120,6 +120,7 @@ int rope(const RopeArgs& a, void* q_out, void* k_out, const w4a16_kv4_cache* cac
     return reinterpret_cast<uintptr_t>(x) % 8 == 0 && st % 4 == 0 && sh % 4 == 0;
   };
   p.vec = quads(a.q, a.q_st, a.q_sh) && quads(a.k, a.k_st, a.k_sh) && (!append || quads(a.v, a.v_st, a.v_sh));
+  p.w_vec = reinterpret_cast<uintptr_t>(a.qw) % 8 == 0 && reinterpret_cast<uintptr_t>(a.kw) % 8 == 0;
   if (p.T * p.chunks * (a.head_dim / 8) / ROPE_THREADS >= 0x7fffffffLL) return W4A16_ERR_INVALID;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a.dtype == W4A16_DTYPE_F16) {

@@ -45,22 +45,36 @@ struct RopeParams {
   int w_f32;                      // weights fp32, else of the inputs' type
   float eps;
   int vec;                        // every quad of q, k, v is 8-byte aligned
+  int w_vec;                      // and of 16-bit weights
   const long long* slots;         // APPEND: [T], page * page_size + offset; < 0: not cached
   CacheView cache;
   int groups;                     // D / G: 1 or 2
 };
 
+// Four channels as they lie in memory, and as fp32.
 template <typename T>
-__device__ __forceinline__ void load_quad(const T* src, int vec, float* x) {
-  T v[4];
-  if (vec) {
-    *reinterpret_cast<uint2*>(v) = __ldg(reinterpret_cast<const uint2*>(src));
-  } else {
+__device__ __forceinline__ uint2 load_quad(const T* src, int vec) {
+  if (vec) return __ldg(reinterpret_cast<const uint2*>(src));
+  const unsigned short* v = reinterpret_cast<const unsigned short*>(src);
+  return make_uint2(v[0] | static_cast<uint32_t>(v[1]) << 16, v[2] | static_cast<uint32_t>(v[3]) << 16);
+}
+template <typename T>
+__device__ __forceinline__ void quad_f32(const uint2& v, float* x) {
+  const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = src[i];
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(v[i]);
+  for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(e[i]);
+}
+
+// Minimum and maximum that are NaN where one of the two is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 template <typename T>
@@ -84,27 +98,24 @@ __device__ __forceinline__ void quantise_row(const float (&x)[8], int e0, int e1
                                              uint8_t* codes, uint32_t* pairs) {
   constexpr int L = D / 8;
   const int g0 = groups == 1 ? 0 : e0 / (D / 2), g1 = groups == 1 ? 0 : e1 / (D / 2);
-  float inv[2], off[2];
+  float c[8];
 #pragma unroll
-  for (int q = 0; q < 2; ++q) off[q] = inv[q] = 0.0f;
+  for (int i = 0; i < 8; ++i) c[i] = fminf(fmaxf(x[i], -kMaxF16), kMaxF16) + (x[i] - x[i]);   // NaN where not finite
+  float inv[2] = {0.0f, 0.0f}, off[2] = {0.0f, 0.0f};
   for (int g = 0; g < groups; ++g) {
     float lo = INFINITY, hi = -INFINITY;
-    bool bad = false;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if ((i < 4 ? g0 : g1) != g) continue;
-      bad |= !(fabsf(x[i]) < INFINITY);
-      const float c = fminf(fmaxf(x[i], -kMaxF16), kMaxF16);
-      lo = fminf(lo, c);
-      hi = fmaxf(hi, c);
+      lo = min_nan(lo, c[i]);
+      hi = max_nan(hi, c[i]);
     }
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      bad |= __shfl_xor_sync(0xffffffffu, bad ? 1 : 0, o) != 0;
+      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    const __half ho = bad ? __ushort_as_half(0x7fffu) : __float2half_rn(lo);
+    const __half ho = __float2half_rn(lo);
     const float fo = __half2float(ho);
     __half hs = __float2half_rn(__fdiv_rn(__fsub_rn(hi, fo), 15.0f));
     if (!(__half2float(hs) > 0.0f)) hs = __float2half_rn(1.0f);
@@ -119,8 +130,7 @@ __device__ __forceinline__ void quantise_row(const float (&x)[8], int e0, int e1
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float c = fminf(fmaxf(x[4 * q + i], -kMaxF16), kMaxF16);
-      const float r = rintf(__fmul_rn(__fsub_rn(c, off[q]), inv[q]));
+      const float r = rintf(__fmul_rn(__fsub_rn(c[4 * q + i], off[q]), inv[q]));
       w |= static_cast<uint32_t>(fminf(fmaxf(r, 0.0f), 15.0f)) << (4 * i);   // NaN: code 0
     }
     if (store) *reinterpret_cast<uint16_t*>(codes + (q ? e1 : e0) / 2) = static_cast<uint16_t>(w);
@@ -128,7 +138,7 @@ __device__ __forceinline__ void quantise_row(const float (&x)[8], int e0, int e1
 }
 
 template <typename T, int D, bool APPEND>
-__global__ void __launch_bounds__(ROPE_THREADS) qk_norm_rope_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(ROPE_THREADS, 3) qk_norm_rope_kernel(const RopeParams p) {
   constexpr int L = D / 8;
   const int l = threadIdx.x % L;
   long long g = (static_cast<long long>(blockIdx.x) * ROPE_THREADS + threadIdx.x) / L;
@@ -142,7 +152,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) qk_norm_rope_kernel(const RopePa
   const int e0 = turns && !p.interleaved ? 4 * l : 8 * l;
   const int e1 = turns && !p.interleaved ? p.rot / 2 + 4 * l : 8 * l + 4;
 
-  float x[UN][8];
+  uint2 raw[UN][2];
 #pragma unroll
   for (int u = 0; u < UN; ++u) {
     const int h = first + u;
@@ -153,12 +163,10 @@ __global__ void __launch_bounds__(ROPE_THREADS) qk_norm_rope_kernel(const RopePa
       src = static_cast<const T*>(p.k) + t * p.k_st + (h - p.heads) * p.k_sh;
     else if (APPEND && h < items)
       src = static_cast<const T*>(p.v) + t * p.v_st + (h - p.heads - p.kv_heads) * p.v_sh;
+    raw[u][0] = raw[u][1] = make_uint2(0, 0);
     if (src != nullptr) {
-      load_quad<T>(src + e0, p.vec, x[u]);
-      load_quad<T>(src + e1, p.vec, x[u] + 4);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[u][i] = 0.0f;
+      raw[u][0] = load_quad<T>(src + e0, p.vec);
+      raw[u][1] = load_quad<T>(src + e1, p.vec);
     }
   }
 
@@ -171,12 +179,10 @@ __global__ void __launch_bounds__(ROPE_THREADS) qk_norm_rope_kernel(const RopePa
       pos = 0;
     }
     if (p.axes == 1) {
-      const float* row = p.cos_sin + pos * p.rot;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        cs[i] = __ldg(row + f + i);
-        sn[i] = __ldg(row + p.rot / 2 + f + i);
-      }
+      const float4 c4 = __ldg(reinterpret_cast<const float4*>(p.cos_sin + pos * p.rot + f));
+      const float4 s4 = __ldg(reinterpret_cast<const float4*>(p.cos_sin + pos * p.rot + p.rot / 2 + f));
+      cs[0] = c4.x; cs[1] = c4.y; cs[2] = c4.z; cs[3] = c4.w;
+      sn[0] = s4.x; sn[1] = s4.y; sn[2] = s4.z; sn[3] = s4.w;
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -207,40 +213,51 @@ __global__ void __launch_bounds__(ROPE_THREADS) qk_norm_rope_kernel(const RopePa
     }
   }
 
+  const void* w_held = nullptr;
+  float wv[8];
 #pragma unroll
   for (int u = 0; u < UN; ++u) {
     const int h = first + u;
     const bool is_q = h < p.heads, is_k = !is_q && h < p.heads + p.kv_heads;
     const void* w = is_q ? p.qw : is_k ? p.kw : nullptr;
+    float x[8];
+    quad_f32<T>(raw[u][0], x);
+    quad_f32<T>(raw[u][1], x + 4);
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(x[u][i], x[u][i], sum);
+    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (w != nullptr) {
+      if (w != w_held) {       // the group's heads are mostly of one kind
+        w_held = w;
+        if (p.w_f32) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) wv[i] = __ldg(static_cast<const float*>(w) + (i < 4 ? e0 : e1 - 4) + i);
+        } else {
+          quad_f32<T>(load_quad<T>(static_cast<const T*>(w) + e0, p.w_vec), wv);
+          quad_f32<T>(load_quad<T>(static_cast<const T*>(w) + e1, p.w_vec), wv + 4);
+        }
+      }
       const float r = __frcp_rn(__fsqrt_rn(__fadd_rn(sum / D, p.eps)));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int e = (i < 4 ? e0 : e1 - 4) + i;
-        const float wv = p.w_f32 ? static_cast<const float*>(w)[e] : to_f32<T>(static_cast<const T*>(w)[e]);
-        x[u][i] = __fmul_rn(__fmul_rn(x[u][i], r), wv);
-      }
+      for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], r), wv[i]);
     }
     if (turns && (is_q || is_k)) {
       if (p.interleaved) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rotate_pair(x[u][2 * i], x[u][2 * i + 1], cs[i], sn[i]);
+        for (int i = 0; i < 4; ++i) rotate_pair(x[2 * i], x[2 * i + 1], cs[i], sn[i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rotate_pair(x[u][i], x[u][i + 4], cs[i], sn[i]);
+        for (int i = 0; i < 4; ++i) rotate_pair(x[i], x[i + 4], cs[i], sn[i]);
       }
     }
     if (is_q || (!APPEND && is_k)) {
       if (live) {
         T* dst = is_q ? static_cast<T*>(p.q_out) + (t * p.heads + h) * D
                       : static_cast<T*>(p.k_out) + (t * p.kv_heads + h - p.heads) * D;
-        store_quad<T>(dst + e0, x[u]);
-        store_quad<T>(dst + e1, x[u] + 4);
+        store_quad<T>(dst + e0, x);
+        store_quad<T>(dst + e1, x + 4);
       }
     }
     if constexpr (APPEND) {
@@ -255,7 +272,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) qk_norm_rope_kernel(const RopePa
         uint32_t* pairs = store ? reinterpret_cast<uint32_t*>(blk + (is_k ? key_pairs_at(D) : value_pairs_at(D, p.groups))) +
                                       tok * p.groups
                                 : nullptr;
-        quantise_row<D>(x[u], e0, e1, p.groups, store, codes, pairs);
+        quantise_row<D>(x, e0, e1, p.groups, store, codes, pairs);
       }
     }
   }

@@ -106,8 +106,15 @@ class KV4Pages:
 
     def like(self) -> "KV4Pages":
         """Tables of the same shape, not initialised."""
-        return KV4Pages(torch.empty_like(self.refs), torch.empty_like(self.block_table),
-                        torch.empty_like(self.kv_lens), self.page_size)
+        new = object.__new__(KV4Pages)
+        P, (R, W) = self.refs.shape[0], self.block_table.shape
+        buf = self.refs.new_empty(R * W + P + R)      # one allocation; the table first, for its alignment
+        new.block_table, new.refs, new.kv_lens = buf[:R * W].view(R, W), buf[R * W:R * W + P], buf[R * W + P:]
+        new.page_size = self.page_size
+        at = buf.data_ptr()
+        new._struct = _lib.KV4TablesStruct(at + 4 * R * W, at, at + 4 * (R * W + P), P, R, W, self.page_size)
+        new._ref = ctypes.byref(new._struct)
+        return new
 
 
 def _on(device_index: int, fn, *args) -> None:
@@ -132,9 +139,27 @@ def _check_heads(name: str, x: Tensor, like: Tensor | None = None) -> None:
             f"{name} must match q in tokens and head_dim: {tuple(x.shape)} and {tuple(like.shape)}")
 
 
-def _rope_args(q: Tensor, positions: Tensor, cos_sin: Tensor, q_weight, k_weight, sections, D: int):
-    """Checked (axes, end0, end1, weight code) of a rotation."""
-    d, T = q.get_device(), q.shape[0]
+def _rope_args(q: Tensor, k: Tensor, v: Tensor | None, positions: Tensor, cos_sin: Tensor, q_weight, k_weight, sections):
+    """Checked (axes, end0, end1, weight code) of a rotation. The common case is one expression; anything
+    else goes through the checks one by one, which say what is wrong."""
+    d, dt, qs, ks, cs = q.get_device(), q.dtype, q.shape, k.shape, cos_sin.shape
+    if (sections is None and d >= 0 and dt in _CODES and len(qs) == 3 and len(ks) == 3 and len(cs) == 2
+            and k.dtype is dt and k.get_device() == d and ks[0] == qs[0] and ks[2] == qs[2] and qs[2] in (64, 128)
+            and q.stride(2) == 1 and k.stride(2) == 1 and cos_sin.dtype is _F32 and cos_sin.is_contiguous()
+            and cos_sin.get_device() == d and cs[1] % 8 == 0 and 0 < cs[1] <= qs[2] and cs[0] > 0
+            and positions.dtype is _I64 and positions.shape == qs[:1] and positions.is_contiguous()
+            and positions.get_device() == d
+            and (v is None or (v.dtype is dt and v.shape == ks and v.get_device() == d and v.stride(2) == 1))
+            and (q_weight is None or (q_weight.dtype is dt and q_weight.shape == qs[2:] and q_weight.get_device() == d
+                                      and q_weight.is_contiguous()))
+            and (k_weight is None or (k_weight.dtype is dt and k_weight.shape == qs[2:] and k_weight.get_device() == d
+                                      and k_weight.is_contiguous()))):
+        return 1, 0, 0, _CODES[dt]
+    _check_heads("q", q)
+    _check_heads("k", k, q)
+    if v is not None:
+        _check_heads("v", v, q)
+    T, D = q.shape[0], q.shape[2]
     rot = cos_sin.shape[-1]
     assert D in (64, 128), f"head_dim={D} must be 64 or 128"
     assert cos_sin.dtype is _F32 and cos_sin.dim() == 2 and cos_sin.is_contiguous() and cos_sin.get_device() == d, (
@@ -192,12 +217,9 @@ def qk_norm_rope(q: Tensor, k: Tensor, positions: Tensor, cos_sin: Tensor, q_wei
     Returns:
         (q, k) dense, of q's type: fp32 arithmetic, rounded once.
     """
-    _check_heads("q", q)
-    _check_heads("k", k, q)
+    axes, end0, end1, wcode = _rope_args(q, k, None, positions, cos_sin, q_weight, k_weight, sections)
     T, H, D = q.shape
-    axes, end0, end1, wcode = _rope_args(q, positions, cos_sin, q_weight, k_weight, sections, D)
-    qo = _out_like(q, None if out is None else out[0])
-    ko = _out_like(k, None if out is None else out[1])
+    qo, ko = (_out_like(q, None), _out_like(k, None)) if out is None else (_out_like(q, out[0]), _out_like(k, out[1]))
     qs, ks = q.stride(), k.stride()
     _on(q.get_device(), _lib.lib().w4a16_qk_norm_rope, q.data_ptr(), k.data_ptr(), _CODES[q.dtype], T, H, k.shape[1], D,
         qs[0], qs[1], ks[0], ks[1], positions.data_ptr(), axes, end0, end1, cos_sin.data_ptr(), cos_sin.shape[0],
@@ -214,18 +236,15 @@ def qk_norm_rope_append(q: Tensor, k: Tensor, v: Tensor, cache: KV4Cache, layer:
 
     ``slots`` int64 [T] says where: page * page_size + place in the page (negative: this token is not
     cached); no slot twice in one call. Returns the queries [T, heads, D]."""
-    _check_heads("q", q)
-    _check_heads("k", k, q)
-    _check_heads("v", v, q)
+    axes, end0, end1, wcode = _rope_args(q, k, v, positions, cos_sin, q_weight, k_weight, sections)
     T, H, D = q.shape
     d = q.get_device()
-    cache._check_layer(layer)
+    assert 0 <= layer < cache.num_layers, f"layer={layer} out of range for {cache.num_layers} layers"
     assert k.shape[1] == cache.num_kv_heads and v.shape[1] == cache.num_kv_heads and D == cache.head_dim, (
         f"k and v must have the cache's {cache.num_kv_heads} heads of {cache.head_dim}")
     assert cache._index == d, "the cache must be on q's device"
     assert slots.dtype is _I64 and slots.shape == (T,) and slots.is_contiguous() and slots.get_device() == d, (
         f"slots must be a contiguous int64 [{T}] tensor on q's device")
-    axes, end0, end1, wcode = _rope_args(q, positions, cos_sin, q_weight, k_weight, sections, D)
     qo = _out_like(q, out)
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     _on(d, _lib.lib().w4a16_qk_norm_rope_append, q.data_ptr(), k.data_ptr(), v.data_ptr(), _CODES[q.dtype], T, H, qs[0],
@@ -243,7 +262,7 @@ def kv4_gather(cache: KV4Cache, layer: int, slots: Tensor, dtype: torch.dtype = 
     assert slots.dtype is _I64 and slots.dim() == 1 and slots.is_contiguous() and slots.get_device() == cache._index, (
         "slots must be a contiguous int64 [n] tensor on the cache's device")
     n = slots.shape[0]
-    out = torch.empty((2, n, cache.num_kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
+    out = cache.pool.new_empty((2, n, cache.num_kv_heads, cache.head_dim), dtype=dtype)
     _on(cache._index, _lib.lib().w4a16_kv4_gather, cache._ref, layer, slots.data_ptr(), n, out.data_ptr(), _CODES[dtype])
     return out
 
@@ -364,7 +383,7 @@ def kv4_reserve(pages: KV4Pages, rows: Tensor, lens: Tensor) -> Tensor:
     n = rows.shape[0] if rows.dim() == 1 else -1
     _ints("rows", rows, n, d)
     _ints("lens", lens, n, d)
-    buf = torch.empty(2 * n + 1, dtype=_I32, device=d)
+    buf = pages.refs.new_empty(2 * n + 1)
     _on(d, _lib.lib().w4a16_kv4_reserve, pages._ref, rows.data_ptr(), lens.data_ptr(), n, buf.data_ptr(),
         buf.data_ptr() + 4 * n)
     return buf[:n]
@@ -381,7 +400,7 @@ def kv4_fork(cache: KV4Cache, pages: KV4Pages, parents: Tensor, children: Tensor
     _ints("parents", parents, n, cache._index)
     _ints("children", children, n, cache._index)
     out = _tables_out(pages, out)
-    buf = torch.empty(3 * n, dtype=_I32, device=cache._index)
+    buf = pages.refs.new_empty(3 * n)
     _on(cache._index, _lib.lib().w4a16_kv4_fork, cache._ref, pages._ref, out._ref, parents.data_ptr(), children.data_ptr(),
         n, buf.data_ptr(), buf.data_ptr() + 4 * n)
     return out, buf[:n]
@@ -404,6 +423,6 @@ def kv4_compact(cache: KV4Cache, pages: KV4Pages, *, out: KV4Pages | None = None
     (new ones, or ``out``, which may be ``pages``)."""
     _check_pages(cache, pages)
     out = _tables_out(pages, out)
-    scratch = torch.empty(2 * cache.num_pages + 1, dtype=_I32, device=cache._index)
+    scratch = pages.refs.new_empty(2 * cache.num_pages + 1)
     _on(cache._index, _lib.lib().w4a16_kv4_compact, cache._ref, pages._ref, out._ref, scratch.data_ptr())
     return out
