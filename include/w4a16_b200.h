@@ -435,7 +435,7 @@ int w4a16_p2p_free(void* ptr);
  */
 typedef struct {
   void* pool;
-  int64_t layers, pages;
+  int64_t layers, pages; /* pages * page_size below 2^32 */
   int32_t kv_heads;
   int32_t head_dim;      /* 64 or 128 */
   int32_t page_size;     /* tokens, a multiple of 16, at most 4096 */

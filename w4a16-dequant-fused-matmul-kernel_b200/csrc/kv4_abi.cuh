@@ -14,7 +14,7 @@ namespace {
 int check_cache(const w4a16_kv4_cache* c, DeviceState** dev) {
   if (c == nullptr || c->layers < 1 || c->pages < 1 || c->pages > 0x7fffffffLL || c->kv_heads < 1 ||
       c->kv_heads > 65535 || (c->head_dim != 64 && c->head_dim != 128) || c->page_size < BLK ||
-      c->page_size % BLK != 0 || c->page_size > 4096 || (c->group_size != 64 && c->group_size != c->head_dim))
+      c->page_size % BLK != 0 || c->page_size > 4096 || c->pages * c->page_size > 0xffffffffLL || (c->group_size != 64 && c->group_size != c->head_dim))
     return W4A16_ERR_INVALID;
   if (c->pool == nullptr) return W4A16_ERR_INVALID;
   if (!aligned16(c->pool)) return W4A16_ERR_ALIGNMENT;
@@ -121,7 +121,7 @@ int rope(const RopeArgs& a, void* q_out, void* k_out, const w4a16_kv4_cache* cac
   };
   p.vec = quads(a.q, a.q_st, a.q_sh) && quads(a.k, a.k_st, a.k_sh) && (!append || quads(a.v, a.v_st, a.v_sh));
   p.w_vec = reinterpret_cast<uintptr_t>(a.qw) % 8 == 0 && reinterpret_cast<uintptr_t>(a.kw) % 8 == 0;
-  if (p.T * p.chunks * (a.head_dim / 8) / ROPE_THREADS >= 0x7fffffffLL) return W4A16_ERR_INVALID;
+  if (p.T * p.chunks > 0x7fffffffLL) return W4A16_ERR_INVALID;   // the kernel counts groups in 32 bits
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a.dtype == W4A16_DTYPE_F16) {
     if (append) launch_rope<__half, true>(p, a.head_dim, s);
@@ -363,9 +363,8 @@ int w4a16_kv4_gather(const w4a16_kv4_cache* cache, int64_t layer, const int64_t*
   p.out = out;
   p.cache = kv4::view_of(*cache, layer);
   p.groups = cache->head_dim / cache->group_size;
-  const long long blocks = (n * cache->kv_heads * (cache->head_dim / 8) + 255) / 256;
-  if (blocks > 0x7fffffffLL) return W4A16_ERR_INVALID;
-  const unsigned grid = static_cast<unsigned>(blocks);
+  if (n * cache->kv_heads > 0x7fffffffLL) return W4A16_ERR_INVALID;   // counted in 32 bits
+  const unsigned grid = static_cast<unsigned>((n * cache->kv_heads * (cache->head_dim / 8) + 255) / 256);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == W4A16_DTYPE_F16) {
     if (cache->head_dim == 128) kv4::kv4_gather_kernel<__half, 128><<<grid, 256, 0, s>>>(p);

@@ -65,16 +65,36 @@ __device__ __forceinline__ void quad_f32(const uint2& v, float* x) {
   for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(e[i]);
 }
 
-// Minimum and maximum that are NaN where one of the two is.
+// Minimum of two that is NaN where one of them is.
 __device__ __forceinline__ float min_nan(float a, float b) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
+
+// N values of every lane reduced over the L lanes of a group, each to L / N of its lanes: lane l
+// ends with value l / (L / N). Every step halves the values that a lane still carries, so all N
+// take N - 1 + log2(L / N) shuffles and not N log2(L), and what follows from a value is then
+// computed once per group and not once per lane.
+template <int N, int L, bool SUM>
+__device__ __forceinline__ float reduce_scatter(float (&v)[N]) {
+  static_assert(N <= L, "one value per lane at the end");
+#pragma unroll
+  for (int o = L / 2, n = N; o > 0; o >>= 1, n = n > 1 ? n / 2 : 1) {
+    if (n > 1) {
+      const bool up = threadIdx.x & o;
+#pragma unroll
+      for (int i = 0; i < n / 2; ++i) {
+        const float got = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + n / 2], o);
+        const float own = up ? v[i + n / 2] : v[i];
+        v[i] = SUM ? own + got : min_nan(own, got);
+      }
+    } else {
+      const float got = __shfl_xor_sync(0xffffffffu, v[0], o);
+      v[0] = SUM ? v[0] + got : min_nan(v[0], got);
+    }
+  }
+  return v[0];
 }
 
 template <typename T>
@@ -91,49 +111,68 @@ __device__ __forceinline__ void rotate_pair(float& a, float& b, float cs, float 
   b = __fadd_rn(__fmul_rn(y, cs), __fmul_rn(x, sn));
 }
 
-// A lane's quads (channels e0 .. e0 + 3 and e1 .. e1 + 3) of one head quantised into its token's
-// row; every lane of the warp calls it (`store` says which have something to write).
-template <int D>
-__device__ __forceinline__ void quantise_row(const float (&x)[8], int e0, int e1, int groups, bool store,
-                                             uint8_t* codes, uint32_t* pairs) {
-  constexpr int L = D / 8;
-  const int g0 = groups == 1 ? 0 : e0 / (D / 2), g1 = groups == 1 ? 0 : e1 / (D / 2);
-  float c[8];
+// A lane's quads (channels e0 .. e0 + 3 and e1 .. e1 + 3) of UN heads quantised into their
+// token's rows; every lane of the warp calls it. `row(h)` gives the block of head first + h, or
+// null where nothing is to be stored, and `is_key(h)` its half of the block.
+template <int D, int GROUPS, typename Row, typename IsKey>
+__device__ __forceinline__ void quantise_rows(const float (&x)[UN][8], int e0, int e1, int tok, Row row,
+                                              IsKey is_key) {
+  constexpr int L = D / 8, N = UN * GROUPS * 2, R = L / N;
+  const int l = threadIdx.x % L;
+  const int g0 = GROUPS == 1 ? 0 : e0 / (D / 2), g1 = GROUPS == 1 ? 0 : e1 / (D / 2);
+  float stat[N];                 // [head][group][minimum, -maximum]
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = fminf(fmaxf(x[i], -kMaxF16), kMaxF16) + (x[i] - x[i]);   // NaN where not finite
-  float inv[2] = {0.0f, 0.0f}, off[2] = {0.0f, 0.0f};
-  for (int g = 0; g < groups; ++g) {
-    float lo = INFINITY, hi = -INFINITY;
+  for (int u = 0; u < UN; ++u) {
+    float lo[2], hi[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if ((i < 4 ? g0 : g1) != g) continue;
-      lo = min_nan(lo, c[i]);
-      hi = max_nan(hi, c[i]);
+    for (int q = 0; q < 2; ++q) {
+      const float* c = x[u] + 4 * q;
+      lo[q] = min_nan(min_nan(c[0], c[1]), min_nan(c[2], c[3]));
+      hi[q] = min_nan(min_nan(-c[0], -c[1]), min_nan(-c[2], -c[3]));
     }
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) {
-      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    for (int g = 0; g < GROUPS; ++g) {
+      stat[(u * GROUPS + g) * 2] = min_nan(g0 == g ? lo[0] : INFINITY, g1 == g ? lo[1] : INFINITY);
+      stat[(u * GROUPS + g) * 2 + 1] = min_nan(g0 == g ? hi[0] : INFINITY, g1 == g ? hi[1] : INFINITY);
     }
-    const __half ho = __float2half_rn(lo);
-    const float fo = __half2float(ho);
-    __half hs = __float2half_rn(__fdiv_rn(__fsub_rn(hi, fo), 15.0f));
-    if (!(__half2float(hs) > 0.0f)) hs = __float2half_rn(1.0f);
-    const float fi = __frcp_rn(__half2float(hs));
-    if (g0 == g) { off[0] = fo; inv[0] = fi; }
-    if (g1 == g) { off[1] = fo; inv[1] = fi; }
-    if (store && threadIdx.x % L == 0)
-      pairs[g] = static_cast<uint32_t>(__half_as_ushort(hs)) | (static_cast<uint32_t>(__half_as_ushort(ho)) << 16);
+  }
+  const float mine = reduce_scatter<N, L, false>(stat);
+  const float other = __shfl_xor_sync(0xffffffffu, mine, R);
+  const int j = l / R;           // this lane's group: j / 2, of head j / 2 / GROUPS
+  float lo = j & 1 ? other : mine, hi = -(j & 1 ? mine : other);
+  const bool finite = fabsf(lo) < INFINITY && fabsf(hi) < INFINITY;
+  lo = finite ? fminf(fmaxf(lo, -kMaxF16), kMaxF16) : NAN;
+  hi = fminf(fmaxf(hi, -kMaxF16), kMaxF16);
+  const __half ho = __float2half_rn(lo);
+  const float fo = __half2float(ho);
+  __half hs = __float2half_rn(__fdiv_rn(__fsub_rn(hi, fo), 15.0f));
+  if (!(__half2float(hs) > 0.0f)) hs = __float2half_rn(1.0f);
+  const float fi = __frcp_rn(__half2float(hs));
+  {
+    const int u = j / 2 / GROUPS;
+    uint8_t* blk = row(u);
+    if (blk != nullptr && l % (2 * R) == 0)
+      reinterpret_cast<uint32_t*>(blk + (is_key(u) ? key_pairs_at(D) : value_pairs_at(D, GROUPS)))[tok * GROUPS + j / 2 % GROUPS] =
+          static_cast<uint32_t>(__half_as_ushort(hs)) | (static_cast<uint32_t>(__half_as_ushort(ho)) << 16);
   }
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    uint32_t w = 0;
+  for (int u = 0; u < UN; ++u) {
+    uint8_t* blk = row(u);
+    const int at = (is_key(u) ? 0 : value_codes_at(D)) + tok * (D / 2);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float r = rintf(__fmul_rn(__fsub_rn(c[4 * q + i], off[q]), inv[q]));
-      w |= static_cast<uint32_t>(fminf(fmaxf(r, 0.0f), 15.0f)) << (4 * i);   // NaN: code 0
+    for (int q = 0; q < 2; ++q) {
+      const int from = (u * GROUPS + (q ? g1 : g0)) * 2 * R;
+      const float off = __shfl_sync(0xffffffffu, fo, from, L), inv = __shfl_sync(0xffffffffu, fi, from, L);
+      // rounding by the addition of 2^23: the code is what the sum's low bits hold
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 3; i >= 0; --i) {
+        const float c = fminf(fmaxf(x[u][4 * q + i], -kMaxF16), kMaxF16);
+        const float r = fminf(fmaxf(__fmul_rn(__fsub_rn(c, off), inv), 0.0f), 15.0f);   // NaN: code 0
+        w = w * 16 + __float_as_uint(__fadd_rn(r, 8388608.0f));
+      }
+      if (blk != nullptr) *reinterpret_cast<uint16_t*>(blk + at + (q ? e1 : e0) / 2) = static_cast<uint16_t>(w);
     }
-    if (store) *reinterpret_cast<uint16_t*>(codes + (q ? e1 : e0) / 2) = static_cast<uint16_t>(w);
   }
 }
 
@@ -141,11 +180,12 @@ template <typename T, int D, bool APPEND>
 __global__ void __launch_bounds__(ROPE_THREADS, 3) qk_norm_rope_kernel(const RopeParams p) {
   constexpr int L = D / 8;
   const int l = threadIdx.x % L;
-  long long g = (static_cast<long long>(blockIdx.x) * ROPE_THREADS + threadIdx.x) / L;
+  uint32_t g = blockIdx.x * (ROPE_THREADS / L) + threadIdx.x / L;
   const bool live = g < p.T * p.chunks;
   if (!live) g = 0;   // stays for the warp's shuffles, stores nothing
-  const long long t = g / p.chunks;
-  const int first = static_cast<int>(g % p.chunks) * UN;
+  const uint32_t token = g / p.chunks;
+  const long long t = token;
+  const int first = (g - token * p.chunks) * UN;
   const int items = p.heads + (APPEND ? 2 : 1) * p.kv_heads;
 
   const bool turns = l < p.rot / 8;
@@ -197,21 +237,16 @@ __global__ void __launch_bounds__(ROPE_THREADS, 3) qk_norm_rope_kernel(const Rop
     }
   }
 
-  long long page = 0;
-  int in_page = 0;
-  bool cached = false;
-  if (APPEND) {
-    const long long slot = p.slots[t];
-    cached = live && slot >= 0;
-    if (cached && slot >= p.cache.pages * p.cache.page_size) {
-      flag_error(kErrIndex);
-      cached = false;
-    }
-    if (cached) {
-      page = slot / p.cache.page_size;
-      in_page = static_cast<int>(slot - page * p.cache.page_size);
-    }
+  float x[UN][8], sums[UN];
+#pragma unroll
+  for (int u = 0; u < UN; ++u) {
+    quad_f32<T>(raw[u][0], x[u]);
+    quad_f32<T>(raw[u][1], x[u] + 4);
+    sums[u] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sums[u] = fmaf(x[u][i], x[u][i], sums[u]);
   }
+  const float norm = __frcp_rn(__fsqrt_rn(__fadd_rn(reduce_scatter<UN, L, true>(sums) / D, p.eps)));
 
   const void* w_held = nullptr;
   float wv[8];
@@ -220,14 +255,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, 3) qk_norm_rope_kernel(const Rop
     const int h = first + u;
     const bool is_q = h < p.heads, is_k = !is_q && h < p.heads + p.kv_heads;
     const void* w = is_q ? p.qw : is_k ? p.kw : nullptr;
-    float x[8];
-    quad_f32<T>(raw[u][0], x);
-    quad_f32<T>(raw[u][1], x + 4);
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float r = __shfl_sync(0xffffffffu, norm, u * (L / UN), L);
     if (w != nullptr) {
       if (w != w_held) {       // the group's heads are mostly of one kind
         w_held = w;
@@ -239,42 +267,56 @@ __global__ void __launch_bounds__(ROPE_THREADS, 3) qk_norm_rope_kernel(const Rop
           quad_f32<T>(load_quad<T>(static_cast<const T*>(w) + e1, p.w_vec), wv + 4);
         }
       }
-      const float r = __frcp_rn(__fsqrt_rn(__fadd_rn(sum / D, p.eps)));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], r), wv[i]);
+      for (int i = 0; i < 8; ++i) x[u][i] = __fmul_rn(__fmul_rn(x[u][i], r), wv[i]);
     }
     if (turns && (is_q || is_k)) {
       if (p.interleaved) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rotate_pair(x[2 * i], x[2 * i + 1], cs[i], sn[i]);
+        for (int i = 0; i < 4; ++i) rotate_pair(x[u][2 * i], x[u][2 * i + 1], cs[i], sn[i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rotate_pair(x[i], x[i + 4], cs[i], sn[i]);
+        for (int i = 0; i < 4; ++i) rotate_pair(x[u][i], x[u][i + 4], cs[i], sn[i]);
       }
     }
     if (is_q || (!APPEND && is_k)) {
       if (live) {
         T* dst = is_q ? static_cast<T*>(p.q_out) + (t * p.heads + h) * D
                       : static_cast<T*>(p.k_out) + (t * p.kv_heads + h - p.heads) * D;
-        store_quad<T>(dst + e0, x);
-        store_quad<T>(dst + e1, x + 4);
+        store_quad<T>(dst + e0, x[u]);
+        store_quad<T>(dst + e1, x[u] + 4);
       }
     }
-    if constexpr (APPEND) {
-      // the lanes of a warp may hold different heads: all of them take part where any has a
-      // key or value head
-      if (__any_sync(0xffffffffu, !is_q && h < items)) {
-        const bool store = cached && !is_q && h < items;
-        const int head = is_k ? h - p.heads : h - p.heads - p.kv_heads;
-        uint8_t* blk = store ? block_ptr(p.cache, page, head, in_page / BLK) : nullptr;
-        const int tok = in_page % BLK;
-        uint8_t* codes = store ? blk + (is_k ? 0 : value_codes_at(D)) + tok * (D / 2) : nullptr;
-        uint32_t* pairs = store ? reinterpret_cast<uint32_t*>(blk + (is_k ? key_pairs_at(D) : value_pairs_at(D, p.groups))) +
-                                      tok * p.groups
-                                : nullptr;
-        quantise_row<D>(x, e0, e1, p.groups, store, codes, pairs);
+  }
+
+  if constexpr (APPEND) {
+    // the lanes of a warp may hold different heads: all of them take part where any has a key
+    // or value head
+    if (!__any_sync(0xffffffffu, first + UN > p.heads)) return;
+    const long long slot = p.slots[t];
+    bool cached = live && slot >= 0;
+    if (cached && slot >= p.cache.pages * p.cache.page_size) {
+      flag_error(kErrIndex);
+      cached = false;
+    }
+    // (below 2^32, as the host checks for the whole layer)
+    const uint32_t block = cached ? static_cast<uint32_t>(slot) / BLK : 0;
+    const uint32_t page = block / p.cache.page_blocks;
+    uint8_t* blk0 = block_ptr(p.cache, page, 0, block - page * p.cache.page_blocks);
+    const auto is_key = [&](int u) { return first + u < p.heads + p.kv_heads; };
+    const auto row = [&](int u) -> uint8_t* {
+      const int h = first + u;
+      if (!cached || h < p.heads || h >= items) return nullptr;
+      return blk0 + (h - p.heads - (is_key(u) ? 0 : p.kv_heads)) * p.cache.page_bytes;
+    };
+    const int tok = static_cast<int>(slot % BLK);
+    if constexpr (D == 128) {
+      if (p.groups == 2) {
+        quantise_rows<D, 2>(x, e0, e1, tok, row, is_key);
+        return;
       }
     }
+    quantise_rows<D, 1>(x, e0, e1, tok, row, is_key);
   }
 }
 
@@ -291,11 +333,11 @@ struct GatherParams {
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_gather_kernel(const GatherParams p) {
   constexpr int L = D / 8;
-  const long long g = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) / L;
   const int l = threadIdx.x % L;
+  const uint32_t g = blockIdx.x * (256 / L) + threadIdx.x / L;
   if (g >= p.n * p.cache.kv_heads) return;
-  const long long t = g / p.cache.kv_heads;
-  const int head = static_cast<int>(g - t * p.cache.kv_heads);
+  const uint32_t t = g / p.cache.kv_heads;
+  const int head = g - t * p.cache.kv_heads;
   long long slot = p.slots[t];
   if (slot >= p.cache.pages * p.cache.page_size) {
     flag_error(kErrIndex);
@@ -303,10 +345,10 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(const GatherParams p) {
   }
   uint32_t word[2] = {0, 0}, pair[2] = {0, 0};
   if (slot >= 0) {
-    const long long page = slot / p.cache.page_size;
-    const int in_page = static_cast<int>(slot - page * p.cache.page_size);
-    const uint8_t* blk = block_ptr(p.cache, page, head, in_page / BLK);
-    const int tok = in_page % BLK;
+    const uint32_t block = static_cast<uint32_t>(slot) / BLK;   // (the host checks for 2^32)
+    const uint32_t page = block / p.cache.page_blocks;
+    const uint8_t* blk = block_ptr(p.cache, page, head, block - page * p.cache.page_blocks);
+    const int tok = static_cast<int>(slot % BLK);
     const int grp = l * 8 / (D / p.groups);
     word[0] = *reinterpret_cast<const uint32_t*>(blk + tok * (D / 2) + 4 * l);
     word[1] = *reinterpret_cast<const uint32_t*>(blk + value_codes_at(D) + tok * (D / 2) + 4 * l);
@@ -320,7 +362,9 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(const GatherParams p) {
     uint32_t* vp = &v.x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float a = static_cast<float>((word[s] >> (8 * i)) & 15u), b = static_cast<float>((word[s] >> (8 * i + 4)) & 15u);
+      // 2^23 + code, exactly, less 2^23
+      const float a = __uint_as_float(0x4B000000u | ((word[s] >> (8 * i)) & 15u)) - 8388608.0f;
+      const float b = __uint_as_float(0x4B000000u | ((word[s] >> (8 * i + 4)) & 15u)) - 8388608.0f;
       vp[i] = pack2<T>(__fadd_rn(__fmul_rn(so.x, a), so.y), __fadd_rn(__fmul_rn(so.x, b), so.y));
     }
     *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + ((s * p.n + t) * p.cache.kv_heads + head) * D + 8 * l) = v;
