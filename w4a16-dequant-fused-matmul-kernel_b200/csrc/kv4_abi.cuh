@@ -12,7 +12,7 @@ namespace {
 
 // The checks every entry point makes of a cache.
 int check_cache(const w4a16_kv4_cache* c, DeviceState** dev) {
-  if (c == nullptr || c->layers < 1 || c->pages < 1 || c->pages > 0x7fffffffLL || c->kv_heads < 1 ||
+  if (c == nullptr || c->layers < 1 || c->layers > 0x7fffffffLL || c->pages < 1 || c->pages > 0x7fffffffLL || c->kv_heads < 1 ||
       c->kv_heads > 65535 || (c->head_dim != 64 && c->head_dim != 128) || c->page_size < BLK ||
       c->page_size % BLK != 0 || c->page_size > 4096 || c->pages * c->page_size > 0xffffffffLL || (c->group_size != 64 && c->group_size != c->head_dim))
     return W4A16_ERR_INVALID;
@@ -27,6 +27,7 @@ CacheView view_of(const w4a16_kv4_cache& c, int64_t layer) {
   v.kv_heads = c.kv_heads;
   v.page_size = c.page_size;
   v.page_blocks = c.page_size / BLK;
+  v.blocks = Divisor(v.page_blocks);
   v.block_bytes = block_bytes(c.head_dim, c.head_dim / c.group_size);
   v.page_bytes = static_cast<long long>(v.page_blocks) * v.block_bytes;
   v.pool = static_cast<uint8_t*>(c.pool) + layer * c.pages * c.kv_heads * v.page_bytes;
@@ -105,7 +106,10 @@ int rope(const RopeArgs& a, void* q_out, void* k_out, const w4a16_kv4_cache* cac
   p.q_out = q_out; p.k_out = k_out;
   p.T = a.T;
   p.heads = a.heads; p.kv_heads = a.kv_heads;
-  p.chunks = (items + UN - 1) / UN;
+  p.q_chunks = (a.heads + UN - 1) / UN;
+  p.k_chunks = (a.kv_heads + UN - 1) / UN;
+  p.chunks = p.q_chunks + (append ? 2 : 1) * p.k_chunks;
+  p.by_chunks = Divisor(p.chunks);
   p.positions = reinterpret_cast<const long long*>(a.positions);
   p.axes = a.axes; p.end0 = a.end0; p.end1 = a.end1;
   p.cos_sin = a.cos_sin;
@@ -302,9 +306,11 @@ void launch_copy(const w4a16_kv4_cache& c, const int* src, const int* dst, const
   p.layers = static_cast<int>(c.layers);
   p.pages = static_cast<int>(c.pages);
   p.src = src; p.dst = dst; p.count = count; p.n = n;
-  const long long work = static_cast<long long>(n) * c.layers;
+  const long long per_part = 16LL * COPY_THREADS * COPY_VECS;
+  p.parts = static_cast<int>((p.copy_bytes + per_part - 1) / per_part);
+  const long long work = static_cast<long long>(n) * c.layers * p.parts;
   const unsigned grid = static_cast<unsigned>(std::min<long long>(work, 8LL * dev.num_sms));
-  kv4_copy_pages_kernel<<<grid, 256, 0, s>>>(p);
+  kv4_copy_pages_kernel<<<grid, COPY_THREADS, 0, s>>>(p);
 }
 
 }  // namespace
@@ -363,6 +369,7 @@ int w4a16_kv4_gather(const w4a16_kv4_cache* cache, int64_t layer, const int64_t*
   p.out = out;
   p.cache = kv4::view_of(*cache, layer);
   p.groups = cache->head_dim / cache->group_size;
+  p.by_heads = kv4::Divisor(cache->kv_heads);
   if (n * cache->kv_heads > 0x7fffffffLL) return W4A16_ERR_INVALID;   // counted in 32 bits
   const unsigned grid = static_cast<unsigned>((n * cache->kv_heads * (cache->head_dim / 8) + 255) / 256);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -16,6 +16,8 @@
 // a block arrives with one contiguous copy of a multiple of 16 bytes.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace w4a16 {
@@ -29,6 +31,19 @@ __host__ __device__ constexpr int value_codes_at(int D) { return BLK * (D / 2); 
 __host__ __device__ constexpr int key_pairs_at(int D) { return BLK * D; }
 __host__ __device__ constexpr int value_pairs_at(int D, int groups) { return BLK * D + BLK * groups * 4; }
 
+// Division of n < 2^31 by a number that the host knows: one multiplication, one addition and one
+// shift, where the instruction sequence of a division takes about twenty.
+// With s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1, n / d = (hi(n m) + n) >> s.
+struct Divisor {
+  uint32_t m, s;
+  Divisor() = default;
+  explicit Divisor(uint32_t d) : m(0), s(0) {
+    while (s < 31 && (1u << s) < d) ++s;
+    m = static_cast<uint32_t>(((((1ull << s) - d) << 32) / d) + 1);
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
+
 // The cache as the kernels see it (one layer's pool for all but the page copies).
 struct CacheView {
   uint8_t* pool;            // first byte of the layer
@@ -36,6 +51,7 @@ struct CacheView {
   int kv_heads;
   int page_size;            // tokens per page
   int page_blocks;          // page_size / 16
+  Divisor blocks;           // by page_blocks
   int block_bytes;
   long long page_bytes;     // bytes of a page of one kv head
 };
@@ -50,18 +66,16 @@ template <>
 __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
 template <>
 __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
 // Two fp32 values rounded to T, packed (lo in the low half).
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  T v[2] = {from_f32<T>(lo), from_f32<T>(hi)};
-  return *reinterpret_cast<uint32_t*>(v);
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
 }
 
 }  // namespace kv4

@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     psrc = 0;
     const int tile = lane / per_tile, blk = pblk + tile * TW * TB + lane % per_tile;
     if (tile < pleft && blk < plast) {
-      const int col = blk / a.cache.page_blocks, page = prow[col];
+      const int col = a.cache.blocks.quotient(blk), page = prow[col];
       if (static_cast<unsigned>(page) < static_cast<unsigned>(a.cache.pages))
         psrc = reinterpret_cast<unsigned long long>(phead + page * (a.cache.kv_heads * a.cache.page_bytes) +
                                                     (blk - col * a.cache.page_blocks) * SH::BLOCK);

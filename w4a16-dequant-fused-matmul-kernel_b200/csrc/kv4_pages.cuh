@@ -56,17 +56,25 @@ struct CopyParams {
   long long layer_bytes;     // bytes of a layer
   long long copy_bytes;      // bytes of a page, all kv heads: a multiple of 16
   int layers, pages;
+  int parts;                 // pieces of a page: at most COPY_THREADS * COPY_VECS uint4 each
   const int *src, *dst;      // [n]; a pair with a negative entry is skipped
   const int* count;          // how many pairs there are, or null: n
   int n;
 };
 
-__global__ void __launch_bounds__(256) kv4_copy_pages_kernel(const CopyParams p) {
+// A page is copied in `parts` near-equal pieces of at most COPY_VECS uint4 a thread, so that each
+// piece's loads are in flight together and a handful of pages still fills the SMs.
+constexpr int COPY_THREADS = 256, COPY_VECS = 4;
+
+__global__ void __launch_bounds__(COPY_THREADS) kv4_copy_pages_kernel(const CopyParams p) {
   const int n = p.count ? min(*p.count, p.n) : p.n;
-  const long long work = static_cast<long long>(n) * p.layers;
+  const long long work = static_cast<long long>(n) * p.layers * p.parts;
+  const long long vecs = p.copy_bytes / 16;
   for (long long w = blockIdx.x; w < work; w += gridDim.x) {
-    const int i = static_cast<int>(w % n);
-    const long long layer = w / n;
+    const long long item = w / p.parts;
+    const int part = static_cast<int>(w - item * p.parts);
+    const long long layer = item / n;
+    const int i = static_cast<int>(item - layer * n);
     const int s = p.src[i], d = p.dst[i];
     if (s < 0 || d < 0) continue;
     if (s >= p.pages || d >= p.pages) {
@@ -76,7 +84,14 @@ __global__ void __launch_bounds__(256) kv4_copy_pages_kernel(const CopyParams p)
     uint8_t* base = p.pool + layer * p.layer_bytes;
     const uint4* from = reinterpret_cast<const uint4*>(base + s * p.copy_bytes);
     uint4* to = reinterpret_cast<uint4*>(base + d * p.copy_bytes);
-    for (long long c = threadIdx.x; c < p.copy_bytes / 16; c += 256) to[c] = from[c];
+    const long long first = part * vecs / p.parts + threadIdx.x, end = (part + 1) * vecs / p.parts;
+    uint4 v[COPY_VECS];
+#pragma unroll
+    for (int c = 0; c < COPY_VECS; ++c)
+      if (first + c * COPY_THREADS < end) v[c] = from[first + c * COPY_THREADS];
+#pragma unroll
+    for (int c = 0; c < COPY_VECS; ++c)
+      if (first + c * COPY_THREADS < end) to[first + c * COPY_THREADS] = v[c];
   }
 }
 

@@ -25,7 +25,7 @@
 namespace w4a16 {
 namespace kv4 {
 
-constexpr int ROPE_THREADS = 256;
+constexpr int ROPE_THREADS = 128;
 constexpr int UN = 4;             // heads of a token per group of lanes
 
 struct RopeParams {
@@ -34,7 +34,8 @@ struct RopeParams {
   void *q_out, *k_out;            // [T, heads, D] dense
   long long T;
   int heads, kv_heads;
-  int chunks;                     // groups per token
+  int chunks, q_chunks, k_chunks; // groups per token; those of queries and of keys (then values)
+  Divisor by_chunks;
   const long long* positions;     // [axes, T]
   int axes, end0, end1;           // frequencies < end0 turn by axis 0, < end1 by axis 1, else axis 2
   const float* cos_sin;           // [max_pos, rot]: cosines, then sines
@@ -59,10 +60,10 @@ __device__ __forceinline__ uint2 load_quad(const T* src, int vec) {
   return make_uint2(v[0] | static_cast<uint32_t>(v[1]) << 16, v[2] | static_cast<uint32_t>(v[3]) << 16);
 }
 template <typename T>
-__device__ __forceinline__ void quad_f32(const uint2& v, float* x) {
+__device__ __forceinline__ void quad_f32(const uint2& v, float2* x) {
   const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(e[i]);
+  x[0] = make_float2(to_f32<T>(e[0]), to_f32<T>(e[1]));
+  x[1] = make_float2(to_f32<T>(e[2]), to_f32<T>(e[3]));
 }
 
 // Minimum of two that is NaN where one of them is.
@@ -98,25 +99,20 @@ __device__ __forceinline__ float reduce_scatter(float (&v)[N]) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store_quad(T* dst, const float* x) {
+__device__ __forceinline__ void store_quad(T* dst, const float2* x) {
   uint2 v;
-  v.x = pack2<T>(x[0], x[1]);
-  v.y = pack2<T>(x[2], x[3]);
+  v.x = pack2<T>(x[0].x, x[0].y);
+  v.y = pack2<T>(x[1].x, x[1].y);
   *reinterpret_cast<uint2*>(dst) = v;
 }
 
-__device__ __forceinline__ void rotate_pair(float& a, float& b, float cs, float sn) {
-  const float x = a, y = b;
-  a = __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn));
-  b = __fadd_rn(__fmul_rn(y, cs), __fmul_rn(x, sn));
-}
-
 // A lane's quads (channels e0 .. e0 + 3 and e1 .. e1 + 3) of UN heads quantised into their
-// token's rows; every lane of the warp calls it. `row(h)` gives the block of head first + h, or
-// null where nothing is to be stored, and `is_key(h)` its half of the block.
-template <int D, int GROUPS, typename Row, typename IsKey>
-__device__ __forceinline__ void quantise_rows(const float (&x)[UN][8], int e0, int e1, int tok, Row row,
-                                              IsKey is_key) {
+// token's rows; every lane of the warp calls it. `block` is the block of the first head, the
+// next `page_bytes` behind it, `store` how many of them are stored; `at` is where their codes
+// begin in it, `pairs_at` their pairs.
+template <int D, int GROUPS>
+__device__ __forceinline__ void quantise_rows(const float2 (&x)[UN][4], int e0, int e1, int tok, uint8_t* block,
+                                              long long page_bytes, int store, int at, int pairs_at) {
   constexpr int L = D / 8, N = UN * GROUPS * 2, R = L / N;
   const int l = threadIdx.x % L;
   const int g0 = GROUPS == 1 ? 0 : e0 / (D / 2), g1 = GROUPS == 1 ? 0 : e1 / (D / 2);
@@ -126,14 +122,19 @@ __device__ __forceinline__ void quantise_rows(const float (&x)[UN][8], int e0, i
     float lo[2], hi[2];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const float* c = x[u] + 4 * q;
-      lo[q] = min_nan(min_nan(c[0], c[1]), min_nan(c[2], c[3]));
-      hi[q] = min_nan(min_nan(-c[0], -c[1]), min_nan(-c[2], -c[3]));
+      const float2 a = x[u][2 * q], b = x[u][2 * q + 1];
+      lo[q] = min_nan(min_nan(a.x, a.y), min_nan(b.x, b.y));
+      hi[q] = min_nan(min_nan(-a.x, -a.y), min_nan(-b.x, -b.y));
     }
+    if constexpr (GROUPS == 1) {
+      stat[2 * u] = min_nan(lo[0], lo[1]);
+      stat[2 * u + 1] = min_nan(hi[0], hi[1]);
+    } else {
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-      stat[(u * GROUPS + g) * 2] = min_nan(g0 == g ? lo[0] : INFINITY, g1 == g ? lo[1] : INFINITY);
-      stat[(u * GROUPS + g) * 2 + 1] = min_nan(g0 == g ? hi[0] : INFINITY, g1 == g ? hi[1] : INFINITY);
+      for (int g = 0; g < GROUPS; ++g) {
+        stat[(u * GROUPS + g) * 2] = min_nan(g0 == g ? lo[0] : INFINITY, g1 == g ? lo[1] : INFINITY);
+        stat[(u * GROUPS + g) * 2 + 1] = min_nan(g0 == g ? hi[0] : INFINITY, g1 == g ? hi[1] : INFINITY);
+      }
     }
   }
   const float mine = reduce_scatter<N, L, false>(stat);
@@ -148,45 +149,49 @@ __device__ __forceinline__ void quantise_rows(const float (&x)[UN][8], int e0, i
   __half hs = __float2half_rn(__fdiv_rn(__fsub_rn(hi, fo), 15.0f));
   if (!(__half2float(hs) > 0.0f)) hs = __float2half_rn(1.0f);
   const float fi = __frcp_rn(__half2float(hs));
-  {
-    const int u = j / 2 / GROUPS;
-    uint8_t* blk = row(u);
-    if (blk != nullptr && l % (2 * R) == 0)
-      reinterpret_cast<uint32_t*>(blk + (is_key(u) ? key_pairs_at(D) : value_pairs_at(D, GROUPS)))[tok * GROUPS + j / 2 % GROUPS] =
-          static_cast<uint32_t>(__half_as_ushort(hs)) | (static_cast<uint32_t>(__half_as_ushort(ho)) << 16);
-  }
+  if (l % (2 * R) == 0 && j / 2 / GROUPS < store)
+    reinterpret_cast<uint32_t*>(block + j / 2 / GROUPS * page_bytes + pairs_at)[tok * GROUPS + j / 2 % GROUPS] =
+        static_cast<uint32_t>(__half_as_ushort(hs)) | (static_cast<uint32_t>(__half_as_ushort(ho)) << 16);
+  uint8_t* codes = block + at + tok * (D / 2);
 #pragma unroll
   for (int u = 0; u < UN; ++u) {
-    uint8_t* blk = row(u);
-    const int at = (is_key(u) ? 0 : value_codes_at(D)) + tok * (D / 2);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int from = (u * GROUPS + (q ? g1 : g0)) * 2 * R;
-      const float off = __shfl_sync(0xffffffffu, fo, from, L), inv = __shfl_sync(0xffffffffu, fi, from, L);
+      const float off = -__shfl_sync(0xffffffffu, fo, from, L), inv = __shfl_sync(0xffffffffu, fi, from, L);
       // rounding by the addition of 2^23: the code is what the sum's low bits hold
       uint32_t w = 0;
 #pragma unroll
-      for (int i = 3; i >= 0; --i) {
-        const float c = fminf(fmaxf(x[u][4 * q + i], -kMaxF16), kMaxF16);
-        const float r = fminf(fmaxf(__fmul_rn(__fsub_rn(c, off), inv), 0.0f), 15.0f);   // NaN: code 0
-        w = w * 16 + __float_as_uint(__fadd_rn(r, 8388608.0f));
+      for (int i = 1; i >= 0; --i) {
+        float2 c = x[u][2 * q + i];
+        c = make_float2(fminf(fmaxf(c.x, -kMaxF16), kMaxF16), fminf(fmaxf(c.y, -kMaxF16), kMaxF16));
+        c = __fmul2_rn(__fadd2_rn(c, make_float2(off, off)), make_float2(inv, inv));
+        c = make_float2(fminf(fmaxf(c.x, 0.0f), 15.0f), fminf(fmaxf(c.y, 0.0f), 15.0f));   // NaN: code 0
+        c = __fadd2_rn(c, make_float2(8388608.0f, 8388608.0f));
+        w = (w * 16 + __float_as_uint(c.y)) * 16 + __float_as_uint(c.x);
       }
-      if (blk != nullptr) *reinterpret_cast<uint16_t*>(blk + at + (q ? e1 : e0) / 2) = static_cast<uint16_t>(w);
+      if (u < store) *reinterpret_cast<uint16_t*>(codes + u * page_bytes + (q ? e1 : e0) / 2) = static_cast<uint16_t>(w);
     }
   }
 }
 
 template <typename T, int D, bool APPEND>
-__global__ void __launch_bounds__(ROPE_THREADS, 3) qk_norm_rope_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(ROPE_THREADS, 8) qk_norm_rope_kernel(const RopeParams p) {
   constexpr int L = D / 8;
   const int l = threadIdx.x % L;
   uint32_t g = blockIdx.x * (ROPE_THREADS / L) + threadIdx.x / L;
   const bool live = g < p.T * p.chunks;
   if (!live) g = 0;   // stays for the warp's shuffles, stores nothing
-  const uint32_t token = g / p.chunks;
+  const uint32_t token = p.by_chunks.quotient(g);
   const long long t = token;
-  const int first = (g - token * p.chunks) * UN;
-  const int items = p.heads + (APPEND ? 2 : 1) * p.kv_heads;
+  const int chunk = g - token * p.chunks;
+  // a group's heads are all of one kind
+  const bool is_q = chunk < p.q_chunks, is_k = !is_q && chunk < p.q_chunks + p.k_chunks;
+  const int first = (chunk - (is_q ? 0 : is_k ? p.q_chunks : p.q_chunks + p.k_chunks)) * UN;
+  const int count = min(UN, (is_q ? p.heads : p.kv_heads) - first);
+  const long long sh = is_q ? p.q_sh : is_k ? p.k_sh : p.v_sh;
+  const T* src = static_cast<const T*>(is_q ? p.q : is_k ? p.k : p.v) + t * (is_q ? p.q_st : is_k ? p.k_st : p.v_st) +
+                 first * sh;
 
   const bool turns = l < p.rot / 8;
   const int e0 = turns && !p.interleaved ? 4 * l : 8 * l;
@@ -194,24 +199,25 @@ __global__ void __launch_bounds__(ROPE_THREADS, 3) qk_norm_rope_kernel(const Rop
 
   uint2 raw[UN][2];
 #pragma unroll
-  for (int u = 0; u < UN; ++u) {
-    const int h = first + u;
-    const T* src = nullptr;
-    if (h < p.heads)
-      src = static_cast<const T*>(p.q) + t * p.q_st + h * p.q_sh;
-    else if (h < p.heads + p.kv_heads)
-      src = static_cast<const T*>(p.k) + t * p.k_st + (h - p.heads) * p.k_sh;
-    else if (APPEND && h < items)
-      src = static_cast<const T*>(p.v) + t * p.v_st + (h - p.heads - p.kv_heads) * p.v_sh;
-    raw[u][0] = raw[u][1] = make_uint2(0, 0);
-    if (src != nullptr) {
-      raw[u][0] = load_quad<T>(src + e0, p.vec);
-      raw[u][1] = load_quad<T>(src + e1, p.vec);
-    }
+  for (int u = 0; u < UN; ++u) raw[u][0] = raw[u][1] = make_uint2(0, 0);
+  if (p.vec) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+      if (u < count) {
+        raw[u][0] = __ldg(reinterpret_cast<const uint2*>(src + u * sh + e0));
+        raw[u][1] = __ldg(reinterpret_cast<const uint2*>(src + u * sh + e1));
+      }
+  } else {
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+      if (u < count) {
+        raw[u][0] = load_quad<T>(src + u * sh + e0, 0);
+        raw[u][1] = load_quad<T>(src + u * sh + e1, 0);
+      }
   }
 
   float cs[4], sn[4];
-  if (turns) {
+  if (turns && (is_q || is_k)) {
     const int f = 4 * l;
     long long pos = p.positions[t];
     if (pos < 0 || pos >= p.max_pos) {
@@ -237,63 +243,80 @@ __global__ void __launch_bounds__(ROPE_THREADS, 3) qk_norm_rope_kernel(const Rop
     }
   }
 
-  float x[UN][8], sums[UN];
+  float2 x[UN][4];
+  float sums[UN];
 #pragma unroll
   for (int u = 0; u < UN; ++u) {
     quad_f32<T>(raw[u][0], x[u]);
-    quad_f32<T>(raw[u][1], x[u] + 4);
-    sums[u] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sums[u] = fmaf(x[u][i], x[u][i], sums[u]);
+    quad_f32<T>(raw[u][1], x[u] + 2);
   }
-  const float norm = __frcp_rn(__fsqrt_rn(__fadd_rn(reduce_scatter<UN, L, true>(sums) / D, p.eps)));
-
-  const void* w_held = nullptr;
-  float wv[8];
+  const void* w = is_q ? p.qw : is_k ? p.kw : nullptr;
+  if (__any_sync(0xffffffffu, w != nullptr)) {
 #pragma unroll
-  for (int u = 0; u < UN; ++u) {
-    const int h = first + u;
-    const bool is_q = h < p.heads, is_k = !is_q && h < p.heads + p.kv_heads;
-    const void* w = is_q ? p.qw : is_k ? p.kw : nullptr;
-    const float r = __shfl_sync(0xffffffffu, norm, u * (L / UN), L);
-    if (w != nullptr) {
-      if (w != w_held) {       // the group's heads are mostly of one kind
-        w_held = w;
-        if (p.w_f32) {
+    for (int u = 0; u < UN; ++u) {
+      float2 sum = __fmul2_rn(x[u][0], x[u][0]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) wv[i] = __ldg(static_cast<const float*>(w) + (i < 4 ? e0 : e1 - 4) + i);
-        } else {
-          quad_f32<T>(load_quad<T>(static_cast<const T*>(w) + e0, p.w_vec), wv);
-          quad_f32<T>(load_quad<T>(static_cast<const T*>(w) + e1, p.w_vec), wv + 4);
+      for (int i = 1; i < 4; ++i) sum = __ffma2_rn(x[u][i], x[u][i], sum);
+      sums[u] = sum.x + sum.y;
+    }
+    const float norm = __frcp_rn(__fsqrt_rn(__fadd_rn(reduce_scatter<UN, L, true>(sums) / D, p.eps)));
+    float2 wv[4];
+    if (w == nullptr) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) wv[i] = make_float2(1.0f, 1.0f);
+    } else if (p.w_f32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* wf = static_cast<const float*>(w) + (i < 2 ? e0 : e1 - 4) + 2 * i;
+        wv[i] = make_float2(__ldg(wf), __ldg(wf + 1));
+      }
+    } else {
+      quad_f32<T>(load_quad<T>(static_cast<const T*>(w) + e0, p.w_vec), wv);
+      quad_f32<T>(load_quad<T>(static_cast<const T*>(w) + e1, p.w_vec), wv + 2);
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      float r = __shfl_sync(0xffffffffu, norm, u * (L / UN), L);
+      if (w == nullptr) r = 1.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[u][i] = __fmul2_rn(__fmul2_rn(x[u][i], make_float2(r, r)), wv[i]);
+    }
+  }
+  if (turns && (is_q || is_k)) {
+    if (p.interleaved) {
+#pragma unroll
+      for (int u = 0; u < UN; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[u][i] = __fadd2_rn(__fmul2_rn(x[u][i], make_float2(cs[i], cs[i])),
+                               __fmul2_rn(make_float2(x[u][i].y, x[u][i].x), make_float2(-sn[i], sn[i])));
+    } else {
+#pragma unroll
+      for (int u = 0; u < UN; ++u)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 a = x[u][i], b = x[u][i + 2], c = make_float2(cs[2 * i], cs[2 * i + 1]);
+          const float2 s = make_float2(sn[2 * i], sn[2 * i + 1]);
+          x[u][i] = __fadd2_rn(__fmul2_rn(a, c), __fmul2_rn(b, make_float2(-s.x, -s.y)));
+          x[u][i + 2] = __fadd2_rn(__fmul2_rn(b, c), __fmul2_rn(a, s));
         }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[u][i] = __fmul_rn(__fmul_rn(x[u][i], r), wv[i]);
     }
-    if (turns && (is_q || is_k)) {
-      if (p.interleaved) {
+  }
+  if (live && (is_q || !APPEND)) {
+    T* dst = (is_q ? static_cast<T*>(p.q_out) + t * p.heads * D : static_cast<T*>(p.k_out) + t * p.kv_heads * D) + first * D;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rotate_pair(x[u][2 * i], x[u][2 * i + 1], cs[i], sn[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) rotate_pair(x[u][i], x[u][i + 4], cs[i], sn[i]);
+    for (int u = 0; u < UN; ++u)
+      if (u < count) {
+        store_quad<T>(dst + u * D + e0, x[u]);
+        store_quad<T>(dst + u * D + e1, x[u] + 2);
       }
-    }
-    if (is_q || (!APPEND && is_k)) {
-      if (live) {
-        T* dst = is_q ? static_cast<T*>(p.q_out) + (t * p.heads + h) * D
-                      : static_cast<T*>(p.k_out) + (t * p.kv_heads + h - p.heads) * D;
-        store_quad<T>(dst + e0, x[u]);
-        store_quad<T>(dst + e1, x[u] + 4);
-      }
-    }
   }
 
   if constexpr (APPEND) {
-    // the lanes of a warp may hold different heads: all of them take part where any has a key
-    // or value head
-    if (!__any_sync(0xffffffffu, first + UN > p.heads)) return;
-    const long long slot = p.slots[t];
+    // the lanes of a warp may hold different kinds: all of them take part where any has keys or
+    // values
+    if (__all_sync(0xffffffffu, is_q)) return;
+    const long long slot = is_q ? -1 : p.slots[t];
     bool cached = live && slot >= 0;
     if (cached && slot >= p.cache.pages * p.cache.page_size) {
       flag_error(kErrIndex);
@@ -301,22 +324,17 @@ __global__ void __launch_bounds__(ROPE_THREADS, 3) qk_norm_rope_kernel(const Rop
     }
     // (below 2^32, as the host checks for the whole layer)
     const uint32_t block = cached ? static_cast<uint32_t>(slot) / BLK : 0;
-    const uint32_t page = block / p.cache.page_blocks;
-    uint8_t* blk0 = block_ptr(p.cache, page, 0, block - page * p.cache.page_blocks);
-    const auto is_key = [&](int u) { return first + u < p.heads + p.kv_heads; };
-    const auto row = [&](int u) -> uint8_t* {
-      const int h = first + u;
-      if (!cached || h < p.heads || h >= items) return nullptr;
-      return blk0 + (h - p.heads - (is_key(u) ? 0 : p.kv_heads)) * p.cache.page_bytes;
-    };
-    const int tok = static_cast<int>(slot % BLK);
+    const uint32_t page = p.cache.blocks.quotient(block);
+    uint8_t* blk = block_ptr(p.cache, page, first, block - page * p.cache.page_blocks);
+    const int tok = static_cast<int>(slot % BLK), store = cached ? count : 0;
+    const int at = is_k ? 0 : value_codes_at(D);
     if constexpr (D == 128) {
       if (p.groups == 2) {
-        quantise_rows<D, 2>(x, e0, e1, tok, row, is_key);
+        quantise_rows<D, 2>(x, e0, e1, tok, blk, p.cache.page_bytes, store, at, is_k ? key_pairs_at(D) : value_pairs_at(D, 2));
         return;
       }
     }
-    quantise_rows<D, 1>(x, e0, e1, tok, row, is_key);
+    quantise_rows<D, 1>(x, e0, e1, tok, blk, p.cache.page_bytes, store, at, is_k ? key_pairs_at(D) : value_pairs_at(D, 1));
   }
 }
 
@@ -328,6 +346,7 @@ struct GatherParams {
   void* out;
   CacheView cache;
   int groups;
+  Divisor by_heads;
 };
 
 template <typename T, int D>
@@ -336,7 +355,7 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(const GatherParams p) {
   const int l = threadIdx.x % L;
   const uint32_t g = blockIdx.x * (256 / L) + threadIdx.x / L;
   if (g >= p.n * p.cache.kv_heads) return;
-  const uint32_t t = g / p.cache.kv_heads;
+  const uint32_t t = p.by_heads.quotient(g);
   const int head = g - t * p.cache.kv_heads;
   long long slot = p.slots[t];
   if (slot >= p.cache.pages * p.cache.page_size) {
@@ -346,7 +365,7 @@ __global__ void __launch_bounds__(256) kv4_gather_kernel(const GatherParams p) {
   uint32_t word[2] = {0, 0}, pair[2] = {0, 0};
   if (slot >= 0) {
     const uint32_t block = static_cast<uint32_t>(slot) / BLK;   // (the host checks for 2^32)
-    const uint32_t page = block / p.cache.page_blocks;
+    const uint32_t page = p.cache.blocks.quotient(block);
     const uint8_t* blk = block_ptr(p.cache, page, head, block - page * p.cache.page_blocks);
     const int tok = static_cast<int>(slot % BLK);
     const int grp = l * 8 / (D / p.groups);
