@@ -5,30 +5,32 @@
 // the group) of one kv head as two tiles of 128, and 128 tokens at a time (64 with two groups):
 //   warps 0-3, 4-7  softmax of row tile 0 and 1, one row per thread (TMEM lane): queries scaled and
 //                   written to shared memory once; then per step the scores from TMEM, the running
-//                   maximum, probabilities times value scales as fp16 over their scores' columns
-//                   (the A operand of the second product), and at the end the sums, divided
+//                   maximum, probabilities as fp16 over their scores' columns (the A operand of the
+//                   second product), and at the end the sums, divided. One thread of each tile issues
+//                   the tile's tcgen05.mma: O_t += P_t V (P from TMEM, V as it lies, token-major,
+//                   through the transposing descriptor), then S_t = Q_t K^T of the next step
 //   warps 8-11      the cache: a token (or one group of it) per thread, read a step ahead; its codes
-//                   as fp16 into the K and V tiles, its pairs as fp32 beside them
-//   warp 12         issues tcgen05.mma: S_t = Q_t K^T (both operands in shared memory), O_t += P_t V
-//                   (P from TMEM, V as it lies, token-major, through the transposing descriptor)
-// While one row tile's softmax runs, the tensor cores work on the other's products:
-//   PV0(j) QK0(j+1) | PV1(j) QK1(j+1) | ...
-// The products of one thread run in order, so QK_t(j+1) may write over P_t(j) after PV_t(j).
+//                   as fp16 into the K tile, its values as fp16 into the V tile, its key pairs as
+//                   fp32 beside them
+// While one row tile's softmax runs, the tensor cores work on the other's products. The products of
+// one thread run in order, so S_t(j+1) may be written over P_t(j) after O_t(j).
 //
-// As in the decode kernel the tensor cores see codes, not values: a key's scale and offset act on its
-// scores, a value's scale on its probability, in fp32, so the scores carry no rounding of keys
-// (values rounded to fp16 first move a log-sum-exp by some 1e-3 where scores reach 80) and p s is
-// the one rounding to 16 bits. Keys' codes are masked words, c 2^-24 (queries carry the 1/16 of odd
-// nibbles); values' are c - 8, so that what p s loses meets centred numbers, and
-// sum p v = sum (p s)(c - 8) + sum p (b + 8 s). With two groups of channels each has its own product
-// S, probabilities and half of V.
+// As in the decode kernel the tensor cores see a key's codes, and its scale and offset act on its
+// scores in fp32, so the scores carry no rounding of keys (values rounded to fp16 first move a
+// log-sum-exp by some 1e-3 where scores reach 80). The codes are masked words, c 2^-24 (queries carry
+// the 1/16 of odd nibbles). With two groups of channels each has its own product S. A value is
+// rounded once, to fp16, as a 16-bit cache would hold it: 2^-11 of it at most, like its
+// probability. (Value scales on the probabilities instead took two more floats per token and row
+// out of shared memory and three more instructions per score.)
+// A value pair that is not finite becomes zeros in V, where a row that does not see the token would
+// meet it as 0 NaN; the rows that do see it are marked and get NaN in those channels at the end.
 //
 // TMEM columns: S0 128, S1 128 (with P over them), O0 128, O1 128: all 512. Channels lie in the
 // order 0 4 1 5 2 6 3 7 inside each eight (how a masked word gives them): in Q and K alike, which
 // leaves the scores as they are, and in V, which the last step undoes.
 //
-// The probabilities of half a step are taken with the running maximum as it stands, and again in
-// the rare case that some score of the warp's rows exceeds it by kLazyMax: one pass over the scores
+// The probabilities of a step are taken with the running maximum as it stands, and again in the
+// rare case that some score of the warp's rows exceeds it by kLazyMax: one pass over the scores
 // instead of two. Every wait is bounded; on expiry the block raises the device error bit and leaves.
 #pragma once
 
@@ -38,7 +40,7 @@ namespace w4a16 {
 namespace kv4 {
 
 constexpr int PF_ROWS = 256;         // query rows per block (two tiles)
-constexpr int PF_THREADS = 13 * 32;
+constexpr int PF_THREADS = 12 * 32;  // three warps per SM quarter: up to 168 registers a thread
 constexpr int PF_TILE = 128 * 128;   // bytes of a [128][64] fp16 tile
 constexpr int PF_PARS = 4;           // steps whose pairs are kept
 
@@ -69,27 +71,100 @@ struct PrefillShape {
   static constexpr int Q_BYTES = 2 * KB * PF_TILE;
   static constexpr int BLOCK_BYTES = TOK * 128;           // [TOK][64] fp16
   static constexpr int KV_BYTES = KB * BLOCK_BYTES;       // one K or V tile
-  static constexpr int PAR_BYTES = PF_PARS * 128 * 16;
+  static constexpr int PAR_BYTES = PF_PARS * 128 * 8;
   static constexpr int SMEM_BYTES = 1024 + Q_BYTES + 4 * KV_BYTES + PAR_BYTES + 256;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
 };
 
-// One word's eight codes, (0,4) (1,5) (2,6) (3,7): c 2^-24 and 16 c 2^-24 in turn, or c - 8.
+// One word's eight codes, (0,4) (1,5) (2,6) (3,7): c 2^-24 and 16 c 2^-24 in turn.
 __device__ __forceinline__ uint4 masked_word(uint32_t w) {
   const uint32_t u = w >> 8;
   return make_uint4(w & 0x000f000fu, w & 0x00f000f0u, u & 0x000f000fu, u & 0x00f000f0u);
 }
-__device__ __forceinline__ uint4 centred_word(uint32_t w) {
+// Their values offset + scale c, each rounded once; within +-65504 with `clamp`.
+__device__ __forceinline__ uint4 value_word(uint32_t w, __half2 scale, __half2 offset, bool clamp) {
   const uint32_t u = w >> 8;
-  // 1024 + c and 64 + c, less 1032 and 72
-  return make_uint4(hadd2_u32(lop3_and_or(w, 0x000F000Fu, 0x64006400u), 0xE408E408u),
-                    hadd2_u32(lop3_and_or(w, 0x00F000F0u, 0x54005400u), 0xD480D480u),
-                    hadd2_u32(lop3_and_or(u, 0x000F000Fu, 0x64006400u), 0xE408E408u),
-                    hadd2_u32(lop3_and_or(u, 0x00F000F0u, 0x54005400u), 0xD480D480u));
+  // 1024 + c and 64 + c, less 1024 and 64: exact
+  const uint32_t c[4] = {hadd2_u32(lop3_and_or(w, 0x000F000Fu, 0x64006400u), 0xE400E400u),
+                         hadd2_u32(lop3_and_or(w, 0x00F000F0u, 0x54005400u), 0xD400D400u),
+                         hadd2_u32(lop3_and_or(u, 0x000F000Fu, 0x64006400u), 0xE400E400u),
+                         hadd2_u32(lop3_and_or(u, 0x00F000F0u, 0x54005400u), 0xD400D400u)};
+  uint4 o;
+  uint32_t* ow = &o.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&c[i]), scale, offset);
+    if (clamp) v = __hmin2(__hmax2(v, __float2half2_rn(-kMaxF16)), __float2half2_rn(kMaxF16));
+    ow[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return o;
+}
+
+// N columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_ld_cols(uint32_t at, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(at, r); }
+// What was loaded is used after the wait only: the wait takes the registers through.
+template <int N>
+__device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 16)
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
+                   "+r"(r[i + 6]), "+r"(r[i + 7]), "+r"(r[i + 8]), "+r"(r[i + 9]), "+r"(r[i + 10]), "+r"(r[i + 11]),
+                   "+r"(r[i + 12]), "+r"(r[i + 13]), "+r"(r[i + 14]), "+r"(r[i + 15])
+                 :
+                 : "memory");
 }
 
 __device__ __forceinline__ uint8_t* swizzled(uint8_t* tile, int row, int chunk) {
   return tile + row * 128 + ((chunk ^ (row & 7)) << 4);
+}
+
+// A step's probabilities with the maximum m: h in fp16, packed by token pairs, and their sum; returns
+// the largest score over m. The scores of the next columns load meanwhile. EDGE: some row does not
+// see every token; this one sees [rel_from, rel_to) of the step.
+template <int NG, int TOK, bool EDGE>
+__device__ __forceinline__ float step_probabilities(uint32_t s_at, const float4* par, float m, const float (&qs)[NG],
+                                                    int rel_from, int rel_to, uint32_t (&h)[TOK / 2], float& l_add) {
+  constexpr int COLS = 16, CHUNK = TOK / COLS;
+  float top = -INFINITY;
+  float2 sum = make_float2(0.0f, 0.0f);
+  uint32_t x[2][NG][COLS];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) tmem_ld_cols(s_at + g * TOK, x[0][g]);
+#pragma unroll
+  for (int c = 0; c < CHUNK; ++c) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) tmem_ld_done(x[c & 1][g]);
+    if (c + 1 < CHUNK) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) tmem_ld_cols(s_at + g * TOK + (c + 1) * COLS, x[(c + 1) & 1][g]);
+    }
+#pragma unroll
+    for (int i = 0; i < COLS; i += 2) {
+      float4 q[NG];
+      float2 y = make_float2(-m, -m);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        q[g] = par[(c * COLS + i) / 2 * NG + g];
+        y = __ffma2_rn(make_float2(q[g].z, q[g].w), make_float2(qs[g], qs[g]), y);
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+        y = __ffma2_rn(make_float2(__uint_as_float(x[c & 1][g][i]), __uint_as_float(x[c & 1][g][i + 1])),
+                       make_float2(q[g].x, q[g].y), y);
+      if (EDGE) {
+        const int tok = c * COLS + i;
+        if (tok < rel_from || tok >= rel_to) y.x = -INFINITY;
+        if (tok + 1 < rel_from || tok + 1 >= rel_to) y.y = -INFINITY;
+      }
+      top = fmaxf(top, fmaxf(y.x, y.y));
+      const float2 e = make_float2(ex2(y.x), ex2(y.y));
+      sum = __fadd2_rn(sum, e);
+      h[(c * COLS + i) / 2] = pack2<__half>(e.x, e.y);
+    }
+  }
+  l_add = sum.x + sum.y;
+  return top;
 }
 
 template <int D, int NG>
@@ -119,31 +194,32 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   uint8_t* qtile = smem;
   uint8_t* ktile = qtile + SH::Q_BYTES;                   // two buffers, then V's two
   uint8_t* vtile = ktile + 2 * SH::KV_BYTES;
-  float4* pars = reinterpret_cast<float4*>(vtile + 2 * SH::KV_BYTES);   // [PF_PARS][NG][TOK]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(pars + PF_PARS * 128);
+  float4* pars = reinterpret_cast<float4*>(vtile + 2 * SH::KV_BYTES);   // [PF_PARS][TOK / 2][NG]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(pars + PF_PARS * 64);
   uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6;
   uint64_t *sfull = bars + 8, *pfull = bars + 10, *pvdone = bars + 12, *drain = bars + 14;
   uint64_t* parfull = bars + 15;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15 + PF_PARS);
   uint32_t* qmax = tmem_slot + 1;
+  uint4* bad = reinterpret_cast<uint4*>(bars + 16 + PF_PARS);   // [PF_PARS]: tokens whose value pair is not finite
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&kfull[i], 4);
-      mbar_init(&kempty[i], 1);
+      mbar_init(&kempty[i], two ? 2 : 1);
       mbar_init(&vfull[i], 4);
-      mbar_init(&vempty[i], 1);
+      mbar_init(&vempty[i], two ? 2 : 1);
       mbar_init(&sfull[i], 1);
       mbar_init(&pfull[i], 4);
       mbar_init(&pvdone[i], 1);
     }
     for (int i = 0; i < PF_PARS; ++i) mbar_init(&parfull[i], 4);
-    mbar_init(drain, 1);
+    mbar_init(drain, two ? 2 : 1);
     *qmax = 0;
     mbar_fence_init();
   }
-  if (warp == 12) {
+  if (warp == 8) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -214,61 +290,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 12) {
-    // ------------------------------ products ------------------------------
-    if (lane == 0) {
-      const uint32_t qk_desc = umma_idesc_f16_f32(128, TOK), pv_desc = umma_idesc_f16_f32(128, D / NG) | kTransposeB;
-      auto qk = [&](int t, int j) {
-        const uint8_t* q = qtile + t * KB * PF_TILE;
-        const uint8_t* k = ktile + (j & 1) * SH::KV_BYTES;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          const uint64_t qd = umma_desc_sw128(smem_u32(q + kb * PF_TILE)), kd = umma_desc_sw128(smem_u32(k + kb * SH::BLOCK_BYTES));
-          const int g = NG == 2 ? kb : 0;
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma_f16(tmem + t * 128 + g * TOK, qd + kk * 2, kd + kk * 2, qk_desc, (NG == 1 && kb) || kk);
-        }
-        tc_commit(&sfull[t]);
-      };
-      bool ok = true;
-      if (steps > 0) {
-        ok = mbar_wait(&kfull[0], 0, p.wait_ns);
-        tc_fence_after();
-        if (ok) {
-          qk(0, 0);
-          if (two) qk(1, 0);
-          tc_commit(&kempty[0]);
-        }
-      }
-      for (int j = 0; ok && j < steps; ++j) {
-        for (int t = 0; ok && t < (two ? 2 : 1); ++t) {
-          ok = (t || mbar_wait(&vfull[j & 1], (j >> 1) & 1, p.wait_ns)) && mbar_wait(&pfull[t], j & 1, p.wait_ns);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const uint64_t vd = umma_desc_sw128_mn(smem_u32(vtile + (j & 1) * SH::KV_BYTES + g * SH::BLOCK_BYTES), SH::BLOCK_BYTES);
-#pragma unroll
-            for (int kk = 0; kk < TOK / 16; ++kk)
-              tc_mma_f16_ts(tmem + 256 + t * 128 + g * 64, tmem + t * 128 + g * TOK + kk * 8, vd + kk * 128, pv_desc, j || kk);
-          }
-          tc_commit(&pvdone[t]);
-          if (t == 1 || !two) tc_commit(&vempty[j & 1]);
-          if (j + 1 < steps) {
-            if (t == 0) {
-              ok = mbar_wait(&kfull[(j + 1) & 1], ((j + 1) >> 1) & 1, p.wait_ns);
-              if (!ok) break;
-              tc_fence_after();
-            }
-            qk(t, j + 1);
-            if (t == 1 || !two) tc_commit(&kempty[(j + 1) & 1]);
-          }
-        }
-      }
-      tc_commit(drain);
-    }
-  } else if (warp >= 8) {
+  if (warp >= 8) {
     // ------------------------------ the cache ------------------------------
     constexpr int CPT = CHUNKS / NG;                     // eights of channels per thread: one group's
     const int tok = (threadIdx.x - 256) % TOK, g = (threadIdx.x - 256) / TOK;
@@ -300,14 +322,18 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       kp = *reinterpret_cast<const uint32_t*>(blk + key_pairs_at(D) + (tb * NG + g) * 4);
       vp = *reinterpret_cast<const uint32_t*>(blk + value_pairs_at(D, NG) + (tb * NG + g) * 4);
     };
-    auto expand = [&](uint8_t* tile, const uint4 (&codes)[CPT / 4], bool centred) {
+    // the codes of a token as K, or with its scale and offset as V
+    auto expand = [&](bool is_v, uint8_t* tile, const uint4 (&codes)[CPT / 4], __half2 scale, __half2 offset, bool clamp) {
 #pragma unroll
       for (int i = 0; i < CPT / 4; ++i) {
         const uint32_t* w = &codes[i].x;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int c = g * CPT + 4 * i + k;
-          *reinterpret_cast<uint4*>(swizzled(tile + (c >> 3) * SH::BLOCK_BYTES, tok, c & 7)) = centred ? centred_word(w[k]) : masked_word(w[k]);
+          uint4 o;
+          if (is_v) o = value_word(w[k], scale, offset, clamp);
+          else o = masked_word(w[k]);
+          *reinterpret_cast<uint4*>(swizzled(tile + (c >> 3) * SH::BLOCK_BYTES, tok, c & 7)) = o;
         }
       }
       fence_proxy_async_smem();
@@ -325,22 +351,32 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
         vc1[i] = vc[i];
       }
       const float2 ks = __half22float2(*reinterpret_cast<const __half2*>(&kp)), vs = __half22float2(*reinterpret_cast<const __half2*>(&vp));
+      const bool finite = fabsf(vs.x) < INFINITY && fabsf(vs.y) < INFINITY;
+      const uint32_t vp1 = finite ? vp : 0;
+      const bool clamp = __any_sync(0xffffffffu, finite && 15.0f * fabsf(vs.x) + fabsf(vs.y) > kMaxF16);
       load(j + 1, page);
       page = page_of(j + 2);
       // the pairs of step j - PF_PARS have been read: its products were done before step j - 2's V tile
       // was written over
-      pars[((j % PF_PARS) * NG + g) * TOK + tok] = make_float4(ks.x * f, ks.y, vs.x, fmaf(8.0f, vs.x, vs.y));
+      const int slot = j % PF_PARS;
+      float* par = reinterpret_cast<float*>(pars + slot * 64 + (tok >> 1) * NG + g) + (tok & 1);
+      par[0] = ks.x * f;
+      par[2] = ks.y;
+      const uint32_t word = __ballot_sync(0xffffffffu, !finite);
+      if (lane == 0) reinterpret_cast<uint32_t*>(bad + slot)[warp - 8] = word;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&parfull[j % PF_PARS]);
+      if (lane == 0) mbar_arrive(&parfull[slot]);
       ok = mbar_wait_backoff(&kempty[j & 1], ((j >> 1) & 1) ^ 1u, p.wait_ns, 64);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      expand(ktile + (j & 1) * SH::KV_BYTES, kc1, false);
+      const __half2 so = *reinterpret_cast<const __half2*>(&vp1), sc = __low2half2(so), of = __high2half2(so);
+      expand(false, ktile + (j & 1) * SH::KV_BYTES, kc1, sc, of, false);
       if (lane == 0) mbar_arrive(&kfull[j & 1]);
       ok = mbar_wait_backoff(&vempty[j & 1], ((j >> 1) & 1) ^ 1u, p.wait_ns, 64);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      expand(vtile + (j & 1) * SH::KV_BYTES, vc1, true);
+      if (clamp) expand(true, vtile + (j & 1) * SH::KV_BYTES, vc1, sc, of, true);
+      else expand(true, vtile + (j & 1) * SH::KV_BYTES, vc1, sc, of, false);
       if (lane == 0) mbar_arrive(&vfull[j & 1]);
     }
   } else if (warp < 4 || two) {
@@ -355,143 +391,107 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
     const int tile_last = min(last_row, row0 + t * 128 + 127);
     const int all_to = min(len, len - count + (row0 + t * 128) / a.share + 1);
     const int all_from = a.window ? max(0, len - count + tile_last / a.share - a.window + 1) : 0;
-    constexpr int HT = 64 / NG;                          // tokens of half a step
-    float m = 0.0f, l = 0.0f, corr[NG];                  // l = sum p, corr = sum p (b + 8 s)
+    // ---- the tile's products, issued by its first thread
+    const bool issuer = (threadIdx.x & 127) == 0;
+    const uint32_t qk_desc = umma_idesc_f16_f32(128, TOK), pv_desc = umma_idesc_f16_f32(128, D) | kTransposeB;
+    auto qk = [&](int j) {
+      if (!mbar_wait(&kfull[j & 1], (j >> 1) & 1, p.wait_ns)) return false;
+      tc_fence_after();
+      const uint8_t* q = qtile + t * KB * PF_TILE;
+      const uint8_t* k = ktile + (j & 1) * SH::KV_BYTES;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) corr[g] = 0.0f;
+      for (int kb = 0; kb < KB; ++kb) {
+        const uint64_t qd = umma_desc_sw128(smem_u32(q + kb * PF_TILE)), kd = umma_desc_sw128(smem_u32(k + kb * SH::BLOCK_BYTES));
+        const int g = NG == 2 ? kb : 0;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          tc_mma_f16(tmem + t * 128 + g * TOK, qd + kk * 2, kd + kk * 2, qk_desc, (NG == 1 && kb) || kk);
+      }
+      tc_commit(&sfull[t]);
+      tc_commit(&kempty[j & 1]);
+      return true;
+    };
+    auto pv = [&](int j) {
+      if (!mbar_wait(&vfull[j & 1], (j >> 1) & 1, p.wait_ns) || !mbar_wait(&pfull[t], j & 1, p.wait_ns)) return false;
+      tc_fence_after();
+      const uint64_t vd = umma_desc_sw128_mn(smem_u32(vtile + (j & 1) * SH::KV_BYTES), SH::BLOCK_BYTES);
+#pragma unroll
+      for (int kk = 0; kk < TOK / 16; ++kk)
+        tc_mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, vd + kk * 128, pv_desc, j || kk);
+      tc_commit(&pvdone[t]);
+      tc_commit(&vempty[j & 1]);
+      return true;
+    };
+    float m = 0.0f, l = 0.0f;
+    uint32_t nan_groups = 0;         // groups whose values are NaN in some token this row sees
     bool fresh = true, ok = true;
-    // The probabilities of half a step with the maximum m: h = p s in fp16, packed by token pairs, and
-    // what l and corr gain; returns the largest score over m.
-    auto half_step = [&](auto edge_tag, const float4* par, uint32_t s_half, int tok0, uint32_t (&h)[NG][HT / 2],
-                         float& l_add, float (&c_add)[NG]) {
-      constexpr bool EDGE = decltype(edge_tag)::value;
-      float top = -INFINITY;
-      l_add = 0.0f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) c_add[g] = 0.0f;
-#pragma unroll
-      for (int c = 0; c < HT; c += 32) {
-        uint32_t x[NG][32];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) tmem_ld_32x32b_x32(s_half + g * TOK + c, x[g]);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float ps[NG][2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float4 q[NG];
-            float y = -m;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-              q[g] = par[g * TOK + c + i + k];
-              y = fmaf(q[g].y, qs[g], y);
-            }
-#pragma unroll
-            for (int g = 0; g < NG; ++g) y = fmaf(__uint_as_float(x[g][i + k]), q[g].x, y);
-            if (EDGE && (tok0 + c + i + k < see_from || tok0 + c + i + k >= see_to)) y = -INFINITY;
-            top = fmaxf(top, y);
-            const float e = ex2(y);
-            l_add += e;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-              if (EDGE && e == 0.0f) {     // a token that is not seen may have any pair, NaN too
-                ps[g][k] = 0.0f;
-              } else {
-                ps[g][k] = e * q[g].z;
-                c_add[g] = fmaf(e, q[g].w, c_add[g]);
-              }
-            }
-          }
-#pragma unroll
-          for (int g = 0; g < NG; ++g) h[g][(c + i) / 2] = pack2<__half>(ps[g][0], ps[g][1]);
-        }
-      }
-      return top;
-    };
-    auto store_half = [&](uint32_t at, const uint32_t (&h)[HT / 2]) {
-#pragma unroll
-      for (int c = 0; c < HT / 2; c += 16) {
-        uint32_t r[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) r[i] = h[c + i];
-        tmem_st_32x32b_x16(at + c, r);
-      }
-    };
-    for (int j = 0; ok && j < steps; ++j) {
-      ok = mbar_wait(&sfull[t], j & 1, p.wait_ns) && mbar_wait(&parfull[j % PF_PARS], (j / PF_PARS) & 1, p.wait_ns);
+    if (issuer && steps > 0) ok = qk(0);
+    for (int j = 0; j < steps; ++j) {
+      const int slot = j % PF_PARS;
+      ok = ok && mbar_wait(&sfull[t], j & 1, p.wait_ns) && mbar_wait(&parfull[slot], (j / PF_PARS) & 1, p.wait_ns);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       const int tok0 = (step0 + j) * TOK;
       const bool edge = tok0 < all_from || tok0 + TOK > all_to;
-#pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        const float4* par = pars + (j % PF_PARS) * NG * TOK + half * HT;
-        uint32_t h[NG][HT / 2];
-        float l_add, c_add[NG];
-        auto take = [&]() {
-          return edge ? half_step(std::true_type(), par, s_at + half * HT, tok0 + half * HT, h, l_add, c_add)
-                      : half_step(std::false_type(), par, s_at + half * HT, tok0 + half * HT, h, l_add, c_add);
-        };
-        float top = take();
+      const float4* par = pars + slot * 64;
+      uint32_t h[TOK / 2];
+      float l_add;
+      for (int pass = 0; pass < 2; ++pass) {
+        const float top = edge ? step_probabilities<NG, TOK, true>(s_at, par, m, qs, see_from - tok0, see_to - tok0, h, l_add)
+                               : step_probabilities<NG, TOK, false>(s_at, par, m, qs, 0, 0, h, l_add);
         const bool grow = top > (fresh ? -INFINITY : kLazyMax);
-        if (__any_sync(0xffffffffu, grow)) {
-          const float by = grow && !fresh ? ex2(-top) : 1.0f;
-          if (grow) {
-            m += top;
-            fresh = false;
-          }
-          l *= by;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) corr[g] *= by;
-          if (j > 0) {                   // the sums so far
-            ok = __all_sync(0xffffffffu, mbar_wait(&pvdone[t], (j - 1) & 1, p.wait_ns));
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-              uint32_t x[16];
-              tmem_ld_32x32b_x16(o_at + c, x);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * by);
-              tmem_st_32x32b_x16(o_at + c, x);
-            }
-          }
-          if (half) {                    // and this step's first half, stored already
-            tmem_st_wait();
-            const __half2 by2 = __float2half2_rn(by);
-#pragma unroll 1
-            for (int c = 0; c < HT / 2 * NG; c += 16) {
-              uint32_t x[16];
-              const uint32_t at = s_at + c / (HT / 2) * TOK + c % (HT / 2);
-              tmem_ld_32x32b_x16(at, x);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&x[i]), by2);
-                x[i] = *reinterpret_cast<const uint32_t*>(&z);
-              }
-              tmem_st_32x32b_x16(at, x);
-            }
-          }
-          top = take();
+        if (pass || !__any_sync(0xffffffffu, grow)) break;
+        const float by = grow && !fresh ? ex2(-top) : 1.0f;
+        if (grow) {
+          m += top;
+          fresh = false;
         }
-        l += l_add;
+        l *= by;
+        if (j > 0) {                     // the sums so far
+          ok = __all_sync(0xffffffffu, mbar_wait(&pvdone[t], (j - 1) & 1, p.wait_ns));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            uint32_t x[16];
+            tmem_ld_cols(o_at + c, x);
+            tmem_ld_done(x);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          corr[g] += c_add[g];
-          store_half(s_at + g * TOK + half * (HT / 2), h[g]);
+            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * by);
+            tmem_st_32x32b_x16(o_at + c, x);
+          }
         }
       }
       if (!ok) break;
+      l += l_add;
+#pragma unroll
+      for (int c = 0; c < TOK / 2; c += 16) {
+        uint32_t r[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) r[i] = h[c + i];
+        tmem_st_32x32b_x16(s_at + c, r);
+      }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&pfull[t]);
+      if (issuer) ok = pv(j) && (j + 1 >= steps || qk(j + 1));
+      __syncwarp();
+      const uint4 bads = bad[slot];
+      if (bads.x | bads.y | bads.z | bads.w) {
+        const uint32_t words[4] = {bads.x, bads.y, bads.z, bads.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          for (uint32_t left = words[w]; left; left &= left - 1) {
+            const int tok = tok0 + w * 32 % TOK + __ffs(left) - 1;
+            if (tok >= see_from && tok < see_to) nan_groups |= 1u << (w * 32 / TOK);
+          }
+      }
     }
+    if (issuer) tc_commit(drain);
     // ---- the row's result
+    ok = __all_sync(0xffffffffu, ok);
     if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&pvdone[t], (steps - 1) & 1, p.wait_ns));
     tc_fence_after();
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -502,15 +502,16 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       uint32_t x[16];
       __syncwarp();
       if (steps > 0) {
-        tmem_ld_32x32b_x16(o_at + c, x);
-        tmem_ld_wait();
+        tmem_ld_cols(o_at + c, x);
+        tmem_ld_done(x);
       }
+      const bool gone = nan_groups >> (c < D / NG ? 0 : NG - 1) & 1;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         float y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)     // column order 0 4 1 5 2 6 3 7
-          y[(i >> 1) + (i & 1) * 4] = steps > 0 && l != 0.0f ? (__uint_as_float(x[8 * k + i]) + (c < D / NG ? corr[0] : corr[NG - 1])) * inv : 0.0f;
+          y[(i >> 1) + (i & 1) * 4] = gone ? NAN : steps > 0 && l != 0.0f ? __uint_as_float(x[8 * k + i]) * inv : 0.0f;
         uint4 o;
         uint32_t* ow = &o.x;
 #pragma unroll
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 8) {
     mbar_wait(drain, 0, kWaitBudgetNs);   // every product has finished before TMEM is released
     __syncwarp();
     tc_fence_after();
