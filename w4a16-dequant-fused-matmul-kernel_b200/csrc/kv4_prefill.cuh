@@ -2,18 +2,20 @@
 // their chunks): o = softmax(scale q k^T) v on the 5th-generation tensor cores.
 //
 // Compute-bound: 4 D operations per row and token. A block takes 256 rows (query token, head of
-// the group) of one kv head as two tiles of 128, and 128 tokens at a time (64 with two groups):
+// the group) of one kv head as two tiles of 128, and 64 tokens at a time (32 with two groups):
 //   warps 0-3, 4-7  softmax of row tile 0 and 1, one row per thread (TMEM lane): queries scaled and
 //                   written to shared memory once; then per step the scores from TMEM, the running
 //                   maximum, probabilities as fp16 over their scores' columns (the A operand of the
-//                   second product), and at the end the sums, divided. One thread of each tile issues
-//                   the tile's tcgen05.mma: O_t += P_t V (P from TMEM, V as it lies, token-major,
-//                   through the transposing descriptor), then S_t = Q_t K^T of the next step
-//   warps 8-11      the cache: a token (or one group of it) per thread, read a step ahead; its codes
-//                   as fp16 into the K tile, its values as fp16 into the V tile, its key pairs as
-//                   fp32 beside them
-// While one row tile's softmax runs, the tensor cores work on the other's products. The products of
-// one thread run in order, so S_t(j+1) may be written over P_t(j) after O_t(j).
+//                   second product), and at the end the sums, divided
+//   warps 8-11      the cache: a token's keys (8, 9) or values (10, 11), or one group of them, per thread,
+//                   read a step ahead; key codes as fp16 into the K ring, values as fp16 into the V ring,
+//                   key pairs as fp32 beside them
+//   warp 12         issues tcgen05.mma: O_t += P_t V (P from TMEM, V as it lies, token-major, through the
+//                   transposing descriptor), then S_t = Q_t K^T two steps ahead
+// Each tile has two buffers of scores, so its softmax goes on with step j + 1 while the tensor cores
+// take up step j's probabilities and write over them the scores of step j + 2 (the products of one thread
+// run in order). With one buffer of 128 tokens softmax and products took turns: 3700 and 3500 cycles
+// per 128 tokens.
 //
 // As in the decode kernel the tensor cores see a key's codes, and its scale and offset act on its
 // scores in fp32, so the scores carry no rounding of keys (values rounded to fp16 first move a
@@ -25,7 +27,7 @@
 // A value pair that is not finite becomes zeros in V, where a row that does not see the token would
 // meet it as 0 NaN; the rows that do see it are marked and get NaN in those channels at the end.
 //
-// TMEM columns: S0 128, S1 128 (with P over them), O0 128, O1 128: all 512. Channels lie in the
+// TMEM columns: S0 2 x 64, S1 2 x 64 (with P over them), O0 128, O1 128: all 512. Channels lie in the
 // order 0 4 1 5 2 6 3 7 inside each eight (how a masked word gives them): in Q and K alike, which
 // leaves the scores as they are, and in V, which the last step undoes.
 //
@@ -40,9 +42,10 @@ namespace w4a16 {
 namespace kv4 {
 
 constexpr int PF_ROWS = 256;         // query rows per block (two tiles)
-constexpr int PF_THREADS = 12 * 32;  // three warps per SM quarter: up to 168 registers a thread
+constexpr int PF_THREADS = 13 * 32;
 constexpr int PF_TILE = 128 * 128;   // bytes of a [128][64] fp16 tile
-constexpr int PF_PARS = 4;           // steps whose pairs are kept
+constexpr int PF_RING = 4;           // K tiles, and V tiles
+constexpr int PF_PARS = 8;           // steps whose pairs are kept
 
 // B operand as it lies with its N index contiguous: [k][64 n] rows of 128 bytes, 128-byte swizzle, blocks
 // of 64 n `block_bytes` apart, 8-row groups 1024 bytes apart.
@@ -67,12 +70,12 @@ struct PrefillParams {
 template <int D, int NG>
 struct PrefillShape {
   static constexpr int KB = D / 64;                       // 64-channel blocks
-  static constexpr int TOK = 128 / NG;                    // tokens per step
+  static constexpr int TOK = 64 / NG;                     // tokens per step
   static constexpr int Q_BYTES = 2 * KB * PF_TILE;
   static constexpr int BLOCK_BYTES = TOK * 128;           // [TOK][64] fp16
   static constexpr int KV_BYTES = KB * BLOCK_BYTES;       // one K or V tile
-  static constexpr int PAR_BYTES = PF_PARS * 128 * 8;
-  static constexpr int SMEM_BYTES = 1024 + Q_BYTES + 4 * KV_BYTES + PAR_BYTES + 256;
+  static constexpr int PAR_BYTES = PF_PARS * 64 * 8;
+  static constexpr int SMEM_BYTES = 1024 + Q_BYTES + 2 * PF_RING * KV_BYTES + PAR_BYTES + 512;
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
 };
 
@@ -192,34 +195,37 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   // an offset, not a cast: the compiler then knows its loads to be from shared memory
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* qtile = smem;
-  uint8_t* ktile = qtile + SH::Q_BYTES;                   // two buffers, then V's two
-  uint8_t* vtile = ktile + 2 * SH::KV_BYTES;
-  float4* pars = reinterpret_cast<float4*>(vtile + 2 * SH::KV_BYTES);   // [PF_PARS][TOK / 2][NG]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(pars + PF_PARS * 64);
-  uint64_t *kfull = bars, *kempty = bars + 2, *vfull = bars + 4, *vempty = bars + 6;
-  uint64_t *sfull = bars + 8, *pfull = bars + 10, *pvdone = bars + 12, *drain = bars + 14;
-  uint64_t* parfull = bars + 15;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15 + PF_PARS);
+  uint8_t* ktile = qtile + SH::Q_BYTES;                   // K's ring, then V's
+  uint8_t* vtile = ktile + PF_RING * SH::KV_BYTES;
+  float4* pars = reinterpret_cast<float4*>(vtile + PF_RING * SH::KV_BYTES);   // [PF_PARS][TOK / 2][NG]
+  uint2* bad = reinterpret_cast<uint2*>(pars + PF_PARS * 32);     // [PF_PARS]: tokens whose value pair is not finite
+  uint64_t* bars = reinterpret_cast<uint64_t*>(bad + PF_PARS);
+  uint64_t *kfull = bars, *kempty = kfull + PF_RING, *vfull = kempty + PF_RING, *vempty = vfull + PF_RING;
+  uint64_t* parfull = vempty + PF_RING;
+  uint64_t *sfull = parfull + PF_PARS, *pfull = sfull + 4;        // [tile][buffer of S]
+  uint64_t *pvdone = pfull + 4, *drain = pvdone + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   uint32_t* qmax = tmem_slot + 1;
-  uint4* bad = reinterpret_cast<uint4*>(bars + 16 + PF_PARS);   // [PF_PARS]: tokens whose value pair is not finite
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&kfull[i], 4);
-      mbar_init(&kempty[i], two ? 2 : 1);
-      mbar_init(&vfull[i], 4);
-      mbar_init(&vempty[i], two ? 2 : 1);
-      mbar_init(&sfull[i], 1);
-      mbar_init(&pfull[i], 4);
-      mbar_init(&pvdone[i], 1);
+    for (int i = 0; i < PF_RING; ++i) {
+      mbar_init(&kfull[i], 2);
+      mbar_init(&kempty[i], 1);
+      mbar_init(&vfull[i], 2);
+      mbar_init(&vempty[i], 1);
     }
     for (int i = 0; i < PF_PARS; ++i) mbar_init(&parfull[i], 4);
-    mbar_init(drain, two ? 2 : 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&sfull[i], 1);
+      mbar_init(&pfull[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&pvdone[i], 1);
+    mbar_init(drain, 1);
     *qmax = 0;
     mbar_fence_init();
   }
-  if (warp == 8) {
+  if (warp == 12) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -290,37 +296,83 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 8) {
-    // ------------------------------ the cache ------------------------------
+  if (warp == 12) {
+    // ------------------------------ products ------------------------------
+    if (lane == 0) {
+      const uint32_t qk_desc = umma_idesc_f16_f32(128, TOK), pv_desc = umma_idesc_f16_f32(128, D) | kTransposeB;
+      const int tiles = two ? 2 : 1;
+      // S_t of step j into its buffer, after the products that read the probabilities there
+      auto qk = [&](int t, int j) {
+        const uint8_t* q = qtile + t * KB * PF_TILE;
+        const uint8_t* k = ktile + (j % PF_RING) * SH::KV_BYTES;
+        const uint32_t to = tmem + t * 128 + (j & 1) * 64;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const uint64_t qd = umma_desc_sw128(smem_u32(q + kb * PF_TILE)), kd = umma_desc_sw128(smem_u32(k + kb * SH::BLOCK_BYTES));
+          const int g = NG == 2 ? kb : 0;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) tc_mma_f16(to + g * TOK, qd + kk * 2, kd + kk * 2, qk_desc, (NG == 1 && kb) || kk);
+        }
+        tc_commit(&sfull[t * 2 + (j & 1)]);
+        if (t + 1 == tiles) tc_commit(&kempty[j % PF_RING]);
+      };
+      bool ok = true;
+      for (int j = 0; ok && j < min(2, steps); ++j) {
+        ok = mbar_wait(&kfull[j], 0, p.wait_ns);
+        if (!ok) break;
+        tc_fence_after();
+        for (int t = 0; t < tiles; ++t) qk(t, j);
+      }
+      for (int j = 0; ok && j < steps; ++j) {
+        for (int t = 0; ok && t < tiles; ++t) {
+          ok = (t || mbar_wait(&vfull[j % PF_RING], (j / PF_RING) & 1, p.wait_ns)) && mbar_wait(&pfull[t * 2 + (j & 1)], (j >> 1) & 1, p.wait_ns);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t vd = umma_desc_sw128_mn(smem_u32(vtile + (j % PF_RING) * SH::KV_BYTES), SH::BLOCK_BYTES);
+#pragma unroll
+          for (int kk = 0; kk < TOK / 16; ++kk)
+            tc_mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + (j & 1) * 64 + kk * 8, vd + kk * 128, pv_desc, j || kk);
+          tc_commit(&pvdone[t]);
+          if (t + 1 == tiles) tc_commit(&vempty[j % PF_RING]);
+          if (j + 2 < steps) {
+            if (t == 0) {
+              ok = mbar_wait(&kfull[(j + 2) % PF_RING], ((j + 2) / PF_RING) & 1, p.wait_ns);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            qk(t, j + 2);
+          }
+        }
+      }
+      tc_commit(drain);
+    }
+  } else if (warp >= 8) {
+    // ------------------------------ the cache: warps 8, 9 keys, 10, 11 values ------------------------------
     constexpr int CPT = CHUNKS / NG;                     // eights of channels per thread: one group's
-    const int tok = (threadIdx.x - 256) % TOK, g = (threadIdx.x - 256) / TOK;
-    uint4 kc[CPT / 4], vc[CPT / 4];
-    uint32_t kp, vp;
-    auto page_of = [&](int j) {       // the page of this thread's token of step j, or -1
+    const bool values = warp >= 10;
+    const int tok = threadIdx.x % TOK, g = threadIdx.x % 64 / TOK;
+    uint4 next[CPT / 4];
+    uint32_t next_pair;
+    auto wanted = [&](int j, int t) { return j < steps && t < len && t >= from; };
+    auto page_of = [&](int j) {       // the page of this thread's token of step j; looked at when it is used
       const int t = (step0 + j) * TOK + tok;
-      if (j >= steps || t >= len || t < from) return -1;
-      const int page = a.table[static_cast<long long>(b) * a.width + (t / BLK) / a.cache.page_blocks];
-      if (static_cast<unsigned>(page) < static_cast<unsigned>(a.cache.pages)) return page;
-      flag_error(kErrIndex);          // read as zeros
-      return -1;
+      return wanted(j, t) ? a.table[static_cast<long long>(b) * a.width + a.cache.blocks.quotient(t / BLK)] : 0;
     };
     auto load = [&](int j, int page) {
-      const int t = (step0 + j) * TOK + tok;
-      if (page < 0) {
 #pragma unroll
-        for (int i = 0; i < CPT / 4; ++i) kc[i] = vc[i] = make_uint4(0, 0, 0, 0);
-        kp = vp = 0;
+      for (int i = 0; i < CPT / 4; ++i) next[i] = make_uint4(0, 0, 0, 0);
+      next_pair = 0;
+      const int t = (step0 + j) * TOK + tok;
+      if (!wanted(j, t)) return;
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.cache.pages)) {
+        flag_error(kErrIndex);                           // read as zeros
         return;
       }
-      const uint8_t* blk = block_ptr(a.cache, page, kh, t / BLK % a.cache.page_blocks);
-      const int tb = t % BLK;
+      const uint8_t* blk = block_ptr(a.cache, page, kh, t / BLK - a.cache.blocks.quotient(t / BLK) * a.cache.page_blocks);
+      const uint8_t* codes = blk + (values ? value_codes_at(D) : 0) + t % BLK * (D / 2) + g * (CPT * 4);
 #pragma unroll
-      for (int i = 0; i < CPT / 4; ++i) {
-        kc[i] = *reinterpret_cast<const uint4*>(blk + tb * (D / 2) + g * (CPT * 4) + 16 * i);
-        vc[i] = *reinterpret_cast<const uint4*>(blk + value_codes_at(D) + tb * (D / 2) + g * (CPT * 4) + 16 * i);
-      }
-      kp = *reinterpret_cast<const uint32_t*>(blk + key_pairs_at(D) + (tb * NG + g) * 4);
-      vp = *reinterpret_cast<const uint32_t*>(blk + value_pairs_at(D, NG) + (tb * NG + g) * 4);
+      for (int i = 0; i < CPT / 4; ++i) next[i] = *reinterpret_cast<const uint4*>(codes + 16 * i);
+      next_pair = *reinterpret_cast<const uint32_t*>(blk + (values ? value_pairs_at(D, NG) : key_pairs_at(D)) + (t % BLK * NG + g) * 4);
     };
     // the codes of a token as K, or with its scale and offset as V
     auto expand = [&](bool is_v, uint8_t* tile, const uint4 (&codes)[CPT / 4], __half2 scale, __half2 offset, bool clamp) {
@@ -339,45 +391,46 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       fence_proxy_async_smem();
       __syncwarp();
     };
+    uint64_t *full = values ? vfull : kfull, *empty = values ? vempty : kempty;
     int page = page_of(0);
     load(0, page);
     page = page_of(1);
     bool ok = true;
     for (int j = 0; ok && j < steps; ++j) {
-      uint4 kc1[CPT / 4], vc1[CPT / 4];
+      uint4 codes[CPT / 4];
 #pragma unroll
-      for (int i = 0; i < CPT / 4; ++i) {
-        kc1[i] = kc[i];
-        vc1[i] = vc[i];
-      }
-      const float2 ks = __half22float2(*reinterpret_cast<const __half2*>(&kp)), vs = __half22float2(*reinterpret_cast<const __half2*>(&vp));
-      const bool finite = fabsf(vs.x) < INFINITY && fabsf(vs.y) < INFINITY;
-      const uint32_t vp1 = finite ? vp : 0;
-      const bool clamp = __any_sync(0xffffffffu, finite && 15.0f * fabsf(vs.x) + fabsf(vs.y) > kMaxF16);
+      for (int i = 0; i < CPT / 4; ++i) codes[i] = next[i];
+      const uint32_t pair = next_pair;
       load(j + 1, page);
       page = page_of(j + 2);
-      // the pairs of step j - PF_PARS have been read: its products were done before step j - 2's V tile
-      // was written over
-      const int slot = j % PF_PARS;
-      float* par = reinterpret_cast<float*>(pars + slot * 64 + (tok >> 1) * NG + g) + (tok & 1);
-      par[0] = ks.x * f;
-      par[2] = ks.y;
-      const uint32_t word = __ballot_sync(0xffffffffu, !finite);
-      if (lane == 0) reinterpret_cast<uint32_t*>(bad + slot)[warp - 8] = word;
+      const float2 so = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+      const bool finite = fabsf(so.x) < INFINITY && fabsf(so.y) < INFINITY;
+      // The pairs of step j - PF_PARS have been read: this warp has seen step j - 1 - PF_RING leave its
+      // ring, a value tile after that step's probabilities, a key tile after those two steps before it.
+      const int slot = j % PF_PARS, ring = j % PF_RING;
+      uint8_t* tile = (values ? vtile : ktile) + ring * SH::KV_BYTES;
+      if (values) {
+        const uint32_t word = __ballot_sync(0xffffffffu, !finite);
+        if (lane == 0) reinterpret_cast<uint32_t*>(bad + slot)[warp - 10] = word;
+      } else {
+        float* par = reinterpret_cast<float*>(pars + slot * 32 + (tok >> 1) * NG + g) + (tok & 1);
+        par[0] = so.x * f;
+        par[2] = so.y;
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&parfull[slot]);
-      ok = mbar_wait_backoff(&kempty[j & 1], ((j >> 1) & 1) ^ 1u, p.wait_ns, 64);
+      ok = mbar_wait_backoff(&empty[ring], ((j / PF_RING) & 1) ^ 1u, p.wait_ns, 64);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const __half2 so = *reinterpret_cast<const __half2*>(&vp1), sc = __low2half2(so), of = __high2half2(so);
-      expand(false, ktile + (j & 1) * SH::KV_BYTES, kc1, sc, of, false);
-      if (lane == 0) mbar_arrive(&kfull[j & 1]);
-      ok = mbar_wait_backoff(&vempty[j & 1], ((j >> 1) & 1) ^ 1u, p.wait_ns, 64);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (clamp) expand(true, vtile + (j & 1) * SH::KV_BYTES, vc1, sc, of, true);
-      else expand(true, vtile + (j & 1) * SH::KV_BYTES, vc1, sc, of, false);
-      if (lane == 0) mbar_arrive(&vfull[j & 1]);
+      if (values) {
+        const uint32_t held = finite ? pair : 0;
+        const __half2 h = *reinterpret_cast<const __half2*>(&held), sc = __low2half2(h), of = __high2half2(h);
+        if (__any_sync(0xffffffffu, finite && 15.0f * fabsf(so.x) + fabsf(so.y) > kMaxF16)) expand(true, tile, codes, sc, of, true);
+        else expand(true, tile, codes, sc, of, false);
+      } else {
+        expand(false, tile, codes, __half2(), __half2(), false);
+      }
+      if (lane == 0) mbar_arrive(&full[ring]);
     }
   } else if (warp < 4 || two) {
     // ------------------------------ softmax ------------------------------
@@ -391,55 +444,24 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
     const int tile_last = min(last_row, row0 + t * 128 + 127);
     const int all_to = min(len, len - count + (row0 + t * 128) / a.share + 1);
     const int all_from = a.window ? max(0, len - count + tile_last / a.share - a.window + 1) : 0;
-    // ---- the tile's products, issued by its first thread
-    const bool issuer = (threadIdx.x & 127) == 0;
-    const uint32_t qk_desc = umma_idesc_f16_f32(128, TOK), pv_desc = umma_idesc_f16_f32(128, D) | kTransposeB;
-    auto qk = [&](int j) {
-      if (!mbar_wait(&kfull[j & 1], (j >> 1) & 1, p.wait_ns)) return false;
-      tc_fence_after();
-      const uint8_t* q = qtile + t * KB * PF_TILE;
-      const uint8_t* k = ktile + (j & 1) * SH::KV_BYTES;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const uint64_t qd = umma_desc_sw128(smem_u32(q + kb * PF_TILE)), kd = umma_desc_sw128(smem_u32(k + kb * SH::BLOCK_BYTES));
-        const int g = NG == 2 ? kb : 0;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          tc_mma_f16(tmem + t * 128 + g * TOK, qd + kk * 2, kd + kk * 2, qk_desc, (NG == 1 && kb) || kk);
-      }
-      tc_commit(&sfull[t]);
-      tc_commit(&kempty[j & 1]);
-      return true;
-    };
-    auto pv = [&](int j) {
-      if (!mbar_wait(&vfull[j & 1], (j >> 1) & 1, p.wait_ns) || !mbar_wait(&pfull[t], j & 1, p.wait_ns)) return false;
-      tc_fence_after();
-      const uint64_t vd = umma_desc_sw128_mn(smem_u32(vtile + (j & 1) * SH::KV_BYTES), SH::BLOCK_BYTES);
-#pragma unroll
-      for (int kk = 0; kk < TOK / 16; ++kk)
-        tc_mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, vd + kk * 128, pv_desc, j || kk);
-      tc_commit(&pvdone[t]);
-      tc_commit(&vempty[j & 1]);
-      return true;
-    };
     float m = 0.0f, l = 0.0f;
     uint32_t nan_groups = 0;         // groups whose values are NaN in some token this row sees
     bool fresh = true, ok = true;
-    if (issuer && steps > 0) ok = qk(0);
     for (int j = 0; j < steps; ++j) {
       const int slot = j % PF_PARS;
-      ok = ok && mbar_wait(&sfull[t], j & 1, p.wait_ns) && mbar_wait(&parfull[slot], (j / PF_PARS) & 1, p.wait_ns);
+      const uint32_t buf = s_at + (j & 1) * 64;
+      ok = mbar_wait(&sfull[t * 2 + (j & 1)], (j >> 1) & 1, p.wait_ns) && mbar_wait(&parfull[slot], (j / PF_PARS) & 1, p.wait_ns);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       const int tok0 = (step0 + j) * TOK;
       const bool edge = tok0 < all_from || tok0 + TOK > all_to;
-      const float4* par = pars + slot * 64;
+      const float4* par = pars + slot * 32;
       uint32_t h[TOK / 2];
       float l_add;
       for (int pass = 0; pass < 2; ++pass) {
-        const float top = edge ? step_probabilities<NG, TOK, true>(s_at, par, m, qs, see_from - tok0, see_to - tok0, h, l_add)
-                               : step_probabilities<NG, TOK, false>(s_at, par, m, qs, 0, 0, h, l_add);
+        const float top = edge ? step_probabilities<NG, TOK, true>(buf, par, m, qs, see_from - tok0, see_to - tok0, h, l_add)
+                               : step_probabilities<NG, TOK, false>(buf, par, m, qs, 0, 0, h, l_add);
         const bool grow = top > (fresh ? -INFINITY : kLazyMax);
         if (pass || !__any_sync(0xffffffffu, grow)) break;
         const float by = grow && !fresh ? ex2(-top) : 1.0f;
@@ -470,29 +492,27 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
         uint32_t r[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) r[i] = h[c + i];
-        tmem_st_32x32b_x16(s_at + c, r);
+        tmem_st_32x32b_x16(buf + c, r);
       }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&pfull[t]);
-      if (issuer) ok = pv(j) && (j + 1 >= steps || qk(j + 1));
-      __syncwarp();
-      const uint4 bads = bad[slot];
-      if (bads.x | bads.y | bads.z | bads.w) {
-        const uint32_t words[4] = {bads.x, bads.y, bads.z, bads.w};
+      const uint2 bads = bad[slot];
+      if (bads.x | bads.y) {
+        const uint32_t words[2] = {bads.x, bads.y};
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < 2; ++w)
           for (uint32_t left = words[w]; left; left &= left - 1) {
             const int tok = tok0 + w * 32 % TOK + __ffs(left) - 1;
             if (tok >= see_from && tok < see_to) nan_groups |= 1u << (w * 32 / TOK);
           }
+        __syncwarp();
       }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pfull[t * 2 + (j & 1)]);
     }
-    if (issuer) tc_commit(drain);
     // ---- the row's result
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&pvdone[t], (steps - 1) & 1, p.wait_ns));
+    // the last two products of P and V, in turn: a wait for the last alone could see the phase before
+    for (int j = max(0, steps - 2); ok && j < steps; ++j) ok = __all_sync(0xffffffffu, mbar_wait(&pvdone[t], j & 1, p.wait_ns));
     tc_fence_after();
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const long long at = static_cast<long long>(first + row / a.share) * a.heads + kh * a.share + row % a.share;
@@ -525,7 +545,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 12) {
     mbar_wait(drain, 0, kWaitBudgetNs);   // every product has finished before TMEM is released
     __syncwarp();
     tc_fence_after();
