@@ -10,8 +10,8 @@
 //   warps 8-11      the cache: a token's keys (8, 9) or values (10, 11), or one group of them, per thread,
 //                   read a step ahead; key codes as fp16 into the K ring, values as fp16 into the V ring,
 //                   key pairs as fp32 beside them
-//   warp 12         issues tcgen05.mma: O_t += P_t V (P from TMEM, V as it lies, token-major, through the
-//                   transposing descriptor), then S_t = Q_t K^T two steps ahead
+//   warps 12, 13    each issues its row tile's tcgen05.mma: O_t += P_t V (P from TMEM, V as it lies,
+//                   token-major, through the transposing descriptor), then S_t = Q_t K^T two steps ahead
 // Each tile has two buffers of scores, so its softmax goes on with step j + 1 while the tensor cores
 // take up step j's probabilities and write over them the scores of step j + 2 (the products of one thread
 // run in order). With one buffer of 128 tokens softmax and products took turns: 3700 and 3500 cycles
@@ -42,7 +42,7 @@ namespace w4a16 {
 namespace kv4 {
 
 constexpr int PF_ROWS = 256;         // query rows per block (two tiles)
-constexpr int PF_THREADS = 13 * 32;
+constexpr int PF_THREADS = 14 * 32;
 constexpr int PF_TILE = 128 * 128;   // bytes of a [128][64] fp16 tile
 constexpr int PF_RING = 4;           // K tiles, and V tiles
 constexpr int PF_PARS = 8;           // steps whose pairs are kept
@@ -202,8 +202,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   uint64_t* bars = reinterpret_cast<uint64_t*>(bad + PF_PARS);
   uint64_t *kfull = bars, *kempty = kfull + PF_RING, *vfull = kempty + PF_RING, *vempty = vfull + PF_RING;
   uint64_t* parfull = vempty + PF_RING;
-  uint64_t *sfull = parfull + PF_PARS, *pfull = sfull + 4;        // [tile][buffer of S]
-  uint64_t *pvdone = pfull + 4, *drain = pvdone + 2;
+  uint64_t *sfull = parfull + PF_PARS, *pfull = sfull + 4;        // [tile][buffer of S], pvdone too
+  uint64_t *pvdone = pfull + 4, *drain = pvdone + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   uint32_t* qmax = tmem_slot + 1;
 
@@ -211,17 +211,17 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   if (threadIdx.x == 0) {
     for (int i = 0; i < PF_RING; ++i) {
       mbar_init(&kfull[i], 2);
-      mbar_init(&kempty[i], 1);
+      mbar_init(&kempty[i], two ? 2 : 1);
       mbar_init(&vfull[i], 2);
-      mbar_init(&vempty[i], 1);
+      mbar_init(&vempty[i], two ? 2 : 1);
     }
     for (int i = 0; i < PF_PARS; ++i) mbar_init(&parfull[i], 4);
     for (int i = 0; i < 4; ++i) {
       mbar_init(&sfull[i], 1);
       mbar_init(&pfull[i], 4);
+      mbar_init(&pvdone[i], 1);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&pvdone[i], 1);
-    mbar_init(drain, 1);
+    mbar_init(drain, two ? 2 : 1);
     *qmax = 0;
     mbar_fence_init();
   }
@@ -296,13 +296,15 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 12) {
+  if (warp >= 12) {
     // ------------------------------ products ------------------------------
-    if (lane == 0) {
+    const int t = warp - 12;
+    if (lane == 0 && (t == 0 || two)) {
       const uint32_t qk_desc = umma_idesc_f16_f32(128, TOK), pv_desc = umma_idesc_f16_f32(128, D) | kTransposeB;
-      const int tiles = two ? 2 : 1;
-      // S_t of step j into its buffer, after the products that read the probabilities there
-      auto qk = [&](int t, int j) {
+      // the scores of step j into their buffer, after the products that read the probabilities there
+      auto qk = [&](int j) {
+        if (!mbar_wait(&kfull[j % PF_RING], (j / PF_RING) & 1, p.wait_ns)) return false;
+        tc_fence_after();
         const uint8_t* q = qtile + t * KB * PF_TILE;
         const uint8_t* k = ktile + (j % PF_RING) * SH::KV_BYTES;
         const uint32_t to = tmem + t * 128 + (j & 1) * 64;
@@ -314,35 +316,22 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
           for (int kk = 0; kk < 4; ++kk) tc_mma_f16(to + g * TOK, qd + kk * 2, kd + kk * 2, qk_desc, (NG == 1 && kb) || kk);
         }
         tc_commit(&sfull[t * 2 + (j & 1)]);
-        if (t + 1 == tiles) tc_commit(&kempty[j % PF_RING]);
+        tc_commit(&kempty[j % PF_RING]);
+        return true;
       };
       bool ok = true;
-      for (int j = 0; ok && j < min(2, steps); ++j) {
-        ok = mbar_wait(&kfull[j], 0, p.wait_ns);
+      for (int j = 0; ok && j < min(2, steps); ++j) ok = qk(j);
+      for (int j = 0; ok && j < steps; ++j) {
+        ok = mbar_wait(&vfull[j % PF_RING], (j / PF_RING) & 1, p.wait_ns) && mbar_wait(&pfull[t * 2 + (j & 1)], (j >> 1) & 1, p.wait_ns);
         if (!ok) break;
         tc_fence_after();
-        for (int t = 0; t < tiles; ++t) qk(t, j);
-      }
-      for (int j = 0; ok && j < steps; ++j) {
-        for (int t = 0; ok && t < tiles; ++t) {
-          ok = (t || mbar_wait(&vfull[j % PF_RING], (j / PF_RING) & 1, p.wait_ns)) && mbar_wait(&pfull[t * 2 + (j & 1)], (j >> 1) & 1, p.wait_ns);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t vd = umma_desc_sw128_mn(smem_u32(vtile + (j % PF_RING) * SH::KV_BYTES), SH::BLOCK_BYTES);
+        const uint64_t vd = umma_desc_sw128_mn(smem_u32(vtile + (j % PF_RING) * SH::KV_BYTES), SH::BLOCK_BYTES);
 #pragma unroll
-          for (int kk = 0; kk < TOK / 16; ++kk)
-            tc_mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + (j & 1) * 64 + kk * 8, vd + kk * 128, pv_desc, j || kk);
-          tc_commit(&pvdone[t]);
-          if (t + 1 == tiles) tc_commit(&vempty[j % PF_RING]);
-          if (j + 2 < steps) {
-            if (t == 0) {
-              ok = mbar_wait(&kfull[(j + 2) % PF_RING], ((j + 2) / PF_RING) & 1, p.wait_ns);
-              if (!ok) break;
-              tc_fence_after();
-            }
-            qk(t, j + 2);
-          }
-        }
+        for (int kk = 0; kk < TOK / 16; ++kk)
+          tc_mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + (j & 1) * 64 + kk * 8, vd + kk * 128, pv_desc, j || kk);
+        tc_commit(&pvdone[t * 2 + (j & 1)]);
+        tc_commit(&vempty[j % PF_RING]);
+        if (j + 2 < steps) ok = qk(j + 2);
       }
       tc_commit(drain);
     }
@@ -471,7 +460,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
         }
         l *= by;
         if (j > 0) {                     // the sums so far
-          ok = __all_sync(0xffffffffu, mbar_wait(&pvdone[t], (j - 1) & 1, p.wait_ns));
+          ok = __all_sync(0xffffffffu, mbar_wait(&pvdone[t * 2 + ((j - 1) & 1)], ((j - 1) >> 1) & 1, p.wait_ns));
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
@@ -511,8 +500,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       if (lane == 0) mbar_arrive(&pfull[t * 2 + (j & 1)]);
     }
     // ---- the row's result
-    // the last two products of P and V, in turn: a wait for the last alone could see the phase before
-    for (int j = max(0, steps - 2); ok && j < steps; ++j) ok = __all_sync(0xffffffffu, mbar_wait(&pvdone[t], j & 1, p.wait_ns));
+    // (a barrier per buffer: the scores of the last step have shown its phase before to be over)
+    if (ok && steps > 0)
+      ok = __all_sync(0xffffffffu, mbar_wait(&pvdone[t * 2 + ((steps - 1) & 1)], ((steps - 1) >> 1) & 1, p.wait_ns));
     tc_fence_after();
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const long long at = static_cast<long long>(first + row / a.share) * a.heads + kh * a.share + row % a.share;
@@ -543,6 +533,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
     if (live && ok && a.lse) a.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
   }
 
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 12) {
