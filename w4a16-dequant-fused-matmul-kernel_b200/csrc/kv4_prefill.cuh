@@ -32,7 +32,7 @@
 // leaves the scores as they are, and in V, which the last step undoes.
 //
 // The probabilities of a step are taken with the running maximum as it stands, and again in the
-// rare case that some score of the warp's rows exceeds it by kLazyMax: one pass over the scores
+// rare case that some score of the warp's rows exceeds it by kPfLazyMax: one pass over the scores
 // instead of two. Every wait is bounded; on expiry the block raises the device error bit and leaves.
 #pragma once
 
@@ -43,6 +43,10 @@ namespace kv4 {
 
 constexpr int PF_ROWS = 256;         // query rows per block (two tiles)
 constexpr int PF_THREADS = 14 * 32;
+// A row's maximum is raised when a score exceeds it by this (base 2): probabilities up to 256, as exact in
+// fp16 as those below 1. At 2.9 (the decode kernel's, whose probabilities carry a scale) 14% of a long
+// prompt's steps took the rescaling path.
+constexpr float kPfLazyMax = 8.0f;
 constexpr int PF_TILE = 128 * 128;   // bytes of a [128][64] fp16 tile
 constexpr int PF_RING = 4;           // K tiles, and V tiles
 constexpr int PF_PARS = 8;           // steps whose pairs are kept
@@ -451,7 +455,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       for (int pass = 0; pass < 2; ++pass) {
         const float top = edge ? step_probabilities<NG, TOK, true>(buf, par, m, qs, see_from - tok0, see_to - tok0, h, l_add)
                                : step_probabilities<NG, TOK, false>(buf, par, m, qs, 0, 0, h, l_add);
-        const bool grow = top > (fresh ? -INFINITY : kLazyMax);
+        const bool grow = top > (fresh ? -INFINITY : kPfLazyMax);
         if (pass || !__any_sync(0xffffffffu, grow)) break;
         const float by = grow && !fresh ? ex2(-top) : 1.0f;
         if (grow) {
