@@ -6,7 +6,8 @@ HALF_ULP[T] * |y|; fp32 sums of at most 128 products add less than 2e-5 of the h
 Attention rounds each probability times its value scale s to fp16 (2^-11 relative, 2^-25 absolute
 below 2^-14) against codes centred on 7.5: at most (2^-11 * s + n * 2^-25) * 7.5 in the weighted mean
 over n tokens; its fp32 scores are within 2e-5 of the largest, which moves the mean by at most that
-times the spread of the values."""
+times the spread of the values. (Prompts round probabilities and values instead, each to within 2^-11
+of a value, in either direction: the same bound, met in the mean.)"""
 from __future__ import annotations
 
 import math

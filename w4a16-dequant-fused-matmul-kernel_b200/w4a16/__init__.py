@@ -11,7 +11,8 @@ reference package (w4a16-kernel/src/w4a16/__init__.py:18-39):
 Beyond the reference, the attention path between those layers (kv_cache.py): a 4-bit paged
 key/value cache (KV4Cache, KV4Pages), query/key norm and rotation (qk_norm_rope,
 qk_norm_rope_append), attention over the cache (kv4_attention) and page management
-(kv4_reserve, kv4_copy_pages, kv4_fork, kv4_release, kv4_compact).
+(kv4_reserve, kv4_copy_pages, kv4_fork, kv4_release, kv4_compact). W4A16Attention (attention.py) is the
+layer that runs them together.
 
 Tensor-parallel layers (column / row sharding over torch.distributed + NCCL)
 live in ``w4a16.parallel``.
@@ -23,6 +24,7 @@ Triton fallback. Importing needs no GPU; calling needs a B200.
 from __future__ import annotations
 
 from ._lib import W4A16Error, check_device_errors
+from .attention import W4A16Attention
 from .gemm import (interleave_gate_up, repack_qweight, stage_copy, swiglu, to_fp16, w4a16_matmul,
                    w4a16_matmul_bf16, w4a16_matmul_f32, w4a16_matmul_host, w4a16_matmul_swiglu)
 from .kv_cache import (KV4Cache, KV4Pages, kv4_attention, kv4_compact, kv4_copy_pages, kv4_fork, kv4_gather,
@@ -63,6 +65,7 @@ __all__ = [
     "kv4_fork",
     "kv4_release",
     "kv4_compact",
+    "W4A16Attention",
 ]
 
 # The reference exported the fused GEMM only when its Triton backend imported

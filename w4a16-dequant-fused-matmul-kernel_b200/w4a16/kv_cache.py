@@ -84,7 +84,7 @@ class KV4Cache:
 class KV4Pages:
     """Which sequence (row) holds which pages: ``refs`` int32 ``[num_pages]`` (rows that hold a page;
     0: free), ``block_table`` int32 ``[rows, pages per row]`` (-1: none), ``kv_lens`` int32 ``[rows]``.
-    :meth:`empty` makes the tables of a pool nobody uses yet."""
+    :meth:`empty` makes the tables of a pool nobody uses yet. The tensors may be written to, not replaced."""
 
     def __init__(self, refs: Tensor, block_table: Tensor, kv_lens: Tensor, page_size: int) -> None:
         for name, t, dim in (("refs", refs, 1), ("block_table", block_table, 2), ("kv_lens", kv_lens, 1)):
@@ -103,6 +103,11 @@ class KV4Pages:
         return cls(torch.zeros(cache.num_pages, dtype=_I32, device=cache.device),
                    torch.full((rows, pages_per_row), -1, dtype=_I32, device=cache.device),
                    torch.zeros(rows, dtype=_I32, device=cache.device), cache.page_size)
+
+    def slots(self, rows: Tensor, positions: Tensor) -> Tensor:
+        """Where tokens ``positions`` of sequences ``rows`` (int64 [T] each) lie, as int64 [T]: what
+        :func:`qk_norm_rope_append` and :func:`kv4_gather` take. Their pages must be reserved."""
+        return self.block_table[rows, positions // self.page_size].long() * self.page_size + positions % self.page_size
 
     def like(self) -> "KV4Pages":
         """Tables of the same shape, not initialised."""
