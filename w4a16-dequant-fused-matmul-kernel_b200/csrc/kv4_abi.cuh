@@ -296,8 +296,9 @@ int launch_prefill(const w4a16_kv4_cache& c, const AttendParams& a, const Attend
   return launch_prefill_as<128, 2>(p, blocks, s);
 }
 
-void launch_copy(const w4a16_kv4_cache& c, const int* src, const int* dst, const int* count, int n, const DeviceState& dev,
-                 cudaStream_t s) {
+// The copies of pages, and how many blocks share them.
+CopyParams copy_params(const w4a16_kv4_cache& c, const int* src, const int* dst, const int* count, int n,
+                       const DeviceState& dev, unsigned* blocks) {
   const CacheView v = view_of(c, 0);
   CopyParams p = {};
   p.pool = v.pool;
@@ -309,8 +310,8 @@ void launch_copy(const w4a16_kv4_cache& c, const int* src, const int* dst, const
   const long long per_part = 16LL * COPY_THREADS * COPY_VECS;
   p.parts = static_cast<int>((p.copy_bytes + per_part - 1) / per_part);
   const long long work = static_cast<long long>(n) * c.layers * p.parts;
-  const unsigned grid = static_cast<unsigned>(std::min<long long>(work, 8LL * dev.num_sms));
-  kv4_copy_pages_kernel<<<grid, COPY_THREADS, 0, s>>>(p);
+  *blocks = static_cast<unsigned>(std::min<long long>(work, 8LL * dev.num_sms));
+  return p;
 }
 
 }  // namespace
@@ -450,7 +451,9 @@ int w4a16_kv4_copy_pages(const w4a16_kv4_cache* cache, const int32_t* src, const
   if (n < 0 || n > 0x7fffffffLL) return W4A16_ERR_INVALID;
   if (n == 0) return W4A16_OK;
   if (src == nullptr || dst == nullptr) return W4A16_ERR_INVALID;
-  kv4::launch_copy(*cache, src, dst, nullptr, static_cast<int>(n), *dev, static_cast<cudaStream_t>(stream));
+  unsigned blocks = 0;
+  const kv4::CopyParams p = kv4::copy_params(*cache, src, dst, nullptr, static_cast<int>(n), *dev, &blocks);
+  kv4::kv4_copy_pages_kernel<<<blocks, kv4::COPY_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(p);
   return kv4::launched();
 }
 
@@ -489,8 +492,9 @@ int w4a16_kv4_fork(const w4a16_kv4_cache* cache, const w4a16_kv4_tables* in, con
     return kv4::launched();
   }
   kv4::kv4_fork_plan_kernel<<<1 + kv4::table_blocks(*in, kv4::SCAN_THREADS, *dev), kv4::SCAN_THREADS, 0, s>>>(p);
-  kv4::kv4_fork_rows_kernel<<<static_cast<unsigned>(n), 256, 0, s>>>(p);
-  kv4::launch_copy(*cache, p.src, p.dst, nullptr, p.n, *dev, s);
+  unsigned blocks = 0;
+  const kv4::CopyParams copy = kv4::copy_params(*cache, p.src, p.dst, nullptr, p.n, *dev, &blocks);
+  kv4::kv4_fork_rows_kernel<<<static_cast<unsigned>(n) + blocks, kv4::COPY_THREADS, 0, s>>>(p, copy);
   return kv4::launched();
 }
 
@@ -523,11 +527,12 @@ int w4a16_kv4_compact(const w4a16_kv4_cache* cache, const w4a16_kv4_tables* in, 
     return W4A16_ERR_INVALID;
   const int pages = in->pages, half = pages / 2;
   kv4::CompactParams p = {kv4::tables_of(*in), kv4::tables_of(*out), scratch, scratch + pages, scratch + pages + half,
-                          scratch + pages + 2 * half};
+                          scratch + pages + 2 * half, static_cast<int>(kv4::table_blocks(*in, kv4::COPY_THREADS, *dev))};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   kv4::kv4_compact_plan_kernel<<<1, kv4::SCAN_THREADS, 0, s>>>(p);
-  kv4::kv4_compact_tables_kernel<<<kv4::table_blocks(*in, 256, *dev), 256, 0, s>>>(p);
-  if (half > 0) kv4::launch_copy(*cache, p.src, p.dst, p.count, half, *dev, s);
+  unsigned blocks = 0;
+  const kv4::CopyParams copy = kv4::copy_params(*cache, p.src, p.dst, p.count, half, *dev, &blocks);
+  kv4::kv4_compact_tables_kernel<<<static_cast<unsigned>(p.table_blocks) + blocks, kv4::COPY_THREADS, 0, s>>>(p, copy);
   return kv4::launched();
 }
 

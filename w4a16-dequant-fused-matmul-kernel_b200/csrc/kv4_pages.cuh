@@ -66,11 +66,12 @@ struct CopyParams {
 // piece's loads are in flight together and a handful of pages still fills the SMs.
 constexpr int COPY_THREADS = 256, COPY_VECS = 4;
 
-__global__ void __launch_bounds__(COPY_THREADS) kv4_copy_pages_kernel(const CopyParams p) {
+// This block's share, the `block`-th of `blocks`.
+__device__ __forceinline__ void copy_pages(const CopyParams& p, unsigned block, unsigned blocks) {
   const int n = p.count ? min(*p.count, p.n) : p.n;
   const long long work = static_cast<long long>(n) * p.layers * p.parts;
   const long long vecs = p.copy_bytes / 16;
-  for (long long w = blockIdx.x; w < work; w += gridDim.x) {
+  for (long long w = block; w < work; w += blocks) {
     const long long item = w / p.parts;
     const int part = static_cast<int>(w - item * p.parts);
     const long long layer = item / n;
@@ -93,6 +94,10 @@ __global__ void __launch_bounds__(COPY_THREADS) kv4_copy_pages_kernel(const Copy
     for (int c = 0; c < COPY_VECS; ++c)
       if (first + c * COPY_THREADS < end) to[first + c * COPY_THREADS] = v[c];
   }
+}
+
+__global__ void __launch_bounds__(COPY_THREADS) kv4_copy_pages_kernel(const CopyParams p) {
+  copy_pages(p, blockIdx.x, gridDim.x);
 }
 
 // ---------------------------------------------------------------------------
@@ -258,15 +263,19 @@ __global__ void __launch_bounds__(SCAN_THREADS) kv4_fork_plan_kernel(const ForkP
   }
 }
 
-// Fork, step 2: block i writes child i's row and counts its pages.
-__global__ void __launch_bounds__(256) kv4_fork_rows_kernel(const ForkParams p) {
+// Fork, step 2: block i < n writes child i's row and counts its pages; the others copy the last pages.
+__global__ void __launch_bounds__(COPY_THREADS) kv4_fork_rows_kernel(const ForkParams p, const CopyParams copy) {
+  if (blockIdx.x >= static_cast<unsigned>(p.n)) {
+    copy_pages(copy, blockIdx.x - p.n, gridDim.x - p.n);
+    return;
+  }
   const Tables& t = p.out;
   const int i = blockIdx.x;
   const int a = p.parents[i], c = p.children[i];
   if (a < 0 || a >= t.rows || c < 0 || c >= t.rows) return;   // flagged in step 1
   const int len = p.ok[i] ? p.in.lens[a] : 0;
   const int held = len / t.page_size + (len % t.page_size != 0);
-  for (int col = threadIdx.x; col < t.width; col += 256) {
+  for (int col = threadIdx.x; col < t.width; col += COPY_THREADS) {
     int page = -1;
     if (col < held) {
       page = col == held - 1 && p.dst[i] >= 0 ? p.dst[i] : p.in.table[static_cast<long long>(a) * t.width + col];
@@ -311,13 +320,15 @@ __global__ void __launch_bounds__(256) kv4_copy_tables_kernel(const Tables in, c
 // ---------------------------------------------------------------------------
 // Compact: with `live` pages in use, the i-th page in use with an id >= live moves to the i-th
 // free page with an id < live; pages below `live` stay where they are, so as few pages move as
-// can. Step 1 (one block): the moves and the map of ids. Step 2: the tables.
+// can. Step 1 (one block): the moves and the map of ids. Step 2: the first `table_blocks` blocks the
+// tables, the others the pages.
 // ---------------------------------------------------------------------------
 struct CompactParams {
   Tables in, out;
   int* map;                  // [pages]: new id of a page
   int *src, *dst;            // [pages / 2] moves
   int* count;                // [1]
+  int table_blocks;
 };
 
 __global__ void __launch_bounds__(SCAN_THREADS) kv4_compact_plan_kernel(const CompactParams p) {
@@ -358,10 +369,15 @@ __global__ void __launch_bounds__(SCAN_THREADS) kv4_compact_plan_kernel(const Co
   }
 }
 
-__global__ void __launch_bounds__(256) kv4_compact_tables_kernel(const CompactParams p) {
+__global__ void __launch_bounds__(COPY_THREADS) kv4_compact_tables_kernel(const CompactParams p, const CopyParams copy) {
+  if (blockIdx.x >= static_cast<unsigned>(p.table_blocks)) {
+    copy_pages(copy, blockIdx.x - p.table_blocks, gridDim.x - p.table_blocks);
+    return;
+  }
   const Tables& t = p.in;
   const long long n = static_cast<long long>(t.rows) * t.width;
-  const long long at = blockIdx.x * 256LL + threadIdx.x, step = gridDim.x * 256LL;
+  const long long at = blockIdx.x * static_cast<long long>(COPY_THREADS) + threadIdx.x;
+  const long long step = p.table_blocks * static_cast<long long>(COPY_THREADS);
   for (long long i = at; i < n; i += step) {
     int page = t.table[i];
     if (page >= t.pages) {

@@ -25,7 +25,7 @@ __all__ = ["KV4Cache", "KV4Pages", "qk_norm_rope", "qk_norm_rope_append", "kv4_g
 _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
 _CODES = {torch.float16: _lib.DTYPE_CODES[torch.float16], torch.bfloat16: _lib.DTYPE_CODES[torch.bfloat16]}
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
-_raw_stream = _lib.stream_of_index
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _lib.stream_of_index)
 _CONTIGUOUS = torch.contiguous_format
 
 
