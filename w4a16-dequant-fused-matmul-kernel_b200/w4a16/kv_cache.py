@@ -114,7 +114,8 @@ class KV4Pages:
         new = object.__new__(KV4Pages)
         P, (R, W) = self.refs.shape[0], self.block_table.shape
         buf = self.refs.new_empty(R * W + P + R)      # one allocation; the table first, for its alignment
-        new.block_table, new.refs, new.kv_lens = buf[:R * W].view(R, W), buf[R * W:R * W + P], buf[R * W + P:]
+        table, new.refs, new.kv_lens = buf.split((R * W, P, R))
+        new.block_table = table.view(R, W)
         new.page_size = self.page_size
         at = buf.data_ptr()
         new._struct = _lib.KV4TablesStruct(at + 4 * R * W, at, at + 4 * (R * W + P), P, R, W, self.page_size)
@@ -148,35 +149,35 @@ def _rope_args(q: Tensor, k: Tensor, v: Tensor | None, positions: Tensor, cos_si
     """Checked (axes, end0, end1, weight code) of a rotation. The common case is one expression; anything
     else goes through the checks one by one, which say what is wrong."""
     d, dt, qs, ks, cs = q.get_device(), q.dtype, q.shape, k.shape, cos_sin.shape
-    if (sections is None and d >= 0 and dt in _CODES and len(qs) == 3 and len(ks) == 3 and len(cs) == 2
+    if sections is None:
+        axes, end0, end1, shape, fits = 1, 0, 0, qs[:1], True
+    else:
+        axes, end0, end1, shape = 3, sum(sections[:1]), sum(sections[:2]), (3, *qs[:1])
+        fits = len(sections) == 3 and min(sections) >= 0 and len(cs) == 2 and 2 * sum(sections) == cs[1]
+    if (fits and d >= 0 and dt in _CODES and len(qs) == 3 and len(ks) == 3 and len(cs) == 2
             and k.dtype is dt and k.get_device() == d and ks[0] == qs[0] and ks[2] == qs[2] and qs[2] in (64, 128)
             and q.stride(2) == 1 and k.stride(2) == 1 and cos_sin.dtype is _F32 and cos_sin.is_contiguous()
             and cos_sin.get_device() == d and cs[1] % 8 == 0 and 0 < cs[1] <= qs[2] and cs[0] > 0
-            and positions.dtype is _I64 and positions.shape == qs[:1] and positions.is_contiguous()
+            and positions.dtype is _I64 and positions.shape == shape and positions.is_contiguous()
             and positions.get_device() == d
             and (v is None or (v.dtype is dt and v.shape == ks and v.get_device() == d and v.stride(2) == 1))
             and (q_weight is None or (q_weight.dtype is dt and q_weight.shape == qs[2:] and q_weight.get_device() == d
                                       and q_weight.is_contiguous()))
             and (k_weight is None or (k_weight.dtype is dt and k_weight.shape == qs[2:] and k_weight.get_device() == d
                                       and k_weight.is_contiguous()))):
-        return 1, 0, 0, _CODES[dt]
+        return axes, end0, end1, _CODES[dt]
     _check_heads("q", q)
     _check_heads("k", k, q)
     if v is not None:
         _check_heads("v", v, q)
-    T, D = q.shape[0], q.shape[2]
-    rot = cos_sin.shape[-1]
+    D, rot = q.shape[2], cos_sin.shape[-1]
     assert D in (64, 128), f"head_dim={D} must be 64 or 128"
     assert cos_sin.dtype is _F32 and cos_sin.dim() == 2 and cos_sin.is_contiguous() and cos_sin.get_device() == d, (
         "cos_sin must be a contiguous fp32 [positions, rotated channels] tensor on q's device")
     assert rot % 8 == 0 and 0 < rot <= D and cos_sin.shape[0] > 0, (
         f"rotated channels ({rot}) must be a multiple of 8, at most head_dim={D}")
-    if sections is None:
-        axes, end0, end1, shape = 1, 0, 0, (T,)
-    else:
-        assert len(sections) == 3 and min(sections) >= 0 and sum(sections) == rot // 2, (
-            f"sections={sections} must be three counts of frequencies that add up to {rot // 2}")
-        axes, end0, end1, shape = 3, sections[0], sections[0] + sections[1], (3, T)
+    assert sections is None or (len(sections) == 3 and min(sections) >= 0 and sum(sections) == rot // 2), (
+        f"sections={sections} must be three counts of frequencies that add up to {rot // 2}")
     assert positions.dtype is _I64 and positions.shape == shape and positions.is_contiguous() and (
         positions.get_device() == d), f"positions must be a contiguous int64 {list(shape)} tensor on q's device"
     code = _CODES[q.dtype]
