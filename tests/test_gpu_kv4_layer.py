@@ -117,15 +117,16 @@ def test_fork_release_and_compact_between_steps():
 
 
 @pytest.mark.parametrize("H,KV,D,group", [(8, 1, 128, 128), (8, 1, 128, 64), (16, 1, 64, 64)])
-def test_prompt_kernel_step_and_tile_edges(H, KV, D, group):
-    """Lengths around the tokens of a step, rows around one and two row tiles, and a window that begins inside a step."""
+def test_small_prompts_step_and_tile_edges(H, KV, D, group):
+    """Prompts of small batches: lengths around the tokens of a step, rows around one and two row tiles, and a window
+    that begins inside a step."""
     for n in (1, 31, 33, 63, 64, 65, 127, 128, 129, 193, 257):
         check_attention([n, 3], [9, 1], H, KV, D, group, 16, F16, seed=n)            # 72 or 144 rows
         check_attention([max(n, 40)], [33], H, KV, D, group, 16, BF16, seed=n)       # a last tile of few rows
         check_attention([300 + n], [40], H, KV, D, group, 16, F16, window=n, seed=n)
 
 
-def test_prompt_sees_a_nan_value_it_attends_to_and_no_other():
+def test_small_prompt_sees_a_nan_value_it_attends_to_and_no_other():
     """A NaN value makes its group NaN for the queries that see it, not for earlier ones or other groups."""
     g = gen(10)
     for group, token in ((64, 70), (128, 70), (64, 129)):
@@ -144,3 +145,41 @@ def test_prompt_sees_a_nan_value_it_attends_to_and_no_other():
             half = 0 if group == 128 else 64
             assert o[sees][..., half:].isnan().all() and o[~sees].isfinite().all() and o[..., :half].isfinite().all()
             assert lse.isfinite().all()
+
+
+@pytest.mark.parametrize("H,KV,D,group", [(64, 8, 128, 128), (64, 8, 128, 64), (48, 16, 64, 64)])
+def test_large_prompts_step_and_tile_edges(H, KV, D, group):
+    """As above with enough rows, kv heads and sequences for the kernel that takes long prompts: lengths around the
+    tokens of a step, one and two row tiles, tiles of few rows, short sequences in the same batch."""
+    share = H // KV
+    for i, n in enumerate((1, 31, 33, 63, 64, 65, 127, 128, 129, 193)):
+        new = [n + 6144 // (3 * KV * share) + 1, 256 // share + 1, 1 + i % 3]
+        assert max(new) * share * KV * 3 > 6144 and max(new) * share > 64
+        check_attention([max(n, new[0]), new[1] + i, n], new[:2] + [min(n, new[2])], H, KV, D, group, 16, F16, seed=n)
+        check_attention([new[0] + n, 7, 300], [new[0], 0, 130 // share], H, KV, D, group, 32, BF16, window=1 + n, seed=n)
+
+
+def test_large_prompt_sees_a_nan_value_it_attends_to_and_no_other():
+    g = gen(10)
+    for group, token in ((64, 70), (128, 70), (64, 129)):
+        c = PlainCache([130], 32, 128, group, 16, gen=g)
+        cache = KV4Cache(1, c.num_pages, 32, 128, page_size=16, group_size=group, pool=c.pool)
+        v = torch.zeros((1, 32, 128), device=DEV, dtype=F16)
+        v[:, 5, 100] = float("nan")
+        k = torch.randn((1, 32, 128), device=DEV, generator=g).half()
+        qk_norm_rope_append(torch.empty(1, 0, 128, device=DEV, dtype=F16), k, v, cache, 0, c.slots(0, token, 1),
+                            torch.zeros(1, dtype=torch.int64, device=DEV), cos_sin_table(1, 8))
+        q = torch.randn((100, 64, 128), device=DEV, generator=g).half()
+        for window in (0, 20):
+            o, lse = kv4_attention(q, cache, 0, c.table, c.kv_lens, window=window, return_lse=True)
+            at = torch.arange(30, 130, device=DEV)
+            sees = (at >= token) & ((at < token + window) if window else True)
+            half = 0 if group == 128 else 64
+            hit, rest = o[:, 10:12], torch.cat([o[:, :10], o[:, 12:]], 1)
+            assert hit[sees][..., half:].isnan().all() and hit[~sees].isfinite().all() and hit[..., :half].isfinite().all()
+            assert rest.isfinite().all() and lse.isfinite().all()
+
+
+def test_large_prompts_of_large_values():
+    """Values near fp16's end in the kernel that rounds them to fp16: finite, and within its bound."""
+    check_attention([200, 90, 160], [170, 90, 100], 16, 16, 128, 128, 32, F16, v_scale=14000.0, seed=1)

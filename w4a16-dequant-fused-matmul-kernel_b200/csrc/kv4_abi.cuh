@@ -259,10 +259,19 @@ int launch_decode(const w4a16_kv4_cache& c, const AttendParams& all, const Atten
   });
 }
 
-// Sequences with more query rows (new tokens x heads of a group) per kv head than this take the
-// tensor-memory kernel, whose blocks of 256 rows each read the cache once; the others the decode
-// kernel, which reads it once per 16 rows but splits it over all SMs.
-constexpr int kDecodeRows = 64;
+// Which kernel takes a sequence goes by its query rows (new tokens x heads of a group) per kv head.
+// The tensor-memory kernel reads the cache once per 256 rows but has a block for no less, so a batch of few
+// such blocks leaves most SMs idle and takes as long as its longest sequence; the decode kernel reads it
+// once per 8 or 16 rows and splits it over all SMs. Up to kDecodeRows rows the decode kernel takes the
+// sequence, and every sequence of a batch of at most kDecodeWork rows x kv heads x sequences. Measured, 32
+// heads of 128 channels on 8 kv heads (decode kernel against the other, us): 8192 tokens, 128 rows: 35,
+// 139; 1024 rows: 157, 182; two sequences of 512 rows: 157, 183, and of 1024: 298, 184; 2048 tokens, 512
+// rows: 31, 61; 1024 rows: 79, 61; 16 sequences of 64 rows, 8192 tokens: 161, 188; of 128: 302, 189.
+constexpr long long kDecodeRows = 64, kDecodeWork = 6144;
+
+long long decode_rows(const AttendPlan& plan) {
+  return plan.rows <= kDecodeWork / std::max(1LL, plan.kv_heads * plan.seqs) ? plan.rows : std::min(plan.rows, kDecodeRows);
+}
 
 template <int D, int NG>
 int launch_prefill_as(const PrefillParams& p, long long blocks, cudaStream_t s) {
@@ -282,11 +291,12 @@ int launch_prefill_as(const PrefillParams& p, long long blocks, cudaStream_t s) 
   return launched();
 }
 
-int launch_prefill(const w4a16_kv4_cache& c, const AttendParams& a, const AttendPlan& plan, int bf16, cudaStream_t s) {
+int launch_prefill(const w4a16_kv4_cache& c, const AttendParams& a, const AttendPlan& plan, int bf16, long long row_limit,
+                   cudaStream_t s) {
   PrefillParams p = {};
   p.a = a;
   p.bf16 = bf16;
-  p.row_limit = kDecodeRows;
+  p.row_limit = static_cast<int>(row_limit);
   p.wait_ns = g_wait_budget_ns.load(std::memory_order_relaxed);
   const long long tiles = (plan.rows + PF_ROWS - 1) / PF_ROWS;
   if (plan.seqs * plan.kv_heads > 0x7fffffffLL / tiles) return W4A16_ERR_INVALID;
@@ -394,8 +404,8 @@ int w4a16_kv4_attention_workspace_size(const w4a16_kv4_cache* cache, int64_t T, 
   if (T < 0 || T > 0x7fffffffLL || heads < 1 || heads % cache->kv_heads != 0 || seqs < 0 || max_q < 0)
     return W4A16_ERR_INVALID;
   if (T == 0 || seqs == 0) return W4A16_OK;
-  const kv4::AttendPlan plan = {seqs, cache->kv_heads,
-                                std::min<long long>(std::min(max_q, T) * (heads / cache->kv_heads), kv4::kDecodeRows)};
+  kv4::AttendPlan plan = {seqs, cache->kv_heads, std::min(max_q, T) * (heads / cache->kv_heads)};
+  plan.rows = kv4::decode_rows(plan);
   *bytes_out = kv4::decode_workspace(*cache, plan, *dev);
   return W4A16_OK;
 }
@@ -430,18 +440,18 @@ int w4a16_kv4_attention(const void* q, int dtype, int64_t T, int heads, int64_t 
   p.groups = cache->head_dim / cache->group_size;
   const kv4::AttendPlan plan = {seqs, cache->kv_heads, (cu_q ? std::min(max_q, T) : T / seqs) * p.share};
   kv4::AttendPlan few = plan;      // the sequences that the decode kernel takes
-  few.rows = std::min<long long>(plan.rows, kv4::kDecodeRows);
+  few.rows = kv4::decode_rows(plan);
   const int64_t need = kv4::decode_workspace(*cache, few, *dev);
   if (workspace == nullptr || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return W4A16_ERR_WORKSPACE;
   const int bf16 = dtype == W4A16_DTYPE_BF16;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (plan.rows > kv4::kDecodeRows) {
-    const int st2 = kv4::launch_prefill(*cache, p, plan, bf16, s);
+  if (plan.rows > few.rows) {
+    const int st2 = kv4::launch_prefill(*cache, p, plan, bf16, few.rows, s);
     if (st2 != W4A16_OK || cu_q == nullptr) return st2;
   }
   // sequences with few rows (every one, unless the batch is mixed)
-  return kv4::launch_decode(*cache, p, few, bf16, kv4::kDecodeRows, workspace, *dev, s);
+  return kv4::launch_decode(*cache, p, few, bf16, static_cast<int>(few.rows), workspace, *dev, s);
 }
 
 int w4a16_kv4_copy_pages(const w4a16_kv4_cache* cache, const int32_t* src, const int32_t* dst, int64_t n, void* stream) {

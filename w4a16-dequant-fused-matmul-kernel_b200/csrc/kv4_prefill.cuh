@@ -17,8 +17,8 @@
 // run in order). With one buffer of 128 tokens softmax and products took turns: 3700 and 3500 cycles
 // per 128 tokens.
 //
-// Three prompts of up to 4096 tokens over up to 8192, 32 heads of 128 channels on 8 kv heads: 1.16 ms, 0.80
-// PFLOP/s, 48% of what a plain bf16 matrix product reaches. A step of 64 tokens takes 2500 cycles, its
+// Three prompts of up to 4096 tokens over up to 8192, 32 heads of 128 channels on 8 kv heads: 1.14 ms, 0.82
+// PFLOP/s, 49% of what a plain bf16 matrix product reaches. A step of 64 tokens takes 2500 cycles, its
 // products 1000 of them: what bounds it is the softmax warps' instructions (1950 cycles a step, two
 // warps to an SM quarter, 128 registers) with the cache warps' in the same issue slots; without
 // exponentials, key pairs and expansion the same schedule takes 0.76 ms. Four softmax warps to a quarter
