@@ -26,8 +26,8 @@
 // of 16 tokens. All tiles form one list that N teams of warps split evenly, whatever the lengths
 // (a segment counts `seg_cost` tiles more than it has, for its queries and its epilogue); a team that holds a part of a segment leaves (m, l, o) in the workspace and, when all its
 // tiles are done, the last of the segment's teams to arrive joins the parts in team order, so
-// results do not depend on timing. (Where there are teams enough and every segment is short, each
-// team takes one whole segment: joining parts costs about 5 us, eight tiles of each warp.) Each warp
+// results do not depend on timing. (Where there are teams enough and no segment is much longer than the
+// others, each team takes one whole segment.) Each warp
 // feeds itself: two stages of a tile, filled by copies
 // that its own lane 0 issues. A piece's end passes through shared memory once: each warp leaves its
 // sums in the stage it has just read, and each then adds up some rows over all warps.
@@ -120,7 +120,13 @@ struct DecodeShape {
 struct Sequence {
   int prefix, segments, first, count, len;
 };
-constexpr int kWholeTiles = 8;             // a segment of at most so many tiles per warp is one team's
+// A team takes one whole segment each, and nothing is joined, where there are teams enough and no segment
+// has many more tiles per warp than the warps' average share: kWholeTiles + 0.9 x the share more, at most
+// kWholeMost. Joining costs what four tiles of a warp alone take, and more where the memory is busy. Measured
+// (whole, split; us): 24 sequences of up to 3001, 5 rows, 16 kv heads of 64: 20.7, 24.8; 48 of 777, 20 rows, 8
+// kv heads of 128: 51, 84; 16 of 6000, 4 rows: 33, 41; one of 6000: 29, 18.5; 24 of 6000 on one kv head: 31,
+// 20.7; 48 of 3000, 16 kv heads of 64: 69, 58.
+constexpr float kWholeTiles = 4.0f, kWholeMost = 13.0f;
 
 struct Segment {
   int start;               // its first tile's place in the list (after the seg_cost places without a tile)
@@ -191,12 +197,10 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
   const int TW = p.team_warps;
   // prefix sums of the sequences' tiles (low half) and segments (high half)
   unsigned long long sums = 0;
-  bool longer = false;               // some segment is longer than one team should take
   for (int base = 0; base < a.seqs; base += W * 32) {
     const int b = base + threadIdx.x;
     Sequence q = {0, 0, 0, 0, 0};
     unsigned long long v = 0;
-    bool more = false;
     if (b < a.seqs) {
       sequence(a, b, q.first, q.count, q.len);
       if (static_cast<long long>(q.count) * a.share > p.row_limit) q.count = 0;
@@ -205,7 +209,6 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
         const unsigned h = segments_of(q.count);
         v = (static_cast<unsigned long long>(h) << 32) | h * (n + p.seg_cost);
       }
-      more = n > kWholeTiles * TW;
     }
     unsigned long long inc = v;
 #pragma unroll
@@ -215,7 +218,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     }
     if (base) __syncthreads();
     if (lane == 31) scan[warp] = inc;
-    longer |= __syncthreads_or(more) != 0;
+    __syncthreads();
     unsigned long long before = sums + inc - v;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
@@ -229,6 +232,15 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
   }
   __syncthreads();
   const int total = static_cast<int>(sums), segments = static_cast<int>(sums >> 32);
+  // whether every segment is one team's: team i then takes segment i
+  bool direct = segments <= p.teams;
+  if (direct) {
+    const float share = static_cast<float>(total - segments * p.seg_cost) / (p.teams * TW);
+    const int whole = static_cast<int>(TW * (share + fminf(kWholeTiles + 0.9f * share, kWholeMost)));
+    bool longer = false;
+    for (int b = threadIdx.x; b < a.seqs; b += W * 32) longer |= tiles_of(seqs[b].count, seqs[b].len) > whole;
+    direct = !__syncthreads_or(longer);
+  }
 
   const int team_in_cta = warp / TW, wt = warp % TW;
   const int team = blockIdx.x * (W / TW) + team_in_cta;
@@ -250,7 +262,6 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
 
   // The team's share [t0, t1) of the list: no more teams than give each warp a tile; the first
   // `more` teams have one place more than the others.
-  const bool direct = !longer && segments <= p.teams;    // or team i takes segment i
   const int N = direct ? segments : min(p.teams, (total + TW - 1) / TW);
   if (team >= N) return;
   const int each = total / N, more = total - each * N;
