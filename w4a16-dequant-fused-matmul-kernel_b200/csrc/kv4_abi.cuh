@@ -264,10 +264,10 @@ int launch_decode(const w4a16_kv4_cache& c, const AttendParams& all, const Atten
 // such blocks leaves most SMs idle and takes as long as its longest sequence; the decode kernel reads it
 // once per 8 or 16 rows and splits it over all SMs. Up to kDecodeRows rows the decode kernel takes the
 // sequence, and every sequence of a batch of at most kDecodeWork rows x kv heads x sequences. Measured, 32
-// heads of 128 channels on 8 kv heads (decode kernel against the other, us): 8192 tokens, 128 rows: 35,
-// 139; 1024 rows: 157, 182; two sequences of 512 rows: 157, 183, and of 1024: 298, 184; 2048 tokens, 512
-// rows: 31, 61; 1024 rows: 79, 61; 16 sequences of 64 rows, 8192 tokens: 161, 188; of 128: 302, 189.
-constexpr long long kDecodeRows = 64, kDecodeWork = 6144;
+// heads of 128 channels on 8 kv heads (decode kernel against the other, us): one sequence of 8192 tokens, 128
+// rows: 35, 139; 1024 rows: 161, 184; 1536 rows: 232, 184; of 1500 tokens, 512 rows: 27, 51; 1024: 44, 51;
+// 1536: 78, 52; 16 sequences of 8192, 64 rows: 161, 188; 96: 236, 189.
+constexpr long long kDecodeRows = 64, kDecodeWork = 8192;
 
 long long decode_rows(const AttendPlan& plan) {
   return plan.rows <= kDecodeWork / std::max(1LL, plan.kv_heads * plan.seqs) ? plan.rows : std::min(plan.rows, kDecodeRows);

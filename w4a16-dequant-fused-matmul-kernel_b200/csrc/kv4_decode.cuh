@@ -32,8 +32,8 @@
 // that its own lane 0 issues. A piece's end passes through shared memory once: each warp leaves its
 // sums in the stage it has just read, and each then adds up some rows over all warps.
 //
-// Two sequences of 131071 and 78000 tokens, 32 heads of 128 channels on 8 kv heads (274 MB): 72 us, 3.8 TB/s;
-// 61 of up to 8000 tokens, 64 heads on 8 (298 MB): 77 us. Of the 72 us, 51 are the tile loop (5.4 TB/s, 84%
+// Two sequences of 131071 and 107000 tokens, 32 heads of 128 channels in groups of 64 on 8 kv heads (274 MB): 74 us;
+// 61 of up to 8000 tokens, 64 heads on 8 (298 MB): 79 us. Of the 74 us, 51 are the tile loop (5.4 TB/s, 84%
 // of a plain copy's rate); 3 go by until the first copy is issued (lengths, prefix sums, the table), 4 at a
 // piece's end and 5 in joining parts, which is what bounds short batches: 12.4 us for one sequence of 777
 // tokens.
