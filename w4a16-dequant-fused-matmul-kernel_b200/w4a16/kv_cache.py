@@ -94,6 +94,7 @@ class KV4Pages:
         assert kv_lens.shape[0] == block_table.shape[0], "kv_lens needs one entry per row of block_table"
         assert page_size >= 16 and page_size % 16 == 0, f"page_size={page_size} must be a multiple of 16"
         self.refs, self.block_table, self.kv_lens, self.page_size = refs, block_table, kv_lens, page_size
+        self._shape, self._index = (refs.shape[0], *block_table.shape), refs.get_device()
         self._struct = _lib.KV4TablesStruct(refs.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), refs.shape[0],
                                             block_table.shape[0], block_table.shape[1], page_size)
         self._ref = ctypes.byref(self._struct)
@@ -111,16 +112,28 @@ class KV4Pages:
 
     def like(self) -> "KV4Pages":
         """Tables of the same shape, not initialised."""
+        return self._like(0)[0]
+
+    def _like(self, extra: int) -> tuple["KV4Pages", Tensor, int]:
+        """:meth:`like`, in one allocation with ``extra`` ints behind the tables: (tables, buffer, the extra ints'
+        address). The views are made when they are asked for: between two operations nobody does."""
         new = object.__new__(KV4Pages)
-        P, (R, W) = self.refs.shape[0], self.block_table.shape
-        buf = self.refs.new_empty(R * W + P + R)      # one allocation; the table first, for its alignment
-        table, new.refs, new.kv_lens = buf.split((R * W, P, R))
-        new.block_table = table.view(R, W)
-        new.page_size = self.page_size
+        P, R, W = new._shape = self._shape
+        new._index, new.page_size = self._index, self.page_size
+        new._buf = buf = torch.empty(R * W + P + R + extra, dtype=_I32, device=self._index)   # the table first: aligned
         at = buf.data_ptr()
-        new._struct = _lib.KV4TablesStruct(at + 4 * R * W, at, at + 4 * (R * W + P), P, R, W, self.page_size)
+        refs, lens = at + 4 * R * W, at + 4 * (R * W + P)
+        new._struct = _lib.KV4TablesStruct(refs, at, lens, P, R, W, self.page_size)
         new._ref = ctypes.byref(new._struct)
-        return new
+        return new, buf, lens + 4 * R
+
+    def __getattr__(self, name: str):
+        if name not in ("refs", "block_table", "kv_lens") or "_buf" not in self.__dict__:
+            raise AttributeError(name)
+        P, R, W = self._shape
+        table, self.refs, self.kv_lens, _ = self._buf.split_with_sizes((R * W, P, R, self._buf.shape[0] - R * W - P - R))
+        self.block_table = table.view(R, W)
+        return self.__dict__[name]
 
 
 def _on(device_index: int, fn, *args) -> None:
@@ -358,17 +371,19 @@ def _ints(name: str, t: Tensor, n: int, device_index: int) -> None:
 
 
 def _check_pages(cache: KV4Cache, pages: KV4Pages) -> None:
-    assert pages.refs.get_device() == cache._index, "the tables must be on the cache's device"
-    assert pages.refs.shape[0] == cache.num_pages and pages.page_size == cache.page_size, (
+    assert pages._index == cache._index, "the tables must be on the cache's device"
+    assert pages._shape[0] == cache.num_pages and pages.page_size == cache.page_size, (
         "the tables must be of the cache's pages")
 
 
-def _tables_out(pages: KV4Pages, out: KV4Pages | None) -> KV4Pages:
+def _tables_out(pages: KV4Pages, out: KV4Pages | None, extra: int = 0) -> tuple[KV4Pages, Tensor | None, int | None]:
+    """(tables to write, a buffer that ends with ``extra`` ints, their address)."""
     if out is None:
-        return pages.like()
-    assert out.refs.shape == pages.refs.shape and out.block_table.shape == pages.block_table.shape and (
-        out.page_size == pages.page_size and out.refs.device == pages.refs.device), "out must be tables of the same shape"
-    return out
+        return pages._like(extra)
+    assert out._shape == pages._shape and out.page_size == pages.page_size and out._index == pages._index, (
+        "out must be tables of the same shape")
+    buf = torch.empty(extra, dtype=_I32, device=pages._index) if extra else None
+    return out, buf, None if buf is None else buf.data_ptr()
 
 
 def kv4_copy_pages(cache: KV4Cache, src: Tensor, dst: Tensor) -> None:
@@ -385,11 +400,11 @@ def kv4_reserve(pages: KV4Pages, rows: Tensor, lens: Tensor) -> Tensor:
     lowest ids, in the order of the requests, and its ``kv_lens`` becomes ``lens[i]``. Returns int32 [n]: 1, or
     0 (row unchanged) where the free pages do not reach that far down the list, the table is too narrow, or
     the row holds more than ``lens[i]`` already. Changes ``pages`` in place."""
-    d = pages.refs.get_device()
+    d = pages._index
     n = rows.shape[0] if rows.dim() == 1 else -1
     _ints("rows", rows, n, d)
     _ints("lens", lens, n, d)
-    buf = pages.refs.new_empty(2 * n + 1)
+    buf = torch.empty(2 * n + 1, dtype=_I32, device=d)
     _on(d, _lib.lib().w4a16_kv4_reserve, pages._ref, rows.data_ptr(), lens.data_ptr(), n, buf.data_ptr(),
         buf.data_ptr() + 4 * n)
     return buf[:n]
@@ -405,20 +420,19 @@ def kv4_fork(cache: KV4Cache, pages: KV4Pages, parents: Tensor, children: Tensor
     n = parents.shape[0] if parents.dim() == 1 else -1
     _ints("parents", parents, n, cache._index)
     _ints("children", children, n, cache._index)
-    out = _tables_out(pages, out)
-    buf = pages.refs.new_empty(3 * n)
+    out, buf, at = _tables_out(pages, out, 3 * n)      # ok, and 2 n of scratch
     _on(cache._index, _lib.lib().w4a16_kv4_fork, cache._ref, pages._ref, out._ref, parents.data_ptr(), children.data_ptr(),
-        n, buf.data_ptr(), buf.data_ptr() + 4 * n)
-    return out, buf[:n]
+        n, at, at and at + 4 * n)
+    return out, parents.new_empty(0) if buf is None else buf.narrow(0, buf.shape[0] - 3 * n, n)
 
 
 def kv4_release(pages: KV4Pages, rows: Tensor, *, out: KV4Pages | None = None) -> KV4Pages:
     """The rows (int32 [n]) give their pages back and are empty. Returns the tables (new ones, or ``out``, which
     may be ``pages``)."""
-    d = pages.refs.get_device()
+    d = pages._index
     n = rows.shape[0] if rows.dim() == 1 else -1
     _ints("rows", rows, n, d)
-    out = _tables_out(pages, out)
+    out = _tables_out(pages, out)[0]
     _on(d, _lib.lib().w4a16_kv4_release, pages._ref, out._ref, rows.data_ptr(), n)
     return out
 
@@ -428,7 +442,6 @@ def kv4_compact(cache: KV4Cache, pages: KV4Pages, *, out: KV4Pages | None = None
     with an id < c, in every layer, and the tables follow. The pages from c on are then free. Returns the tables
     (new ones, or ``out``, which may be ``pages``)."""
     _check_pages(cache, pages)
-    out = _tables_out(pages, out)
-    scratch = pages.refs.new_empty(2 * cache.num_pages + 1)
-    _on(cache._index, _lib.lib().w4a16_kv4_compact, cache._ref, pages._ref, out._ref, scratch.data_ptr())
+    out, buf, at = _tables_out(pages, out, 2 * cache.num_pages + 1)
+    _on(cache._index, _lib.lib().w4a16_kv4_compact, cache._ref, pages._ref, out._ref, at)
     return out
