@@ -123,10 +123,10 @@ struct Sequence {
 // A team takes one whole segment each, and nothing is joined, where there are teams enough and no segment
 // has many more tiles per warp than the warps' average share: kWholeTiles + 0.9 x the share more, at most
 // kWholeMost. Joining costs what four tiles of a warp alone take, and more where the memory is busy. Measured
-// (whole, split; us): 24 sequences of up to 3001, 5 rows, 16 kv heads of 64: 20.7, 24.8; 48 of 777, 20 rows, 8
-// kv heads of 128: 51, 84; 16 of 6000, 4 rows: 33, 41; one of 6000: 29, 18.5; 24 of 6000 on one kv head: 31,
+// (whole, split; us): 24 sequences with a window of 1024, 5 rows, 16 kv heads of 64: 20.7, 24.8; 48 of 777, 20
+// rows, 8 kv heads of 128: 51, 84; 16 of 6000, 4 rows: 33, 41; one of 6000: 29, 18.5; 24 of 6000 on one kv head: 31,
 // 20.7; 48 of 3000, 16 kv heads of 64: 69, 58.
-constexpr float kWholeTiles = 4.0f, kWholeMost = 13.0f;
+constexpr float kWholeTiles = 4.0f, kWholeMost = 9.0f;
 
 struct Segment {
   int start;               // its first tile's place in the list (after the seg_cost places without a tile)
