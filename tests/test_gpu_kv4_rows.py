@@ -1,0 +1,83 @@
+"""kv4_attention computes each query row as if it were alone: a row of another magnitude, or with an infinity
+or NaN in it, beside rows of ordinary ones, in every kernel and tile.
+
+Tolerance of a row, from its own numbers: half a unit in the last place of the output; probabilities (times value
+scales, or values beside them) rounded to fp16: 2^-11 of the largest value; scores in fp32, and the query's
+channels kept to 2^-24 of the row's largest: within 2e-5 of the row's own bound on its scores, |q| max |k| scale,
+which moves the mean by at most that times the spread of the values."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import w4a16
+from kv4_plain import PlainCache, attend
+from w4a16 import KV4Cache, kv4_attention
+
+pytestmark = pytest.mark.gpu
+
+HALF_ULP = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+F16, BF16 = torch.float16, torch.bfloat16
+FACTORS = [1e-6, 1e-3, 2.0 ** 10, 2.0 ** 14, 6e4, 1e8, 1e30, math.inf, -math.inf, math.nan]
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def check_rows(c, q, new, o, lse, skip=None, scale=None, window=0):
+    """Each row of q [T, heads, D] against the float64 form within the tolerance of its own scores; rows marked in
+    `skip` [T, heads] are left out."""
+    T, H, D = q.shape
+    sc = 1 / math.sqrt(D) if scale is None else scale
+    first = 0
+    for b, (n, m) in enumerate(zip(c.lens, new)):
+        if m == 0 or n == 0:
+            first += m
+            continue
+        rows = slice(first, first + m)
+        first += m
+        qq = q[rows].double()
+        keep = torch.ones((m, H), dtype=torch.bool, device="cuda") if skip is None else ~skip[rows]
+        want, wl = attend(torch.where(keep[..., None], qq, torch.zeros_like(qq)), c.k[b], c.v[b], H // c.kv, sc, window)
+        top = qq.norm(dim=-1) * c.k[b].norm(dim=-1).amax() * abs(sc)
+        vmax = c.v[b].abs().amax()
+        tol = HALF_ULP[q.dtype] * want.abs() + (2.0 ** -11 * vmax + 2e-5 * (1 + top) * vmax)[..., None]
+        err = (o[rows].double() - want).abs()
+        assert ((err <= tol) | ~keep[..., None]).all(), (b, (err / tol)[keep].max().item())
+        seen = keep & (wl > -math.inf)
+        assert ((lse[rows].double() - wl).abs() <= 2e-5 * (1 + top))[seen].all(), (b, (lse[rows].double() - wl)[seen].abs().max())
+
+
+def attend_with_one_row(factor, lens, new, H, KV, D, group, dtype, token, head):
+    """One row's largest channel (or, for a finite factor, the whole row) set apart."""
+    g = gen(H + D)
+    c = PlainCache(lens, KV, D, group, 32, gen=g)
+    cache = KV4Cache(1, c.num_pages, KV, D, page_size=32, group_size=group, pool=c.pool)
+    q = torch.randn((sum(new), H, D), generator=g, device="cuda").clamp(-1, 1).to(dtype)
+    if math.isfinite(factor):
+        q[token, head] *= factor
+    else:
+        q[token, head, 5] = factor
+    cu = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+    o, lse = kv4_attention(q, cache, 0, c.table, c.kv_lens, cu_q=cu, max_q=max(new), return_lse=True)
+    skip = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    skip[token, head] = not math.isfinite(factor)
+    check_rows(c, q, new, o, lse, skip)
+    if math.isnan(factor):
+        assert o[token, head].isnan().all()
+    assert w4a16.check_device_errors() == 0
+
+
+@pytest.mark.parametrize("factor", FACTORS)
+@pytest.mark.parametrize("lens,new,H,KV,D,group", [
+    ([777, 60], [1, 1], 16, 2, 128, 128),         # tiles of eight rows
+    ([300, 777], [3, 2], 16, 2, 128, 64),         # of sixteen
+    ([150, 40], [4, 9], 6, 2, 64, 64),
+])
+def test_single_and_drafted_tokens(factor, lens, new, H, KV, D, group):
+    if abs(factor) <= 65504 or not math.isfinite(factor):
+        attend_with_one_row(factor, lens, new, H, KV, D, group, F16, 0, 3)
+    attend_with_one_row(factor, lens, new, H, KV, D, group, BF16, sum(new) - 1, H - 1)

@@ -11,8 +11,10 @@
 // give 16 c * 2^-24; the queries' fragments for them carry 1/16, and the sums of the values'
 // channels with an odd nibble are divided by 16 at the end.
 //
-// The tile's queries are scaled to a largest magnitude in [1, 2) by a power of two (exact, and any
-// bf16 query then fits fp16). p s is the one rounding to 16 bits, h (2^-11). Rounded against codes of
+// Each row's queries are scaled by a power of two of its own to a largest magnitude in [2^14, 2^15): any bf16
+// query then fits fp16, its channels are exact down to 2^-24 of the row's largest (odd nibbles with their 1/16),
+// and no row's magnitude (an infinity, say) tells on its neighbours. It costs two multiplications per 16 tokens
+// and group: 1.5 us of 74 for the long case below, nothing in one group per head. p s is the one rounding to 16 bits, h (2^-11). Rounded against codes of
 // 7.5 on average it would cost more than a rounding of p against centred values, so the sum is
 // taken as sum h (c - 7.5) + sum p (b + 7.5 s), the second term in fp32; the sum of h comes from one
 // more product, with ones.
@@ -384,15 +386,16 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     // ---- the rows' queries as B fragments, their sums, and what a score is scaled by
     uint32_t qf[NT][KW][4];
     float qs[NT][2][NG];
+    float f[NT][2];                   // what a product is multiplied by, with the key's scale
     int to[NT][2], from[NT][2];       // tokens [from, to) that a row sees
-    float x[NT][KW][8], top = 0.0f;
+    const float units = a.scale * kLog2e;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = s.rt * ROWS + nt * 8 + r;
       const bool live = row < s.count * a.share;
       const uint16_t* src = static_cast<const uint16_t*>(a.q);
       if (live) src += (s.first + row / a.share) * a.q_st + (s.kh * a.share + row % a.share) * a.q_sh;
-      float sum[NG];
+      float x[KW][8], sum[NG], top = 0.0f;
 #pragma unroll
       for (int i = 0; i < NG; ++i) sum[i] = 0.0f;
 #pragma unroll
@@ -403,20 +406,35 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (p.bf16) {
-            x[nt][i][2 * j] = __uint_as_float(vv[j] << 16);
-            x[nt][i][2 * j + 1] = __uint_as_float(vv[j] & 0xffff0000u);
+            x[i][2 * j] = __uint_as_float(vv[j] << 16);
+            x[i][2 * j + 1] = __uint_as_float(vv[j] & 0xffff0000u);
           } else {
             const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&vv[j]));
-            x[nt][i][2 * j] = h.x;
-            x[nt][i][2 * j + 1] = h.y;
+            x[i][2 * j] = h.x;
+            x[i][2 * j + 1] = h.y;
           }
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          top = fmaxf(top, fabsf(x[nt][i][j]));
-          sum[NG == 1 ? 0 : i / 2] += x[nt][i][j];
+          top = fmaxf(top, fabsf(x[i][j]));
+          sum[NG == 1 ? 0 : i / 2] += x[i][j];
         }
       }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // 2^e <= top < 2^(e+1), kept where the powers of two below are normal (an infinity stays one)
+      const int e2 = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -112), 127);
+      const float down = __uint_as_float(static_cast<uint32_t>(127 + 14 - e2) << 23);
+      const float row_f = units * 1024.0f * __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);   // 2^24 2^(e - 14)
+#pragma unroll
+      for (int i = 0; i < KW; ++i)
+        // fragment words: nibbles (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16 of word key_word(i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float by = (j & 1) ? down * 0.0625f : down;
+          const __half2 h = __floats2half2_rn(x[i][j] * by, x[i][j + 4] * by);
+          qf[nt][i][j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
@@ -427,29 +445,13 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
       for (int c = 0; c < 2; ++c) {   // accumulators hold rows 2 q4 and 2 q4 + 1
         const int src_lane = 4 * (2 * q4 + c);
 #pragma unroll
-        for (int i = 0; i < NG; ++i) qs[nt][c][i] = __shfl_sync(0xffffffffu, sum[i] * (a.scale * kLog2e), src_lane);
+        for (int i = 0; i < NG; ++i) qs[nt][c][i] = __shfl_sync(0xffffffffu, sum[i] * units, src_lane);
+        f[nt][c] = __shfl_sync(0xffffffffu, row_f, src_lane);
         // a row past the last sees everything, so that it makes no tile an edge
         to[nt][c] = __shfl_sync(0xffffffffu, live ? min(s.len, pos + 1) : s.len, src_lane);
         from[nt][c] = __shfl_sync(0xffffffffu, live && a.window ? max(0, pos - a.window + 1) : 0, src_lane);
       }
     }
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    // 2^e <= top < 2^(e+1), kept where 2^-e and 2^e are normal
-    const int e2 = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
-    const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
-    const float f = a.scale * kLog2e * 16777216.0f * __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < KW; ++i)
-        // fragment words: nibbles (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16 of word key_word(i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float by = (j & 1) ? down * 0.0625f : down;
-          const __half2 h = __floats2half2_rn(x[nt][i][j] * by, x[nt][i][j + 4] * by);
-          qf[nt][i][j] = *reinterpret_cast<const uint32_t*>(&h);
-        }
     int all_from = 0, all_to = 0x7fffffff;   // tokens that every row of this warp's tile sees
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -530,12 +532,12 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
           }
           const float2 pr0 = __half22float2(*reinterpret_cast<const __half2*>(&pairs[r * NG + gr]));
           const float2 pr1 = __half22float2(*reinterpret_cast<const __half2*>(&pairs[(r + 8) * NG + gr]));
-          const float s0 = pr0.x * f, s1 = pr1.x * f;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              y[k][nt][c] = fmaf(d[nt][c], c < 2 ? s0 : s1, fmaf(c < 2 ? pr0.y : pr1.y, qs[nt][c & 1][gr], y[k][nt][c]));
+              y[k][nt][c] = fmaf(d[nt][c], (c < 2 ? pr0.x : pr1.x) * f[nt][c & 1],
+                                 fmaf(c < 2 ? pr0.y : pr1.y, qs[nt][c & 1][gr], y[k][nt][c]));
         }
       }
       if constexpr (EDGE) {
