@@ -81,3 +81,31 @@ def test_single_and_drafted_tokens(factor, lens, new, H, KV, D, group):
     if abs(factor) <= 65504 or not math.isfinite(factor):
         attend_with_one_row(factor, lens, new, H, KV, D, group, F16, 0, 3)
     attend_with_one_row(factor, lens, new, H, KV, D, group, BF16, sum(new) - 1, H - 1)
+
+
+@pytest.mark.parametrize("magnitude", [1e5, 1e8, 1e12, 1e30])
+@pytest.mark.parametrize("lens,new,H,KV,D,group", [
+    ([400, 150], [130, 70], 64, 8, 128, 128), ([300, 140], [140, 66], 64, 8, 128, 64), ([290, 290], [131, 100], 64, 8, 64, 64),
+    ([777, 60], [1, 1], 16, 2, 128, 128),
+])
+def test_queries_whose_scores_pass_the_resolution_of_fp32(magnitude, lens, new, H, KV, D, group):
+    """A result is then some mean of the values of the tokens whose scores are largest up to that resolution, and
+    finite: 2^-11 of the values apart (each rounded to fp16), and half a unit of bf16."""
+    g = gen(7)
+    c = PlainCache(lens, KV, D, group, 32, gen=g)
+    cache = KV4Cache(1, c.num_pages, KV, D, page_size=32, group_size=group, pool=c.pool)
+    q = (torch.randn((sum(new), H, D), generator=g, device="cuda") * magnitude).bfloat16()
+    cu = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+    o, lse = kv4_attention(q, cache, 0, c.table, c.kv_lens, cu_q=cu, max_q=max(new), return_lse=True)
+    assert o.isfinite().all() and lse.isfinite().all()
+    first = 0
+    for b, (n, m) in enumerate(zip(lens, new)):
+        qq = q[first:first + m].double()
+        vmax = c.v[b].abs().amax()
+        got = o[first:first + m].double()
+        assert (got.abs() <= vmax * (1 + 2.0 ** -8 + 2.0 ** -11)).all()
+        _, wl = attend(qq, c.k[b], c.v[b], H // KV, 1 / math.sqrt(D), 0)
+        top = qq.norm(dim=-1) * c.k[b].norm(dim=-1).amax() / math.sqrt(D)
+        assert ((lse[first:first + m].double() - wl).abs() <= 2e-5 * (1 + top)).all()
+        first += m
+    assert w4a16.check_device_errors() == 0

@@ -54,6 +54,10 @@ constexpr int PF_THREADS = 14 * 32;
 // fp16 as those below 1. At 2.9 (the decode kernel's, whose probabilities carry a scale) 14% of a long
 // prompt's steps took the rescaling path.
 constexpr float kPfLazyMax = 8.0f;
+// A score's two terms are at most 65504 |scale| log2(e) sum|q|. Up to this sum they are below 2^25, and taking the
+// maximum off inside the sum moves a score by a few units at most. A block with a row beyond takes it off afterwards, so that
+// the largest score is zero exactly (at scores of 1e12 all others were off by 1e5, and sums of nothing).
+constexpr float kPfPlainSum = 512.0f;
 constexpr int PF_TILE = 128 * 128;   // bytes of a [128][64] fp16 tile
 constexpr int PF_RING = 4;           // K tiles, and V tiles
 constexpr int PF_PARS = 8;           // steps whose pairs are kept
@@ -156,8 +160,8 @@ __device__ __forceinline__ uint8_t* swizzled(uint8_t* tile, int row, int chunk) 
 }
 
 // A step's probabilities with the maximum m: h in fp16, packed by token pairs, and their sum; returns
-// the largest score over m. EDGE: some row does not
-// see every token; this one sees [rel_from, rel_to) of the step.
+// the largest score. EDGE: some row does not see every token (this one sees [rel_from, rel_to) of the step),
+// or has large scores.
 template <int NG, int TOK, bool EDGE>
 __device__ __forceinline__ float step_probabilities(uint32_t s_at, const float4* par, float m, const float (&qs)[NG],
                                                     int rel_from, int rel_to, uint32_t (&h)[TOK / 2], float& l_add) {
@@ -178,7 +182,7 @@ __device__ __forceinline__ float step_probabilities(uint32_t s_at, const float4*
 #pragma unroll
     for (int i = 0; i < COLS; i += 2) {
       float4 q[NG];
-      float2 y = make_float2(-m, -m);
+      float2 y = EDGE ? make_float2(0.0f, 0.0f) : make_float2(-m, -m);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         q[g] = par[(c * COLS + i) / 2 * NG + g];
@@ -194,13 +198,14 @@ __device__ __forceinline__ float step_probabilities(uint32_t s_at, const float4*
         if (tok + 1 < rel_from || tok + 1 >= rel_to) y.y = -INFINITY;
       }
       top = fmaxf(top, fmaxf(y.x, y.y));
+      if (EDGE) y = __fadd2_rn(y, make_float2(-m, -m));
       const float2 e = make_float2(ex2(y.x), ex2(y.y));
       sum = __fadd2_rn(sum, e);
       h[(c * COLS + i) / 2] = pack2<__half>(e.x, e.y);
     }
   }
   l_add = sum.x + sum.y;
-  return top;
+  return EDGE ? top : m + top;
 }
 
 template <int D, int NG>
@@ -269,12 +274,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   float qs[NG];                    // sums of the row's queries per group, times scale log2(e)
   int row = 0;
   uint4 v[CHUNKS];
+  bool large = false;
   if (warp < 8) {
     row = row0 + threadIdx.x;
     const bool live = row <= last_row;
     const uint16_t* src = static_cast<const uint16_t*>(a.q);
     if (live) src += (first + row / a.share) * a.q_st + (kh * a.share + row % a.share) * a.q_sh;
-    float top = 0.0f;
+    float top = 0.0f, all = 0.0f;
 #pragma unroll
     for (int i = 0; i < NG; ++i) qs[i] = 0.0f;
 #pragma unroll
@@ -287,16 +293,18 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
         if (p.bf16) h = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
         else h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
         top = fmaxf(top, fmaxf(fabsf(h.x), fabsf(h.y)));
+        all += fabsf(h.x) + fabsf(h.y);
         qs[c / (CHUNKS / NG)] += h.x + h.y;
       }
     }
+    large = fabsf(a.scale * kLog2e) * all > kPfPlainSum;
 #pragma unroll
     for (int i = 0; i < NG; ++i) qs[i] *= a.scale * kLog2e;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) atomicMax(qmax, __float_as_uint(top));
   }
-  __syncthreads();
+  large = __syncthreads_or(large);
   const int e2 = min(max(static_cast<int>(*qmax >> 23) - 127, -100), 100);
   // what a product of codes c 2^-24 and scaled queries is multiplied by, with the key's scale
   const float f = a.scale * kLog2e * 16777216.0f * __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
@@ -491,19 +499,20 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       if (!ok) break;
       tc_fence_after();
       const int tok0 = (step0 + j) * TOK;
-      const bool edge = tok0 < all_from || tok0 + TOK > all_to;
+      const bool edge = large || tok0 < all_from || tok0 + TOK > all_to;
       const float4* par = pars + slot * 32;
       uint32_t h[TOK / 2];
       float l_add;
 #pragma unroll 1
       for (int pass = 0; pass < 2; ++pass) {
-        const float top = edge ? step_probabilities<NG, TOK, true>(buf, par, m, qs, see_from - tok0, see_to - tok0, h, l_add)
+        const float most = edge ? step_probabilities<NG, TOK, true>(buf, par, m, qs, see_from - tok0, see_to - tok0, h, l_add)
                                : step_probabilities<NG, TOK, false>(buf, par, m, qs, 0, 0, h, l_add);
-        const bool grow = top > (fresh ? -INFINITY : kPfLazyMax);
+        const float over = most - m;
+        const bool grow = over > (fresh ? -INFINITY : kPfLazyMax);
         if (pass || !__any_sync(0xffffffffu, grow)) break;
-        const float by = grow && !fresh ? ex2(-top) : 1.0f;
+        const float by = grow && !fresh ? ex2(-over) : 1.0f;
         if (grow) {
-          m += top;
+          m = most;
           fresh = false;
         }
         l *= by;
