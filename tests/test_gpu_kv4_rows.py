@@ -109,3 +109,36 @@ def test_queries_whose_scores_pass_the_resolution_of_fp32(magnitude, lens, new, 
         assert ((lse[first:first + m].double() - wl).abs() <= 2e-5 * (1 + top)).all()
         first += m
     assert w4a16.check_device_errors() == 0
+
+
+@pytest.mark.parametrize("factor", FACTORS)
+@pytest.mark.parametrize("lens,new,H,KV,D,group", [
+    ([400, 150], [130, 70], 64, 8, 128, 128),     # more than 8192 rows x kv heads x sequences, and than 64 rows
+    ([300, 140], [140, 66], 64, 8, 128, 64),
+    ([290, 290], [131, 100], 64, 8, 64, 64),
+])
+def test_prompts(factor, lens, new, H, KV, D, group):
+    assert max(new) * (H // KV) * KV * len(new) > 8192
+    if abs(factor) <= 65504 or not math.isfinite(factor):
+        attend_with_one_row(factor, lens, new, H, KV, D, group, F16, 37, 3)
+    attend_with_one_row(factor, lens, new, H, KV, D, group, BF16, sum(new) - 1, H - 1)
+    attend_with_one_row(factor, lens, new, H, KV, D, group, BF16, 0, 9)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_rows_of_all_magnitudes_in_one_prompt(dtype):
+    """Every row of its own magnitude, rows of zeros among them, windows and a last tile of few rows."""
+    g = gen(4)
+    new, H, KV, D = [150, 35], 64, 8, 128
+    c = PlainCache([333, 35], KV, D, D, 32, gen=g)
+    cache = KV4Cache(1, c.num_pages, KV, D, page_size=32, pool=c.pool)
+    span = 14 if dtype is F16 else 40
+    q = torch.randn((sum(new), H, D), generator=g, device="cuda").clamp(-1, 1)
+    q *= 2.0 ** torch.randint(-span, span + 1, (sum(new), H, 1), generator=g, device="cuda").float()
+    q[::7, ::3] = 0
+    q = q.to(dtype)
+    cu = torch.tensor([0, 150, 185], dtype=torch.int32, device="cuda")
+    for window in (0, 40):
+        o, lse = kv4_attention(q, cache, 0, c.table, c.kv_lens, cu_q=cu, max_q=150, window=window, return_lse=True)
+        check_rows(c, q, new, o, lse, window=window)
+    assert w4a16.check_device_errors() == 0

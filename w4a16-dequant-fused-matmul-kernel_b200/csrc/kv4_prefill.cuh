@@ -34,6 +34,12 @@
 // A value pair that is not finite becomes zeros in V, where a row that does not see the token would
 // meet it as 0 NaN; the rows that do see it are marked and get NaN in those channels at the end.
 //
+// The block's queries are scaled by one power of two, to a largest finite magnitude in [2^14, 2^15), which fits
+// fp16. It keeps the channels of a row down to 2^-24 of the block's largest (odd nibbles with their 1/16): enough for
+// rows whose largest channel is within 2^kPfSpread of that. Where some row lies below, each row has its own power
+// of two, and its products the ratio of it to the block's: one packed multiplication per two products, which only the
+// steps at the causal edge and those of such blocks carry.
+//
 // TMEM columns: S0 2 x 64, S1 2 x 64 (with P over them), O0 128, O1 128: all 512. Channels lie in the
 // order 0 4 1 5 2 6 3 7 inside each eight (how a masked word gives them): in Q and K alike, which
 // leaves the scores as they are, and in V, which the last step undoes.
@@ -58,6 +64,7 @@ constexpr float kPfLazyMax = 8.0f;
 // maximum off inside the sum moves a score by a few units at most. A block with a row beyond takes it off afterwards, so that
 // the largest score is zero exactly (at scores of 1e12 all others were off by 1e5, and sums of nothing).
 constexpr float kPfPlainSum = 512.0f;
+constexpr int kPfSpread = 13;
 constexpr int PF_TILE = 128 * 128;   // bytes of a [128][64] fp16 tile
 constexpr int PF_RING = 4;           // K tiles, and V tiles
 constexpr int PF_PARS = 8;           // steps whose pairs are kept
@@ -161,10 +168,10 @@ __device__ __forceinline__ uint8_t* swizzled(uint8_t* tile, int row, int chunk) 
 
 // A step's probabilities with the maximum m: h in fp16, packed by token pairs, and their sum; returns
 // the largest score. EDGE: some row does not see every token (this one sees [rel_from, rel_to) of the step),
-// or has large scores.
+// or has large scores or a power of two of its own: its products are to be multiplied by `ratio`.
 template <int NG, int TOK, bool EDGE>
 __device__ __forceinline__ float step_probabilities(uint32_t s_at, const float4* par, float m, const float (&qs)[NG],
-                                                    int rel_from, int rel_to, uint32_t (&h)[TOK / 2], float& l_add) {
+                                                    int rel_from, int rel_to, float ratio, uint32_t (&h)[TOK / 2], float& l_add) {
   constexpr int COLS = 16, CHUNK = TOK / COLS;
   float top = -INFINITY;
   float2 sum = make_float2(0.0f, 0.0f);
@@ -189,9 +196,11 @@ __device__ __forceinline__ float step_probabilities(uint32_t s_at, const float4*
         y = __ffma2_rn(make_float2(q[g].z, q[g].w), make_float2(qs[g], qs[g]), y);
       }
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
-        y = __ffma2_rn(make_float2(__uint_as_float(x[c][g][i]), __uint_as_float(x[c][g][i + 1])),
-                       make_float2(q[g].x, q[g].y), y);
+      for (int g = 0; g < NG; ++g) {
+        float2 s = make_float2(__uint_as_float(x[c][g][i]), __uint_as_float(x[c][g][i + 1]));
+        if (EDGE) s = __fmul2_rn(s, make_float2(ratio, ratio));
+        y = __ffma2_rn(s, make_float2(q[g].x, q[g].y), y);
+      }
       if (EDGE) {
         const int tok = c * COLS + i;
         if (tok < rel_from || tok >= rel_to) y.x = -INFINITY;
@@ -243,7 +252,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   uint64_t *sfull = parfull + PF_PARS, *pfull = sfull + 4;        // [tile][buffer of S], pvdone too
   uint64_t *pvdone = pfull + 4, *drain = pvdone + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-  uint32_t* qmax = tmem_slot + 1;
+  uint32_t *qmax = tmem_slot + 1, *qmin = tmem_slot + 2;   // largest and smallest of the rows' largest magnitudes
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -261,6 +270,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
     }
     mbar_init(drain, two ? 2 : 1);
     *qmax = 0;
+    *qmin = 0x7f800000u;
     mbar_fence_init();
   }
   if (warp == 12) {
@@ -269,18 +279,18 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   }
 
   __syncthreads();
-  // ---- queries: thread = row; all of the block's scaled by one power of two to a largest magnitude in
-  // [1, 2) (exact), so bf16 ones fit fp16
+  // ---- queries: thread = row
   float qs[NG];                    // sums of the row's queries per group, times scale log2(e)
+  float top = 0.0f;                // the row's largest magnitude
   int row = 0;
   uint4 v[CHUNKS];
-  bool large = false;
+  bool special = false;            // some row has large scores, or a power of two of its own
   if (warp < 8) {
     row = row0 + threadIdx.x;
     const bool live = row <= last_row;
     const uint16_t* src = static_cast<const uint16_t*>(a.q);
     if (live) src += (first + row / a.share) * a.q_st + (kh * a.share + row % a.share) * a.q_sh;
-    float top = 0.0f, all = 0.0f;
+    float all = 0.0f;
 #pragma unroll
     for (int i = 0; i < NG; ++i) qs[i] = 0.0f;
 #pragma unroll
@@ -297,19 +307,30 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
         qs[c / (CHUNKS / NG)] += h.x + h.y;
       }
     }
-    large = fabsf(a.scale * kLog2e) * all > kPfPlainSum;
+    special = fabsf(a.scale * kLog2e) * all > kPfPlainSum;
 #pragma unroll
     for (int i = 0; i < NG; ++i) qs[i] *= a.scale * kLog2e;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) atomicMax(qmax, __float_as_uint(top));
+    // rows of zeros, and those with an infinity (which have no result to be exact in), have no say
+    if (!(top < INFINITY)) top = 0.0f;
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    const uint32_t lo = __reduce_min_sync(0xffffffffu, top > 0.0f ? __float_as_uint(top) : 0x7f800000u);
+    if (lane == 0) {
+      atomicMax(qmax, hi);
+      atomicMin(qmin, lo);
+    }
   }
-  large = __syncthreads_or(large);
-  const int e2 = min(max(static_cast<int>(*qmax >> 23) - 127, -100), 100);
-  // what a product of codes c 2^-24 and scaled queries is multiplied by, with the key's scale
-  const float f = a.scale * kLog2e * 16777216.0f * __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
+  special = __syncthreads_or(special);
+  // exponents, kept where the powers of two below are normal
+  auto exponent = [](uint32_t bits) { return max(static_cast<int>(bits >> 23) - 127, -112); };
+  const int e2 = exponent(*qmax);
+  const bool apart = e2 - exponent(*qmin) > kPfSpread;
+  special |= apart;
+  const int e_row = apart && top > 0.0f ? exponent(__float_as_uint(top)) : e2;
+  const float ratio = e_row < e2 - 126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 + e_row - e2) << 23);
+  // what a product of codes c 2^-24 and queries scaled to 2^14 is multiplied by, with the key's scale
+  const float f = a.scale * kLog2e * 1024.0f * __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
   if (warp < 8) {
-    const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23), down16 = down * 0.0625f;
+    const float down = __uint_as_float(static_cast<uint32_t>(127 + 14 - e_row) << 23), down16 = down * 0.0625f;
     uint8_t* tile = qtile + (threadIdx.x >> 7) * KB * PF_TILE;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
@@ -499,14 +520,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
       if (!ok) break;
       tc_fence_after();
       const int tok0 = (step0 + j) * TOK;
-      const bool edge = large || tok0 < all_from || tok0 + TOK > all_to;
+      const bool edge = special || tok0 < all_from || tok0 + TOK > all_to;
       const float4* par = pars + slot * 32;
       uint32_t h[TOK / 2];
       float l_add;
 #pragma unroll 1
       for (int pass = 0; pass < 2; ++pass) {
-        const float most = edge ? step_probabilities<NG, TOK, true>(buf, par, m, qs, see_from - tok0, see_to - tok0, h, l_add)
-                               : step_probabilities<NG, TOK, false>(buf, par, m, qs, 0, 0, h, l_add);
+        const float most = edge ? step_probabilities<NG, TOK, true>(buf, par, m, qs, see_from - tok0, see_to - tok0, ratio, h, l_add)
+                                : step_probabilities<NG, TOK, false>(buf, par, m, qs, 0, 0, 1.0f, h, l_add);
         const float over = most - m;
         const bool grow = over > (fresh ? -INFINITY : kPfLazyMax);
         if (pass || !__any_sync(0xffffffffu, grow)) break;
