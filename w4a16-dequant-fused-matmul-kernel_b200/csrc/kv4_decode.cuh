@@ -17,7 +17,9 @@
 // and group: 1.5 us of 74 for the long case below, nothing in one group per head. p s is the one rounding to 16 bits, h (2^-11). Rounded against codes of
 // 7.5 on average it would cost more than a rounding of p against centred values, so the sum is
 // taken as sum h (c - 7.5) + sum p (b + 7.5 s), the second term in fp32; the sum of h comes from one
-// more product, with ones.
+// more product, with ones. So that h has its 11 bits for small values too, the values' scales are multiplied by
+// 2^10 (p s >= 2^-24 is then a normal number; unscaled, a mean of values of 1e-4 was off by 3%), and by less from the
+// first scale above 8 on that a warp meets, so that p s stays finite.
 //
 // Both products take the cache as the M side of mma.m16n8k16 (16 tokens, or 16 channels) and
 // eight query rows as its N side, so no row of the tensor core is wasted on padding queries when
@@ -52,8 +54,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNoMax = -1e30f;           // running maximum before any token
 // The running maximum follows only when a score exceeds it by this much (log2): p <= 7.46, and
-// p * s stays finite in fp16 as no scale exceeds (65504 + 65504) / 15 = 8734.
-constexpr float kLazyMax = 2.9f;
+// p * s stays finite in fp16 as the scales are brought to at most kMostScale.
+constexpr float kLazyMax = 2.9f, kMostScale = 8192.0f;
 constexpr int MAX_SEQS = 2048;             // sequences per launch (their prefix sums lie in shared memory)
 
 __device__ __forceinline__ float ex2(float x) {
@@ -452,6 +454,10 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
         from[nt][c] = __shfl_sync(0xffffffffu, live && a.window ? max(0, pos - a.window + 1) : 0, src_lane);
       }
     }
+    // tokens that some row of the tile sees
+    const int last_row = min((s.rt + 1) * ROWS, s.count * a.share) - 1, pos0 = s.len - s.count;
+    const int any_to = min(s.len, pos0 + last_row / a.share + 1);
+    const int any_from = a.window ? max(0, pos0 + s.rt * ROWS / a.share - a.window + 1) : 0;
     int all_from = 0, all_to = 0x7fffffff;   // tokens that every row of this warp's tile sees
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -468,6 +474,8 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
 
     float acc[NT][SETS * 4][4] = {}, hsum[NT][NG][4] = {};
     float m[NT][2], l[NT][2], corr[NT][2][NG];
+    float vs = kMostScale / 8;                 // what the values' scales are multiplied by,
+    uint32_t vs_for = 0x4800;                  // up to this one (fp16: 8)
     unsigned fresh = (1u << (2 * NT)) - 1u;    // rows that have seen no token yet (their m is 0 until then)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -552,9 +560,19 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
             }
       }
 
+      // ---- the values' scales, a token and group per lane at a time: is one too large
+      constexpr int SCALES = TT * NG / 32;
+      auto pair_of = [&](int i) {
+        const int at = i * 32 + lane;
+        return tile + at / (BLK * NG) * SH::BLOCK + value_pairs_at(D, NG) + at % (BLK * NG) * 4;
+      };
+      bool look = false;
+#pragma unroll
+      for (int i = 0; i < SCALES; ++i) look |= (*reinterpret_cast<const uint16_t*>(pair_of(i)) & 0x7fffu) > vs_for;
+
       // ---- running maximum
       float top_y[NT][2];
-      bool grows = fresh != 0;
+      bool grows = fresh != 0 || look;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -566,6 +584,34 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
           grows |= v > kLazyMax;
         }
       if (__any_sync(0xffffffffu, grows)) {
+        if (__any_sync(0xffffffffu, look)) {
+          uint32_t most = 0;
+#pragma unroll 1
+          for (int i = 0; i < SCALES; ++i) {
+            const int at = i * 32 + lane, k = at / (BLK * NG), tok = tok0 + at / NG;
+            const uint32_t sc = *reinterpret_cast<const uint16_t*>(pair_of(i)) & 0x7fffu;
+            // (tokens that no row sees, and scales that are not finite, have no say)
+            const bool seen = !EDGE || (((blocks >> k) & 1u) && tok >= any_from && tok < any_to);
+            if (seen && sc < 0x7c00u) most = max(most, sc);
+          }
+          most = __reduce_max_sync(0xffffffffu, most);
+          if (most > vs_for) {
+            const int e = static_cast<int>(most >> 10) - 15;       // most < 2^(e + 1)
+            vs_for = (most & 0x7c00u) + 0x400u;
+            const float to = __uint_as_float(static_cast<uint32_t>(127 + 12 - e) << 23);
+            const float by = to / vs;
+            vs = to;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                for (int i = 0; i < NG; ++i) hsum[nt][i][c] *= by;
+#pragma unroll
+                for (int i = 0; i < SETS * 4; ++i) acc[nt][i][c] *= by;
+              }
+          }
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -616,6 +662,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
           const float2 pr0 = __half22float2(*reinterpret_cast<const __half2*>(&pairs[r * NG + gr]));
           const float2 pr1 = __half22float2(*reinterpret_cast<const __half2*>(&pairs[(r + 8) * NG + gr]));
           const float o0 = fmaf(7.5f, pr0.x, pr0.y), o1 = fmaf(7.5f, pr1.x, pr1.y);
+          const float sv0 = pr0.x * vs, sv1 = pr1.x * vs;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float ps[4];
@@ -623,13 +670,13 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
                 const float pv = y[k][nt][c];
-                ps[c] = pv == 0.0f ? 0.0f : pv * (c < 2 ? pr0.x : pr1.x);
+                ps[c] = pv == 0.0f ? 0.0f : pv * (c < 2 ? sv0 : sv1);
                 if (pv != 0.0f) corr[nt][c & 1][gr] = fmaf(pv, c < 2 ? o0 : o1, corr[nt][c & 1][gr]);
               }
             } else {
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
-                ps[c] = y[k][nt][c] * (c < 2 ? pr0.x : pr1.x);
+                ps[c] = y[k][nt][c] * (c < 2 ? sv0 : sv1);
                 corr[nt][c & 1][gr] = fmaf(y[k][nt][c], c < 2 ? o0 : o1, corr[nt][c & 1][gr]);
               }
             }
@@ -675,6 +722,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     }
 
     // ---- this warp's sums over its lanes of tokens
+    const float back = 1.0f / vs;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -691,7 +739,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
       for (int c = 0; c < 2; ++c) {
         if ((fresh >> (2 * nt + c)) & 1u) m[nt][c] = kNoMax;
 #pragma unroll
-        for (int i = 0; i < NG; ++i) corr[nt][c][i] = fmaf(-7.5f, hsum[nt][i][c], corr[nt][c][i]);
+        for (int i = 0; i < NG; ++i) corr[nt][c][i] = fmaf(-7.5f * back, hsum[nt][i][c], corr[nt][c][i]);
       }
 
     // ---- the warp's sums into the stage it has just read, the rest beside
@@ -701,7 +749,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int i = 0; i < SETS * 4; ++i)
-          sums[(nt * SETS * 4 + i) * 32] = make_float4(acc[nt][i][0], acc[nt][i][1], acc[nt][i][2], acc[nt][i][3]);
+          sums[(nt * SETS * 4 + i) * 32] = make_float4(acc[nt][i][0] * back, acc[nt][i][1] * back, acc[nt][i][2] * back, acc[nt][i][3] * back);
         if (r == 0) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
