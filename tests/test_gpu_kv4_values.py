@@ -1,4 +1,4 @@
-"""kv4_attention on values of every size: small ones, and sizes that differ from token to token.
+"""kv4_attention on values of every size: small ones, sizes that differ from token to token, groups without spread.
 
 Tolerance of a result: half a unit in the last place of the output; probabilities times value scales (or values and
 probabilities) rounded to fp16, 2^-11 of the largest value the row may see; scores in fp32, within 2e-5 of the row's
@@ -154,3 +154,31 @@ def test_values_of_all_sizes_are_equally_exact(v_scale, n, new, H, KV, D, group)
     rms = (got - want).square().mean(-1).sqrt()
     tol = (2.0 ** -11 + 2e-6 * (1 + top)) * spread * vd.abs().amax() + 2.0 ** -8 * want.square().mean(-1).sqrt()
     assert (rms <= tol).all(), (rms / tol).max().item()
+
+
+@pytest.mark.parametrize("D,group", [(128, 128), (128, 64), (64, 64)])
+@pytest.mark.parametrize("new,share", [(1, 4), (3, 4), (70, 8)])
+def test_groups_without_spread(D, group, new, share):
+    """Values that are one number each group: zero, small, large, and one per token; beside them ordinary ones."""
+    g = gen(D + new)
+    n, KV = 517, 16
+    k = torch.randn((n, KV, D), generator=g, device="cuda").half()
+    v = torch.randn((n, KV, D), generator=g, device="cuda").half()
+    v[:, 0] = 0
+    v[:, 1] = 1e-3
+    v[:, 2] = 300.0
+    v[:, 3] = (torch.randn((n, 1), generator=g, device="cuda") * 1e-2).half()
+    v[:, 4, :64] = 0
+    v[::3, 5] = 0                                   # some tokens
+    v[:, 6] = (v[:, 6].float() * 1e-3).half()
+    v[::3, 6] = 1e-3                                # among small ones
+    cache, table, lens, kd, vd = appended(k, v, group)
+    q = (torch.randn((new, KV * share, D), generator=g, device="cuda") * 2).half()
+    o, lse = kv4_attention(q, cache, 0, table, lens, return_lse=True)
+    compare(q, kd, vd, o, lse, share)
+    o = o.unflatten(1, (KV, share)).double()
+    assert (o[:, 0] == 0).all()
+    if group == 64:
+        assert (o[:, 4, :, :64] == 0).all()
+    for head in (1, 2):                             # a mean of one number: fp32's and the output's roundings
+        assert ((o[:, head] - vd[0, head, 0]).abs() <= (2.0 ** -11 + 1e-5) * vd[0, head, 0]).all()

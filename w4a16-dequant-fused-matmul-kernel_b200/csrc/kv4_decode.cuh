@@ -14,12 +14,15 @@
 // Each row's queries are scaled by a power of two of its own to a largest magnitude in [2^14, 2^15): any bf16
 // query then fits fp16, its channels are exact down to 2^-24 of the row's largest (odd nibbles with their 1/16),
 // and no row's magnitude (an infinity, say) tells on its neighbours. It costs two multiplications per 16 tokens
-// and group: 1.5 us of 74 for the long case below, nothing in one group per head. p s is the one rounding to 16 bits, h (2^-11). Rounded against codes of
-// 7.5 on average it would cost more than a rounding of p against centred values, so the sum is
-// taken as sum h (c - 7.5) + sum p (b + 7.5 s), the second term in fp32; the sum of h comes from one
-// more product, with ones. So that h has its 11 bits for small values too, the values' scales are multiplied by
-// 2^10 (p s >= 2^-24 is then a normal number; unscaled, a mean of values of 1e-4 was off by 3%), and by less from the
-// first scale above 8 on that a warp meets, so that p s stays finite.
+// and group: 1 us of 73 for the long case below, nothing measurable with one group per head.
+//
+// p s is the one rounding to 16 bits, h (2^-11). Rounded against codes of 7.5 on average it would cost more than a
+// rounding of p against centred values, so the sum is taken as sum h (c - 7.5) + sum p (b + 7.5 s), the second term
+// in fp32; the sum of h comes from one more product, with ones. So that h has its 11 bits for small values too, the
+// values' scales are multiplied by 2^10 (p s >= 2^-24 is then a normal number; unscaled, a mean of values of 1e-4 is off
+// by 2%), and by less from the first scale above 8 on that a warp meets, so that p s stays finite. A group without
+// spread has the scale 1 and codes of zero: its scale is taken as zero, or 7.5 times the rounding of its p would stand
+// beside its offset, which may be nothing. Looking for both costs 0.2 us for one token and 2 of 76 for a batch.
 //
 // Both products take the cache as the M side of mma.m16n8k16 (16 tokens, or 16 channels) and
 // eight query rows as its N side, so no row of the tensor core is wasted on padding queries when
@@ -560,7 +563,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
             }
       }
 
-      // ---- the values' scales, a token and group per lane at a time: is one too large
+      // ---- the values' scales, a token and group per lane at a time: is one too large, or perhaps no scale
       constexpr int SCALES = TT * NG / 32;
       auto pair_of = [&](int i) {
         const int at = i * 32 + lane;
@@ -568,7 +571,10 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
       };
       bool look = false;
 #pragma unroll
-      for (int i = 0; i < SCALES; ++i) look |= (*reinterpret_cast<const uint16_t*>(pair_of(i)) & 0x7fffu) > vs_for;
+      for (int i = 0; i < SCALES; ++i) {
+        const uint32_t sc = *reinterpret_cast<const uint16_t*>(pair_of(i)) & 0x7fffu;
+        look |= sc > vs_for || sc == 0x3c00u;
+      }
 
       // ---- running maximum
       float top_y[NT][2];
@@ -589,7 +595,20 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
 #pragma unroll 1
           for (int i = 0; i < SCALES; ++i) {
             const int at = i * 32 + lane, k = at / (BLK * NG), tok = tok0 + at / NG;
-            const uint32_t sc = *reinterpret_cast<const uint16_t*>(pair_of(i)) & 0x7fffu;
+            uint16_t* pair = const_cast<uint16_t*>(reinterpret_cast<const uint16_t*>(pair_of(i)));
+            uint32_t sc = *pair & 0x7fffu;
+            if (sc == 0x3c00u) {
+              const uint4* codes = reinterpret_cast<const uint4*>(tile + k * SH::BLOCK + value_codes_at(D) +
+                                                                  at % (BLK * NG) * (D / 2 / NG));
+              uint32_t any = 0;
+#pragma unroll
+              for (int j = 0; j < D / 32 / NG; ++j) any |= codes[j].x | codes[j].y | codes[j].z | codes[j].w;
+              if (any == 0) {
+                *pair = 0;
+                fence_proxy_async_smem();      // the stage is copied into again
+                sc = 0;
+              }
+            }
             // (tokens that no row sees, and scales that are not finite, have no say)
             const bool seen = !EDGE || (((blocks >> k) & 1u) && tok >= any_from && tok < any_to);
             if (seen && sc < 0x7c00u) most = max(most, sc);
@@ -611,6 +630,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
                 for (int i = 0; i < SETS * 4; ++i) acc[nt][i][c] *= by;
               }
           }
+          __syncwarp();
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
