@@ -316,6 +316,13 @@ int w4a16_prefill_plan(int64_t M, int64_t N, int64_t K, int num_sms, int* which,
                        int* splits);
 
 /*
+ * Which CUDA graph capture `stream` is part of: a number of its own for each, 0 when it is not capturing. A workspace
+ * whose zeroing was captured is not zero until the graph runs, and one that a graph uses must not serve launches
+ * outside it at the same time: give each capture a workspace of its own, zeroed inside it.
+ */
+int w4a16_stream_capture_id(void* stream, uint64_t* id_out);
+
+/*
  * After W4A16_ERR_TIMEOUT: zero `workspace_bytes` of a caller's GEMM workspace
  * (when `workspace` is not NULL) and this device's w4a16_gemm_noalloc scratch
  * array (when set up), asynchronously on `stream`; allocates nothing. The next
@@ -498,7 +505,7 @@ int w4a16_kv4_gather(const w4a16_kv4_cache* cache, int64_t layer, const int64_t*
  * gives zeros and lse = -inf. max_q: at least the longest sequence's queries (ignored when cu_q is
  * null). workspace: w4a16_kv4_attention_workspace_size bytes, 256-byte aligned, ZEROED before its
  * first use and left ready for the next call on the same stream; calls that may run at the same time
- * need one each.
+ * need one each, and so does each graph capture (zeroed inside it). Only its first 65536 bytes have to be zero.
  */
 int w4a16_kv4_attention(const void* q, int dtype, int64_t T, int heads, int64_t q_token_stride, int64_t q_head_stride,
                         const w4a16_kv4_cache* cache, int64_t layer, const int32_t* block_table, int64_t table_width,

@@ -1142,6 +1142,19 @@ int w4a16_set_prefill_kernel(int which) {
   return W4A16_OK;
 }
 
+int w4a16_stream_capture_id(void* stream, uint64_t* id_out) {
+  if (id_out == nullptr) return W4A16_ERR_INVALID;
+  *id_out = 0;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+    cudaGetLastError();
+    return W4A16_ERR_LAUNCH;
+  }
+  if (status != cudaStreamCaptureStatusNone) *id_out = id;
+  return W4A16_OK;
+}
+
 int w4a16_reset_scratch(void* workspace, int64_t workspace_bytes, void* stream) {
   if (workspace_bytes < 0 || (workspace == nullptr && workspace_bytes != 0)) return W4A16_ERR_INVALID;
   DeviceState* dev = nullptr;

@@ -24,6 +24,7 @@ PREFILL_AUTO, PREFILL_SMEM_B, PREFILL_TMEM_A = 0, 1, 2
 W4A16_ERR_TIMEOUT = -5
 W4A16_ERR_WORKSPACE = -6
 W4A16_ERR_INDEX = -8
+KV4_ZEROED = 65536   # bytes of the attention's workspace that have to be zero before its first use
 DTYPE_CODES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
 
 _c_i64 = ctypes.c_int64
@@ -91,6 +92,7 @@ SIGNATURES = {
     "w4a16_p2p_open": ([_vp, ctypes.POINTER(_vp)], ctypes.c_int),
     "w4a16_p2p_close": ([_vp], ctypes.c_int),
     "w4a16_p2p_free": ([_vp], ctypes.c_int),
+    "w4a16_stream_capture_id": ([_vp, ctypes.POINTER(ctypes.c_uint64)], _c_int),
     "w4a16_kv4_page_bytes": ([_c_int] * 3 + [ctypes.POINTER(_c_i64)], _c_int),
     "w4a16_qk_norm_rope": ([_vp, _vp, _c_int, _c_i64] + [_c_int] * 3 + [_c_i64] * 4 + [_vp] + [_c_int] * 3 +
                            [_vp, _c_i64, _c_int, _c_int, _vp, _vp, _c_int, ctypes.c_float, _vp, _vp, _vp], _c_int),
@@ -198,6 +200,36 @@ _ws_cache: dict[tuple[int, int], torch.Tensor] = {}
 _kv4_ws_cache: dict[tuple[int, int], torch.Tensor] = {}   # attention's, which it does not leave zero
 _ws_retired: list[torch.Tensor] = []
 
+_capture_ws: dict[tuple[str, int, int], tuple[int, torch.Tensor]] = {}
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_current_captures = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
+def _captures(device_index: int, stream: int) -> bool:
+    """Whether the device's current stream, ``stream``, is being captured into a CUDA graph."""
+    return _current_captures() if device_index == _current_device() else capture_id(stream) != 0
+
+
+def capture_id(stream: int) -> int:
+    """A number of its own for each CUDA graph capture; 0 when ``stream`` is not capturing."""
+    out = ctypes.c_uint64(0)
+    check(lib().w4a16_stream_capture_id(stream, ctypes.byref(out)), "w4a16_stream_capture_id")
+    return int(out.value)
+
+
+def _capture_workspace(kind: str, nbytes: int, zeroed: int, device_index: int, stream: int) -> torch.Tensor:
+    """A workspace of the capture that ``stream`` is part of: in the graph's memory, its first ``zeroed`` bytes zeroed
+    inside the graph before the first call that uses it. What the graph's replays leave in it, in whatever order
+    with other graphs and calls outside, meets nobody else."""
+    key, capture = (kind, device_index, stream), capture_id(stream)
+    with _ws_lock:
+        made, ws = _capture_ws.get(key, (0, None))
+        if made != capture or ws.numel() < nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device_index)
+            ws[:zeroed].zero_()
+            _capture_ws[key] = (capture, ws)
+    return ws
+
 
 _ws_size_cache: dict[tuple[int, int, int, int, int], int] = {}
 
@@ -233,7 +265,10 @@ def gemm_workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tens
 
 
 def kv4_workspace(nbytes: int, device_index: int, stream: int) -> torch.Tensor:
-    """The attention kernels' scratch buffer (zeroed when made) of >= nbytes for this stream."""
+    """The attention kernels' scratch buffer (zeroed when made) of >= nbytes for this stream, or for the graph
+    capture that the stream is part of."""
+    if _captures(device_index, stream):
+        return _capture_workspace("kv4", nbytes, KV4_ZEROED, device_index, stream)
     key = (device_index, stream)
     ws = _kv4_ws_cache.get(key)
     if ws is None or ws.numel() < nbytes:
