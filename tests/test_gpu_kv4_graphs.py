@@ -13,13 +13,13 @@ pytestmark = pytest.mark.gpu
 
 
 class Dirt:
-    """A graph whose replay fills the free memory of a graph pool (and stream) with 0xFF."""
+    """A graph whose replay fills the free memory of a graph pool (and stream) with one 64-bit word."""
 
-    def __init__(self, pool, nbytes, stream=None):
+    def __init__(self, pool, nbytes, stream=None, word=-1):
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph, pool=pool, stream=stream):
-            x = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
-            x.fill_(255)
+            x = torch.empty(nbytes // 8, dtype=torch.int64, device="cuda")
+            x.fill_(word)
             del x
 
     def spread(self):
@@ -77,4 +77,32 @@ def test_calls_outside_a_graph_on_its_stream():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(large[4][0], large[3]) and torch.equal(small[4][0], small[3])
+    assert w4a16.check_device_errors() == 0
+
+
+def test_gemm_graphs_replayed_in_another_order():
+    """The GEMMs' workspace holds pieces of column strips (few rows) and counters of K splits (many rows)."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    K, N, G = 4096, 2048, 128
+    w = w4a16.quantize_weight((torch.randn((K, N), generator=g, device="cuda") * 0.02).half(), G)
+    pool = torch.cuda.graph_pool_handle()
+    dirt = Dirt(pool, 128 << 20, word=1 << 32)       # as a piece of a strip that has arrived looks, and odd counters of one
+    xs = [torch.randn((m, K), generator=g, device="cuda").half() for m in (1, 40, 8, 100)]
+    assert all(w4a16._lib.gemm_workspace_bytes(x.shape[0], N, K, G, x.device) > 0 for x in xs)
+    want = [w4a16.w4a16_matmul(x, *w, G) for x in xs]
+    outs = [torch.full((2, *y.shape), float("nan"), device="cuda", dtype=y.dtype) for y in want]
+    graphs = []
+    for x, out in zip(xs, outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            for o in out:
+                w4a16.w4a16_matmul(x, *w, G, out=o)
+        graphs.append(graph)
+    for order in ((2, 0, 3, 1), (1, 3), (0, 1, 2, 3)):
+        dirt.spread()
+        for i in order:
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i][0], want[i]) and torch.equal(outs[i][1], want[i]), (order, i)
+            outs[i].fill_(float("nan"))
     assert w4a16.check_device_errors() == 0

@@ -24,6 +24,7 @@ PREFILL_AUTO, PREFILL_SMEM_B, PREFILL_TMEM_A = 0, 1, 2
 W4A16_ERR_TIMEOUT = -5
 W4A16_ERR_WORKSPACE = -6
 W4A16_ERR_INDEX = -8
+GEMM_ZEROED = (5 << 20) + 65536   # bytes of a GEMM's workspace that have to be zero: the pieces', and the counters of K splits
 KV4_ZEROED = 65536   # bytes of the attention's workspace that have to be zero before its first use
 DTYPE_CODES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
 
@@ -192,8 +193,8 @@ def check_device_errors(device: torch.device | int | None = None) -> int:
 # ---------------------------------------------------------------------------
 # GEMM workspace: one zeroed buffer per (device, stream), grown on demand. The
 # decode kernel leaves it zero after every launch, so the buffer is
-# reused without clearing. Superseded buffers are kept alive because a CUDA
-# graph captured earlier may still refer to them.
+# reused without clearing. Superseded buffers are kept alive because another thread may
+# be launching with one. A graph capture has one of its own, zeroed inside the graph.
 # ---------------------------------------------------------------------------
 _ws_lock = threading.Lock()
 _ws_cache: dict[tuple[int, int], torch.Tensor] = {}
@@ -249,9 +250,12 @@ def gemm_workspace_bytes(M: int, N: int, K: int, G: int, device: torch.device) -
 
 
 def gemm_workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tensor | None:
-    """A zeroed, 256-byte-aligned scratch buffer of >= nbytes for this stream."""
+    """A zeroed, 256-byte-aligned scratch buffer of >= nbytes for this stream, or for the graph
+    capture that the stream is part of."""
     if nbytes <= 0:
         return None
+    if _captures(device.index, stream):
+        return _capture_workspace("gemm", nbytes, GEMM_ZEROED, device.index, stream)
     key = (device.index, stream)
     with _ws_lock:
         ws = _ws_cache.get(key)
@@ -287,16 +291,19 @@ _ws_for: dict[tuple[int, int, int, int, int, int], tuple[int | None, int]] = {}
 
 def workspace_for(M: int, N: int, K: int, G: int, device_index: int, stream: int) -> tuple[int | None, int]:
     """(pointer, bytes) of the zeroed workspace a GEMM of this shape uses on ``stream``
-    of device ``device_index``; (None, 0) when the shape needs none. Memoised: a hit
-    is one dictionary lookup (the buffer it names is kept alive by the cache below)."""
+    of device ``device_index``; (None, 0) when the shape needs none. Memoised outside graph
+    captures: a hit is one dictionary lookup (the buffer it names is kept alive by the cache below)."""
     key = (M, N, K, G, device_index, stream)
-    hit = _ws_for.get(key)
+    captures = _captures(device_index, stream)
+    hit = None if captures else _ws_for.get(key)
     if hit is not None:
         return hit
     dev = torch.device("cuda", device_index)
     nbytes = gemm_workspace_bytes(M, N, K, G, dev) if M > 0 and N > 0 else 0
     ws = gemm_workspace(nbytes, dev, stream)
     val = (None, 0) if ws is None else (ws.data_ptr(), ws.numel())
+    if captures:
+        return val
     with _ws_lock:
         # a later, larger request can replace the stream's buffer: drop memoised entries
         # that name a retired buffer
