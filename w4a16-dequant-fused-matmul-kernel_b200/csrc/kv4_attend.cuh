@@ -29,6 +29,12 @@ struct AttendParams {
   int groups;
 };
 
+// The first token that the query at position `pos` sees; a window may be anything up to the largest int, and a
+// position below zero (more new tokens than cached ones).
+__device__ __forceinline__ int sees_from(const AttendParams& p, int pos) {
+  return p.window && pos >= p.window ? pos - p.window + 1 : 0;
+}
+
 // A sequence's queries [first, first + count) and its cached tokens (none of what does not fit the
 // arrays).
 __device__ __forceinline__ void sequence(const AttendParams& p, int b, int& first, int& count, int& len) {

@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
   }
 
   // the first tile that some query of a sequence sees, how many there are, and its segments
-  auto tile0_of = [&](int count, int len) { return a.window ? max(0, len - count - a.window + 1) / TT : 0; };
+  auto tile0_of = [&](int count, int len) { return sees_from(a, len - count) / TT; };
   auto tiles_of = [&](int count, int len) { return count ? max(0, (len + TT - 1) / TT - tile0_of(count, len)) : 0; };
   auto segments_of = [&](int count) { return a.cache.kv_heads * ((count * a.share + ROWS - 1) / ROWS); };
 
@@ -454,13 +454,13 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
         f[nt][c] = __shfl_sync(0xffffffffu, row_f, src_lane);
         // a row past the last sees everything, so that it makes no tile an edge
         to[nt][c] = __shfl_sync(0xffffffffu, live ? min(s.len, pos + 1) : s.len, src_lane);
-        from[nt][c] = __shfl_sync(0xffffffffu, live && a.window ? max(0, pos - a.window + 1) : 0, src_lane);
+        from[nt][c] = __shfl_sync(0xffffffffu, live ? sees_from(a, pos) : 0, src_lane);
       }
     }
     // tokens that some row of the tile sees
     const int last_row = min((s.rt + 1) * ROWS, s.count * a.share) - 1, pos0 = s.len - s.count;
     const int any_to = min(s.len, pos0 + last_row / a.share + 1);
-    const int any_from = a.window ? max(0, pos0 + s.rt * ROWS / a.share - a.window + 1) : 0;
+    const int any_from = sees_from(a, pos0 + s.rt * ROWS / a.share);
     int all_from = 0, all_to = 0x7fffffff;   // tokens that every row of this warp's tile sees
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)

@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
   const int last_row = min(rows, row0 + PF_ROWS) - 1;
   // tokens some row of the block sees, in steps of TOK
   const int pos0 = len - count + row0 / a.share, pos1 = len - count + last_row / a.share;
-  const int from = a.window ? max(0, pos0 - a.window + 1) : 0, to = min(len, pos1 + 1);
+  const int from = sees_from(a, pos0), to = min(len, pos1 + 1);
   const int step0 = from / TOK;
   const int steps = max(0, (to + TOK - 1) / TOK - step0);
   const bool two = row0 + 128 <= last_row;
@@ -503,11 +503,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1) kv4_prefill_kernel(const Prefil
     const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + 256 + t * 128;
     const bool live = row <= last_row;
     const int pos = len - count + row / a.share;
-    const int see_to = live ? min(len, pos + 1) : len, see_from = live && a.window ? max(0, pos - a.window + 1) : 0;
+    const int see_to = live ? min(len, pos + 1) : len, see_from = live ? sees_from(a, pos) : 0;
     // tokens every row of this tile sees
     const int tile_last = min(last_row, row0 + t * 128 + 127);
     const int all_to = min(len, len - count + (row0 + t * 128) / a.share + 1);
-    const int all_from = a.window ? max(0, len - count + tile_last / a.share - a.window + 1) : 0;
+    const int all_from = sees_from(a, len - count + tile_last / a.share);
     float m = 0.0f, l = 0.0f;
     uint32_t nan_groups = 0;         // groups whose values are NaN in some token this row sees
     bool fresh = true, ok = true, scores = false, pairs = false;   // the next step's are there

@@ -27,6 +27,7 @@ _CODES = {torch.float16: _lib.DTYPE_CODES[torch.float16], torch.bfloat16: _lib.D
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _lib.stream_of_index)
 _CONTIGUOUS = torch.contiguous_format
+_INT_MAX = 2 ** 31 - 1
 
 
 class KV4Cache:
@@ -343,7 +344,7 @@ def kv4_attention(q: Tensor, cache: KV4Cache, layer: int, block_table: Tensor, k
     ws = _lib.kv4_workspace(need, d, _raw_stream(d)) if need else None
     _on(d, _lib.lib().w4a16_kv4_attention, q.data_ptr(), _CODES[dt], T, H, qt, qs, cache._ref, layer,
         block_table.data_ptr(), width, kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), B, max_q,
-        D ** -0.5 if scale is None else scale, window, o.data_ptr(), None if lse is None else lse.data_ptr(),
+        D ** -0.5 if scale is None else scale, min(window, _INT_MAX), o.data_ptr(), None if lse is None else lse.data_ptr(),
         None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
     return (o, lse) if return_lse else o
 
