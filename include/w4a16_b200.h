@@ -502,7 +502,7 @@ int w4a16_kv4_gather(const w4a16_kv4_cache* cache, int64_t layer, const int64_t*
  * beyond its length are not read); its queries are q[cu_q[b] : cu_q[b + 1]], or T / seqs each when
  * cu_q is null, the last of which stands at position kv_lens[b] - 1. A query sees the tokens up to its
  * own position, or the last `window` of those when window > 0; one that sees none (a length of 0)
- * gives zeros and lse = -inf. max_q: at least the longest sequence's queries (ignored when cu_q is
+ * gives zeros and lse = -inf, and so do queries before cu_q[0] and from cu_q[seqs] on. max_q: at least the longest sequence's queries (ignored when cu_q is
  * null). workspace: w4a16_kv4_attention_workspace_size bytes, 256-byte aligned, ZEROED before its
  * first use and left ready for the next call on the same stream; calls that may run at the same time
  * need one each, and so does each graph capture (zeroed inside it). Only its first 65536 bytes have to be zero.

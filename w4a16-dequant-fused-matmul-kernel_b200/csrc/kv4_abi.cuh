@@ -243,6 +243,8 @@ int launch_decode(const w4a16_kv4_cache& c, const AttendParams& all, const Atten
       }
       p.bf16 = bf16;
       p.row_limit = row_limit;
+      p.before = b0 == 0;
+      p.after = b0 + p.a.seqs == all.seqs;
       p.team_warps = tw;
       // a piece's queries and end cost a team about what three tiles of each of its warps do (6 us
       // where a tile takes 2)

@@ -100,6 +100,7 @@ struct DecodeParams {
   AttendParams a;
   int bf16;                // q and o bf16, else fp16
   int row_limit;           // sequences with more rows than this are left to the other kernel
+  int before, after;       // whether queries before cu_q[0], and from cu_q[seqs] on, are this launch's
   int team_warps;          // warps per team: 1, 2, 4, ... W
   int seg_cost;            // tiles that a segment counts more than it has
   int teams;               // most teams (CTAs * W / team_warps)
@@ -265,6 +266,20 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     for (long long i = wt * 32 + lane; i < rows * (D / 8); i += TW * 32) o[i] = make_uint4(0, 0, 0, 0);
     if (a.lse)
       for (long long i = wt * 32 + lane; i < rows; i += TW * 32) a.lse[at + i] = -INFINITY;
+  }
+
+  // queries of no sequence
+  if (a.cu_q) {
+    const int head = p.before ? min(max(a.cu_q[0], 0), a.T) : 0, tail = p.after ? max(a.cu_q[a.seqs], head) : a.T;
+    const long long step = static_cast<long long>(gridDim.x) * W * 32, at = blockIdx.x * W * 32LL + threadIdx.x;
+    auto nothing = [&](long long first, long long rows) {
+      uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + first * a.heads * D);
+      for (long long i = at; i < rows * a.heads * (D / 8); i += step) o[i] = make_uint4(0, 0, 0, 0);
+      if (a.lse)
+        for (long long i = at; i < rows * a.heads; i += step) a.lse[first * a.heads + i] = -INFINITY;
+    };
+    if (head > 0) nothing(0, head);
+    if (tail < a.T) nothing(tail, a.T - tail);
   }
 
   // The team's share [t0, t1) of the list: no more teams than give each warp a tile; the first

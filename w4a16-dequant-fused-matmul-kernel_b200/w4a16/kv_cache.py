@@ -300,7 +300,8 @@ def kv4_attention(q: Tensor, cache: KV4Cache, layer: int, block_table: Tensor, k
         kv_lens: int32 [sequences]: cached tokens, the new ones (already appended) included. 0: an unused
             place in the batch, whose queries give zeros.
         cu_q: int32 [sequences + 1]: the first query of each sequence; None: T / sequences each. A sequence's
-            last query stands at position kv_lens - 1; each sees the tokens up to its own position.
+            last query stands at position kv_lens - 1; each sees the tokens up to its own position. Queries before
+            cu_q[0] and from cu_q[-1] on (padding) give zeros.
         max_q: the most queries a sequence has (with cu_q; default T).
         scale: of the scores; default 1 / sqrt(D).
         window: only the last ``window`` tokens up to a query's position; 0: all.
