@@ -91,3 +91,38 @@ def test_more_sequences_than_one_launch_takes():
         part, part_lse = kv4_attention(q[a:b], pages, 0, table[lo:lo + 1250], kv_lens[lo:lo + 1250],
                                        cu_q=cu[lo:lo + 1251] - a, max_q=3, return_lse=True)
         assert torch.equal(o[a:b], part) and torch.equal(lse[a:b], part_lse), lo
+
+
+def test_ragged_calls_leave_nothing_behind():
+    """The workspace does not depend on a call's sizes, and nothing is kept for each of them."""
+    c, cache, q, _ = case([70, 40, 9, 30], [40, 40, 9, 30], 8, 2, 64, 64, F16)
+
+    def kept():
+        return sum(len(v) for v in vars(cache).values() if isinstance(v, dict))
+
+    def call(new):
+        cu = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+        kv4_attention(q[:sum(new)], cache, 0, c.table, c.kv_lens, cu_q=cu, max_q=max(new))
+
+    call([1, 1, 1, 1])
+    before, memory = kept(), None
+    for i in range(1, 40):
+        call([i, 1 + i % 7, 1, 1 + i % 3])
+        torch.cuda.synchronize()
+        memory = torch.cuda.memory_allocated() if memory is None else memory
+        assert torch.cuda.memory_allocated() <= memory + 1024
+    assert kept() == before
+
+
+def test_a_larger_cache_on_the_same_stream():
+    """The stream's workspace is replaced by a larger one between two calls of the smaller cache."""
+    small, large = case([20000, 100], [1, 1], 8, 2, 64, 64, F16, 1), case([30000] + [200] * 79, [1] * 80, 32, 2, 128, 64, F16, 2)
+    want = [kv4_attention(q, cache, 0, c.table, c.kv_lens, **kw) for c, cache, q, kw in (small, large)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for i in (0, 1, 0, 1):
+            c, cache, q, kw = (small, large)[i]
+            o, lse = kv4_attention(q, cache, 0, c.table, c.kv_lens, **kw)
+            side.synchronize()
+            assert torch.equal(o, want[i][0]) and torch.equal(lse, want[i][1])

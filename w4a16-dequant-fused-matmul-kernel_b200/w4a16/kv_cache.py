@@ -71,12 +71,25 @@ class KV4Cache:
         self._struct = _lib.KV4CacheStruct(pool.data_ptr(), num_layers, num_pages, num_kv_heads, head_dim, page_size,
                                            group_size)
         self._ref = ctypes.byref(self._struct)
-        self._ws_sizes: dict[tuple, int] = {}
+        self._ws_bytes = 0
 
     @staticmethod
     def bytes_per_page(head_dim: int, page_size: int, group_size: int) -> int:
         """Bytes of a page of one layer and kv head."""
         return page_size * (head_dim + 8 * (head_dim // group_size))
+
+    def _workspace_bytes(self) -> int:
+        """What any attention over this cache needs: the largest it can be depends on the cache and the device only,
+        and is reached with one warp to a team (many sequences), in the shapes of 8 and of 16 query rows."""
+        if self._ws_bytes == 0:
+            size = ctypes.c_int64(0)
+            with torch.cuda.device(self._index):
+                for heads in (1, 16):
+                    _lib.check(_lib.lib().w4a16_kv4_attention_workspace_size(
+                        self._ref, 1 << 16, heads * self.num_kv_heads, 1 << 16, 1, ctypes.byref(size)),
+                        "w4a16_kv4_attention_workspace_size")
+                    self._ws_bytes = max(self._ws_bytes, size.value)
+        return self._ws_bytes
 
     def _check_layer(self, layer: int) -> None:
         assert 0 <= layer < self.num_layers, f"layer={layer} out of range for {self.num_layers} layers"
@@ -334,19 +347,11 @@ def kv4_attention(q: Tensor, cache: KV4Cache, layer: int, block_table: Tensor, k
         assert max_q >= 0, f"max_q={max_q} must not be negative"
     o = torch.empty_like(q, memory_format=_CONTIGUOUS) if out is None else _out_like(q, out)
     lse = q.new_empty((T, H), dtype=_F32) if return_lse else None
-    key = (T, H, B, max_q)
-    need = cache._ws_sizes.get(key)
-    if need is None:
-        size = ctypes.c_int64(0)
-        with torch.cuda.device(d):
-            _lib.check(_lib.lib().w4a16_kv4_attention_workspace_size(cache._ref, T, H, B, max_q, ctypes.byref(size)),
-                       "w4a16_kv4_attention_workspace_size")
-        need = cache._ws_sizes[key] = size.value
-    ws = _lib.kv4_workspace(need, d, _raw_stream(d)) if need else None
+    ws = _lib.kv4_workspace(cache._ws_bytes or cache._workspace_bytes(), d, _raw_stream(d))
     _on(d, _lib.lib().w4a16_kv4_attention, q.data_ptr(), _CODES[dt], T, H, qt, qs, cache._ref, layer,
         block_table.data_ptr(), width, kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), B, max_q,
         D ** -0.5 if scale is None else scale, min(window, _INT_MAX), o.data_ptr(), None if lse is None else lse.data_ptr(),
-        None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
+        ws.data_ptr(), ws.numel())
     return (o, lse) if return_lse else o
 
 
