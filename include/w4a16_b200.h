@@ -520,7 +520,8 @@ int w4a16_kv4_copy_pages(const w4a16_kv4_cache* cache, const int32_t* src, const
 
 /* Row rows[i] gets free pages (the lowest ids, in the order of the requests) up to lens[i] tokens, and
  * kv_lens[rows[i]] = lens[i]. ok[i] = 1; 0, with the row unchanged, where the free pages do not reach
- * that far down the list, the table is too narrow or lens[i] is less than the row holds. No row twice.
+ * that far down the list, the table is too narrow or lens[i] is less than the row holds. Pages that a row
+ * has beyond its length (kv_lens was lowered) are used before free ones. No row twice.
  * scratch: n + 1 ints. */
 int w4a16_kv4_reserve(const w4a16_kv4_tables* tables, const int32_t* rows, const int32_t* lens, int64_t n, int32_t* ok,
                       int32_t* scratch, void* stream);

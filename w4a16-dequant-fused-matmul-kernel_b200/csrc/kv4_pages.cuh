@@ -124,7 +124,8 @@ __device__ __forceinline__ void lowest_free(const int* refs, int pages, int need
 
 // Growth: row rows[i] gets pages up to lens[i] tokens. ok[i] = 1 where it has them (its kv_lens
 // is then lens[i]); 0, and nothing changed, where the free pages before it in the order of the
-// request do not reach, the table is too narrow, or lens[i] is less than it has.
+// request do not reach, the table is too narrow, or lens[i] is less than it has. Pages that the row
+// has beyond its length (which was lowered) are used before free ones.
 struct ReserveParams {
   Tables t;
   const int *req_rows, *req_lens;
@@ -148,7 +149,12 @@ __global__ void __launch_bounds__(SCAN_THREADS) kv4_reserve_kernel(const Reserve
         const int want = len / t.page_size + (len % t.page_size != 0);
         if (have >= 0 && len >= have && want <= t.width) {
           good = 1;
-          need = want - (have / t.page_size + (have % t.page_size != 0));
+          int held = have / t.page_size + (have % t.page_size != 0);
+          for (; held < want; ++held) {
+            const int page = t.table[static_cast<long long>(r) * t.width + held];
+            if (page < 0 || page >= t.pages || t.refs[page] <= 0) break;
+          }
+          need = want - held;
         }
       }
     }
@@ -177,8 +183,8 @@ __global__ void __launch_bounds__(SCAN_THREADS) kv4_reserve_kernel(const Reserve
       if (p.start[mid] <= j) lo = mid; else hi = mid - 1;
     }
     if (p.start[lo + 1] > got) return;   // refused
-    const int r = p.req_rows[lo], have = t.lens[r];
-    const int col = have / t.page_size + (have % t.page_size != 0) + j - p.start[lo];
+    const int r = p.req_rows[lo], len = p.req_lens[lo];
+    const int col = len / t.page_size + (len % t.page_size != 0) - p.ok[lo] + j - p.start[lo];
     t.table[static_cast<long long>(r) * t.width + col] = id;
     t.refs[id] = 1;
   });

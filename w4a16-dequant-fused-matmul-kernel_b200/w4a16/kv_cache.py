@@ -98,7 +98,9 @@ class KV4Cache:
 class KV4Pages:
     """Which sequence (row) holds which pages: ``refs`` int32 ``[num_pages]`` (rows that hold a page;
     0: free), ``block_table`` int32 ``[rows, pages per row]`` (-1: none), ``kv_lens`` int32 ``[rows]``.
-    :meth:`empty` makes the tables of a pool nobody uses yet. The tensors may be written to, not replaced."""
+    :meth:`empty` makes the tables of a pool nobody uses yet. The tensors may be written to, not replaced. An entry of
+    ``kv_lens`` may be lowered (rejected drafts): the row keeps its pages, and grows into them first. Not below what
+    it shares with other rows, though: new tokens would be written into their page."""
 
     def __init__(self, refs: Tensor, block_table: Tensor, kv_lens: Tensor, page_size: int) -> None:
         for name, t, dim in (("refs", refs, 1), ("block_table", block_table, 2), ("kv_lens", kv_lens, 1)):
@@ -406,7 +408,8 @@ def kv4_reserve(pages: KV4Pages, rows: Tensor, lens: Tensor) -> Tensor:
     """Let row ``rows[i]`` hold ``lens[i]`` tokens (int32 [n] each, no row twice): it gets the free pages with the
     lowest ids, in the order of the requests, and its ``kv_lens`` becomes ``lens[i]``. Returns int32 [n]: 1, or
     0 (row unchanged) where the free pages do not reach that far down the list, the table is too narrow, or
-    the row holds more than ``lens[i]`` already. Changes ``pages`` in place."""
+    the row holds more than ``lens[i]`` already. Pages that a row has beyond its length (its ``kv_lens`` was lowered)
+    are used before free ones. Changes ``pages`` in place."""
     d = pages._index
     n = rows.shape[0] if rows.dim() == 1 else -1
     _ints("rows", rows, n, d)
