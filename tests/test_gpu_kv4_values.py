@@ -182,3 +182,19 @@ def test_groups_without_spread(D, group, new, share):
         assert (o[:, 4, :, :64] == 0).all()
     for head in (1, 2):                             # a mean of one number: fp32's and the output's roundings
         assert ((o[:, head] - vd[0, head, 0]).abs() <= (2.0 ** -11 + 1e-5) * vd[0, head, 0]).all()
+
+
+@pytest.mark.parametrize("token", [3, 40, 66])
+@pytest.mark.parametrize("new,share", [(1, 4), (2, 6), (70, 8)])
+def test_a_nan_of_vanishing_weight_is_still_one(token, new, share):
+    """The weight 2^-350 of a NaN value is zero in fp32, in a whole tile as in one that the sequence ends in."""
+    n, KV, D = 70, 16, 64
+    g = gen(token)
+    k = torch.randn((n, KV, D), generator=g, device="cuda").half()
+    v = torch.randn((n, KV, D), generator=g, device="cuda").half()
+    k[token], v[token] = -10, float("nan")
+    cache, table, lens, _, _ = appended(k, v, 64)
+    q = torch.full((new, KV * share, D), 3.0, device="cuda", dtype=F16)
+    o = kv4_attention(q, cache, 0, table, lens)
+    sees = torch.arange(n - new, n, device="cuda") >= token
+    assert o[sees].isnan().all() and o[~sees].isfinite().all()

@@ -689,7 +689,8 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            y[k][nt][c] = ex2(y[k][nt][c]);
+            // (minus zero: not seen. The weight of a token that is seen may vanish, but a NaN of it does not)
+            y[k][nt][c] = EDGE && y[k][nt][c] == -INFINITY ? -0.0f : ex2(y[k][nt][c]);
             l[nt][c & 1] += y[k][nt][c];
           }
 #pragma unroll
@@ -705,8 +706,9 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
                 const float pv = y[k][nt][c];
-                ps[c] = pv == 0.0f ? 0.0f : pv * (c < 2 ? sv0 : sv1);
-                if (pv != 0.0f) corr[nt][c & 1][gr] = fmaf(pv, c < 2 ? o0 : o1, corr[nt][c & 1][gr]);
+                const bool seen = __float_as_uint(pv) != 0x80000000u;
+                ps[c] = seen ? pv * (c < 2 ? sv0 : sv1) : 0.0f;
+                if (seen) corr[nt][c & 1][gr] = fmaf(pv, c < 2 ? o0 : o1, corr[nt][c & 1][gr]);
               }
             } else {
 #pragma unroll
