@@ -290,13 +290,15 @@ _ws_for: dict[tuple[int, int, int, int, int, int], tuple[int | None, int]] = {}
 
 
 def workspace_for(M: int, N: int, K: int, G: int, device_index: int, stream: int) -> tuple[int | None, int]:
-    """(pointer, bytes) of the zeroed workspace a GEMM of this shape uses on ``stream``
-    of device ``device_index``; (None, 0) when the shape needs none. Memoised outside graph
+    """(pointer, bytes) of the zeroed workspace a GEMM of this shape uses on ``stream``,
+    the current stream of the current device ``device_index``; (None, 0) when the shape needs none. Memoised outside graph
     captures: a hit is one dictionary lookup (the buffer it names is kept alive by the cache below)."""
     key = (M, N, K, G, device_index, stream)
-    captures = _captures(device_index, stream)
-    hit = None if captures else _ws_for.get(key)
-    if hit is not None:
+    hit = _ws_for.get(key)
+    if hit is not None and hit[0] is None:
+        return hit
+    captures = _current_captures()
+    if hit is not None and not captures:
         return hit
     dev = torch.device("cuda", device_index)
     nbytes = gemm_workspace_bytes(M, N, K, G, dev) if M > 0 and N > 0 else 0
