@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
   uint64_t* bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(seqs + MAX_SEQS) + 15) & ~static_cast<uintptr_t>(15));
   unsigned long long* scan = reinterpret_cast<unsigned long long*>(bars + 2 * W);
   int* flags = reinterpret_cast<int*>(scan);             // two per team, then each warp's stage with its sums
+  int* ends = flags + 3 * W;                             // cu_q's ends
 
   const AttendParams& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -211,6 +212,8 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
     unsigned long long v = 0;
     if (b < a.seqs) {
       sequence(a, b, q.first, q.count, q.len);
+      if (a.cu_q && b == 0) ends[0] = a.cu_q[0];
+      if (a.cu_q && b == a.seqs - 1) ends[1] = a.cu_q[a.seqs];
       if (static_cast<long long>(q.count) * a.share > p.row_limit) q.count = 0;
       const int n = tiles_of(q.count, q.len);
       if (n) {
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_decode_kernel(const DecodeParam
 
   // queries of no sequence
   if (a.cu_q) {
-    const int head = p.before ? min(max(a.cu_q[0], 0), a.T) : 0, tail = p.after ? max(a.cu_q[a.seqs], head) : a.T;
+    const int head = p.before ? min(max(ends[0], 0), a.T) : 0, tail = p.after ? max(ends[1], head) : a.T;
     const long long step = static_cast<long long>(gridDim.x) * W * 32, at = blockIdx.x * W * 32LL + threadIdx.x;
     auto nothing = [&](long long first, long long rows) {
       uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + first * a.heads * D);
