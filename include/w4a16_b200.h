@@ -71,7 +71,8 @@ const char* w4a16_strerror(int status);
  * the tensor-memory-operand prefill kernel, when it splits K, keeps arrival
  * counters (left zero) and fp32 partial tiles past that offset. So one zeroed
  * buffer serves every later call on the same stream, whatever the shape;
- * launches that may run concurrently need separate workspaces. A prefill call
+ * launches that may run concurrently need separate workspaces, and a graph
+ * capture needs one of its own, zeroed inside the graph. A prefill call
  * given less workspace than the query returned runs without splitting K. (A
  * launch abandoned on W4A16_ERR_TIMEOUT can leave words set: zero the buffer
  * again before reusing it.) May be NULL when the size query returned 0.

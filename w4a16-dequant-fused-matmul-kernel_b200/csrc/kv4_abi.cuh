@@ -267,8 +267,10 @@ int launch_decode(const w4a16_kv4_cache& c, const AttendParams& all, const Atten
 // once per 8 or 16 rows and splits it over all SMs. Up to kDecodeRows rows the decode kernel takes the
 // sequence, and every sequence of a batch of at most kDecodeWork rows x kv heads x sequences. Measured, 32
 // heads of 128 channels on 8 kv heads (decode kernel against the other, us): one sequence of 8192 tokens, 128
-// rows: 35, 139; 1024 rows: 161, 184; 1536 rows: 232, 184; of 1500 tokens, 512 rows: 27, 51; 1024: 44, 51;
-// 1536: 78, 52; 16 sequences of 8192, 64 rows: 161, 188; 96: 236, 189.
+// rows: 34, 138; 1024 rows: 166, 188; 1536 rows: 243, 188; of 1500 tokens, 512 rows: 26, 50; 1024: 43, 49;
+// 1536: 78, 50; 16 sequences of 8192, 64 rows: 167, 141; 96: 244, 141 (with many segments the crossing lies
+// somewhat below 64). In two groups per head, one of 8192, 512 rows: 102, 234; 1024: 197, 236; 1536: 315, 235;
+// with heads of 64, 512: 61, 167; 1024: 116, 168; 1536: 166, 168.
 constexpr long long kDecodeRows = 64, kDecodeWork = 8192;
 
 long long decode_rows(const AttendPlan& plan) {

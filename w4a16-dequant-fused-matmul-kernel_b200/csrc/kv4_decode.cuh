@@ -31,19 +31,19 @@
 //
 // Work: a segment is a kv head of a sequence (and a tile of 8 NT of its rows), a tile TB blocks
 // of 16 tokens. All tiles form one list that N teams of warps split evenly, whatever the lengths
-// (a segment counts `seg_cost` tiles more than it has, for its queries and its epilogue); a team that holds a part of a segment leaves (m, l, o) in the workspace and, when all its
-// tiles are done, the last of the segment's teams to arrive joins the parts in team order, so
-// results do not depend on timing. (Where there are teams enough and no segment is much longer than the
-// others, each team takes one whole segment.) Each warp
-// feeds itself: two stages of a tile, filled by copies
-// that its own lane 0 issues. A piece's end passes through shared memory once: each warp leaves its
-// sums in the stage it has just read, and each then adds up some rows over all warps.
+// (a segment counts `seg_cost` tiles more than it has, for its queries and its epilogue); a team that holds a
+// part of a segment leaves (m, l, o) in the workspace and, when all its tiles are done, the last of the segment's
+// teams to arrive joins the parts in team order, so results do not depend on timing. (Where there are teams enough
+// and no segment is much longer than the others, each team takes one whole segment.) Each warp feeds itself: two
+// stages of a tile, filled by copies that its own lane 0 issues. A piece's end passes through shared memory once:
+// each warp leaves its sums in the stage it has just read, and each then adds up some rows over all warps.
 //
-// Two sequences of 131071 and 107000 tokens, 32 heads of 128 channels in groups of 64 on 8 kv heads (274 MB): 74 us;
-// 61 of up to 8000 tokens, 64 heads on 8 (298 MB): 79 us. Of the 74 us, 51 are the tile loop (5.4 TB/s, 84%
-// of a plain copy's rate); 3 go by until the first copy is issued (lengths, prefix sums, the table), 4 at a
-// piece's end and 5 in joining parts, which is what bounds short batches: 12.4 us for one sequence of 777
-// tokens.
+// Two sequences of 131071 and 107000 tokens, 32 heads of 128 channels in groups of 64 on 8 kv heads (274 MB): 74.5 us,
+// 3.7 TB/s; 61 of up to 8000 tokens, 64 heads on 8 (298 MB): 80 us, 3.7 TB/s; one of 777 tokens: 12.1 us. By the
+// batch's counters no unit is full: 54% of the issue slots, 54% of the ALU pipe (masking codes, packing), 22% of
+// the tensor pipe, with four warps to a scheduler (128 registers), which mostly wait for an instruction before theirs.
+// Timed inside the kernel, when the long case took 74 us: 51 in the tile loop (5.4 TB/s), 3 until the first copy is
+// issued (lengths, prefix sums, the table), 4 at a piece's end, 5 in joining parts; the other 11 have no name yet.
 #pragma once
 
 #include <type_traits>
@@ -131,9 +131,9 @@ struct Sequence {
 // A team takes one whole segment each, and nothing is joined, where there are teams enough and no segment
 // has many more tiles per warp than the warps' average share: kWholeTiles + 0.9 x the share more, at most
 // kWholeMost. Joining costs what four tiles of a warp alone take, and more where the memory is busy. Measured
-// (whole, split; us): 24 sequences with a window of 1024, 5 rows, 16 kv heads of 64: 20.7, 24.8; 48 of 777, 20
-// rows, 8 kv heads of 128: 51, 84; 16 of 6000, 4 rows: 33, 41; one of 6000: 29, 18.5; 24 of 6000 on one kv head: 31,
-// 20.7; 48 of 3000, 16 kv heads of 64: 69, 58.
+// (whole, split; us): 24 sequences with a window of 1024, 5 rows, 16 kv heads of 64: 19.7, 24.6; 48 of 777, 20
+// rows, 8 kv heads of 128: 50, 90; 16 of 6000, 4 rows: 32, 41; one of 6000: 30, 16.7; 24 of 6000 on one kv head: 30,
+// 19.5; 48 of 3000, 16 kv heads of 64: 66, 57; one of 777: 11.8, 14.4.
 constexpr float kWholeTiles = 4.0f, kWholeMost = 9.0f;
 
 struct Segment {

@@ -17,12 +17,12 @@
 // run in order). With one buffer of 128 tokens softmax and products took turns: 3700 and 3500 cycles
 // per 128 tokens.
 //
-// Three prompts of up to 4096 tokens over up to 8192, 32 heads of 128 channels on 8 kv heads: 1.14 ms, 0.82
-// PFLOP/s, 49% of what a plain bf16 matrix product reaches. A step of 64 tokens takes 2500 cycles, its
-// products 1000 of them: what bounds it is the softmax warps' instructions (1950 cycles a step, two
-// warps to an SM quarter, 128 registers) with the cache warps' in the same issue slots; without
-// exponentials, key pairs and expansion the same schedule takes 0.76 ms. Four softmax warps to a quarter
-// of 80 registers each (even and odd steps by different threads) took 1.28 ms.
+// Three prompts of up to 4096 tokens over up to 8192, 32 heads of 128 channels on 8 kv heads: 1.18 ms, 0.79
+// PFLOP/s, 47% of what a plain bf16 matrix product reaches; in two groups per head 1.46 ms, with heads of 64 1.04 ms.
+// A step of 64 tokens takes 2600 cycles, its products 1000 of them: what bounds it is the softmax warps'
+// instructions (traced at 2500: 1950 cycles a step, two warps to an SM quarter, 128 registers) with the cache
+// warps' in the same issue slots; without exponentials, key pairs and expansion the schedule took 0.76 ms of then
+// 1.14. Four softmax warps to a quarter of 80 registers each (even and odd steps by different threads) took 1.28 ms.
 //
 // As in the decode kernel the tensor cores see a key's codes, and its scale and offset act on its
 // scores in fp32, so the scores carry no rounding of keys (values rounded to fp16 first move a

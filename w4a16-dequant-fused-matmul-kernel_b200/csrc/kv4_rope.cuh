@@ -21,11 +21,11 @@
 // computed from a head's or group's statistics is computed by few lanes for all of them (reduce_scatter).
 // A group's heads are of one kind, with one base address; pairs of fp32 go through one instruction.
 //
-// 4096 tokens of 32 + 8 heads of 128 fp16 channels (86 MB in and out): 16.6 us, 5.2 TB/s, 81% of a plain
-// copy's rate. 8192 tokens of 64 + 8 heads of bf16 with their values into the cache (8 kv heads):
-// 74 us, 3.8 TB/s; there the issue slots are two thirds full (40% of the ALU pipe with conversions
+// 4096 tokens of 32 + 8 heads of 128 fp16 channels (86 MB in and out): 17 us, 5.1 TB/s, 79% of a plain
+// copy's rate. 8192 tokens of 64 + 8 heads of bf16 with their values into the cache (8 kv heads; 316 MB):
+// 73 us, 4.3 TB/s; there 71% of the issue slots are full (54% of the ALU pipe with conversions
 // of 16-bit pairs, minima and code packing), and blocks of 128 threads at 64 registers took 6% less time than
-// blocks of 256 (the same occupancy, given back sooner).
+// blocks of 256 (the same occupancy, given back sooner). Reading 8192 tokens of 8 heads back: 10.4 us, 4.1 TB/s.
 #pragma once
 
 #include "kv4_common.cuh"
