@@ -28,6 +28,7 @@ _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _lib.stream_of_index)
 _CONTIGUOUS = torch.contiguous_format
 _INT_MAX = 2 ** 31 - 1
+_largest_workspace: dict[tuple[int, int, int], int] = {}
 
 
 class KV4Cache:
@@ -79,16 +80,19 @@ class KV4Cache:
         return page_size * (head_dim + 8 * (head_dim // group_size))
 
     def _workspace_bytes(self) -> int:
-        """What any attention over this cache needs: the largest it can be depends on the cache and the device only,
-        and is reached with one warp to a team (many sequences), in the shapes of 8 and of 16 query rows."""
-        if self._ws_bytes == 0:
-            size = ctypes.c_int64(0)
+        """What any attention over this cache needs: the largest it can be depends on the head's layout and the device
+        only, and is reached with one warp to a team (many sequences), in the shapes of 8 and of 16 query rows."""
+        key = (self._index, self.head_dim, self.group_size)
+        if key not in _largest_workspace:
+            size, most = ctypes.c_int64(0), 0
             with torch.cuda.device(self._index):
                 for heads in (1, 16):
                     _lib.check(_lib.lib().w4a16_kv4_attention_workspace_size(
                         self._ref, 1 << 16, heads * self.num_kv_heads, 1 << 16, 1, ctypes.byref(size)),
                         "w4a16_kv4_attention_workspace_size")
-                    self._ws_bytes = max(self._ws_bytes, size.value)
+                    most = max(most, size.value)
+            _largest_workspace[key] = most
+        self._ws_bytes = _largest_workspace[key]
         return self._ws_bytes
 
     def _check_layer(self, layer: int) -> None:
