@@ -240,9 +240,11 @@ __global__ void __launch_bounds__(THREADS, 4) verify_kernel(const VerifyParams p
   }
 
   // ---- the warp whose range holds the border, else the last one with anything
-  // (a number below 0, or none, counts as 0)
-  const double border = fmax(uniforms[p.drafts] * total, 0.0);
-  const unsigned over0 = __ballot_sync(0xffffffffu, prefix[0] > border), over1 = __ballot_sync(0xffffffffu, prefix[1] > border);
+  // (a number below 0, or none, counts as 0; one of 1 or more lies behind every sum. Prefix sums of neighbours are
+  // rounded apart, so that a range that holds nothing can seem to exceed the border first: it is passed over.)
+  const double border = uniforms[p.drafts] >= 1.0f ? INFINITY : fmax(uniforms[p.drafts] * total, 0.0);
+  const unsigned over0 = __ballot_sync(0xffffffffu, prefix[0] > border && sum[0] > 0.0);
+  const unsigned over1 = __ballot_sync(0xffffffffu, prefix[1] > border && sum[1] > 0.0);
   const unsigned any0 = __ballot_sync(0xffffffffu, sum[0] > 0.0), any1 = __ballot_sync(0xffffffffu, sum[1] > 0.0);
   const int owner = over0 ? __ffs(over0) - 1 : over1 ? 31 + __ffs(over1) : any1 ? 63 - __clz(any1) : any0 ? 31 - __clz(any0) : 0;
   if (owner != static_cast<int>(me)) {
@@ -251,8 +253,8 @@ __global__ void __launch_bounds__(THREADS, 4) verify_kernel(const VerifyParams p
   }
   long long found = -1;
   if (total > 0.0) {
-    // what lies before the range, which does not exceed the border (and so on, down to the row of 32: whatever
-    // exceeds it holds something)
+    // what lies before the range; then the first quarter that exceeds the border, the last one where rounding says
+    // that none does
     double before = __shfl_sync(0xffffffffu, owner <= 32 ? prefix[0] : prefix[1], (owner - 1) & 31);
     if (owner == 0) before = 0.0;
     int k = 0;
