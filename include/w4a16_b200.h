@@ -593,9 +593,9 @@ int w4a16_kv4_compact(const w4a16_kv4_cache* cache, const w4a16_kv4_tables* in, 
  * the last axis contiguous, strides in elements; tokens [seqs, drafts]; uniforms [seqs, drafts + 1] in [0, 1);
  * counts [seqs] or null: how many of its drafts a sequence has. Draft i is accepted while uniforms[i] * q < p. out
  * [seqs, drafts + 1]: the a accepted ones, the token drawn behind them, -1 from there on; accepted [seqs]: a. The
- * token is the first v at which the running sum of r exceeds uniforms[drafts] times its whole, in fp64: r =
- * max(target[a] - draft[a], 0), or target[a] where all drafts were accepted or r is nothing; -1 where that is nothing
- * too. Differences that are not finite count as nothing. kv_lens (or null): entry rows[b] of n_lens (b where rows is
+ * token is the first v at which the running sum of r (within 2^-45 + vocab 2^-64 of the whole) exceeds uniforms[drafts]
+ * times its whole: r = max(target[a] - draft[a], 0), or target[a] where all drafts were accepted or r is nothing;
+ * -1 where that is nothing too. Differences that are not finite count as nothing. kv_lens (or null): entry rows[b] of n_lens (b where rows is
  * null) is lowered by the sequence's rejected drafts. A token, count or row out of range raises the index flag: the
  * draft is rejected, the count cut to 0..drafts, the length left as it is.
  */

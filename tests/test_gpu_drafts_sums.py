@@ -1,5 +1,5 @@
 """The draw of verify_drafts where the running sums come near the border: ranges that hold nothing, numbers at the end of
-their range."""
+their range, and sums of many values of very different sizes."""
 from __future__ import annotations
 
 from fractions import Fraction
@@ -63,3 +63,47 @@ def test_numbers_beyond_the_range_take_the_last_token(V):
     for u in (1.0, 1.5, float("inf")):
         out, _ = verify_drafts(target[:, None], None, torch.empty((400, 0), dtype=torch.int64, device="cuda"), torch.full((400, 1), u, device="cuda"))
         assert out[:, 0].tolist() == last.tolist()
+
+
+def mirrored(V, seed, sharp):
+    """Values that read the same from both ends, and what the first half has more than the second: nothing yet."""
+    rng = np.random.default_rng(seed)
+    half = np.exp(rng.normal(size=V // 2) * sharp).astype(np.float32)
+    half /= 2 * half.sum(dtype=np.float64)
+    half[0], half[-1] = 0.0, 2.0 ** -20
+    return np.concatenate([half, half[::-1]])
+
+
+# The kernel's sums are within 2^-45 of themselves and 2^-53 more for each fp64 addition of a thread, 1024 of them here: within
+# 2^-42.7 of the whole together. A half that has 2^-41 of the whole more than the other moves the edge by 2^-42 from where half
+# of the whole lies, so the token is decided, whatever the order of the sums.
+MORE = 2.0 ** -41
+
+
+@pytest.mark.parametrize("batch", [1, 40, 300])
+@pytest.mark.parametrize("V", [20000, 1 << 17, (1 << 17) + 2, 1 << 22])
+def test_the_token_does_not_depend_on_the_batch(V, batch):
+    for seed in range(8):
+        row = mirrored(V, seed, sharp=1.0 + seed)
+        assert drawn(row + np.float32(MORE) * (np.arange(V) == 0), 0.5, batch) == V // 2 - 1, seed
+        assert drawn(row + np.float32(MORE) * (np.arange(V) == V - 1), 0.5, batch) == V // 2, seed
+
+
+@pytest.mark.parametrize("batch", [1, 40, 300])
+@pytest.mark.parametrize("V", [20000, 1 << 17, (1 << 17) + 2, 1 << 22])
+def test_the_token_does_not_depend_on_the_batch_with_a_draft(V, batch):
+    """The same for what a target has over a draft."""
+    for seed in range(8):
+        p = mirrored(V, seed, sharp=1.0 + seed)
+        part = np.random.default_rng(100 + seed).random(V // 2, dtype=np.float32)
+        q = p * np.concatenate([part, part[::-1]])
+        q[V // 2 - 1:V // 2 + 1] = 0.0
+        q[[5, V - 6]] = 4 * p[[5, V - 6]]                 # token 5 is not accepted
+        whole = (p.astype(np.float64) - np.minimum(p, q)).sum()
+        assert whole > 0.2                                # (so MORE is no less of it)
+        for at, want in ((0, V // 2 - 1), (V - 1, V // 2)):
+            target = torch.from_numpy(p + np.float32(MORE) * (np.arange(V) == at)).cuda()
+            draft = torch.from_numpy(q).cuda()
+            out, accepted = verify_drafts(target.expand(batch, 2, V), draft.expand(batch, 1, V), torch.full((batch, 1), 5, device="cuda"),
+                                          torch.tensor([[0.9, 0.5]], device="cuda").expand(batch, 2).contiguous())
+            assert (accepted == 0).all() and (out[:, 0] == want).all(), (seed, out[:, 0])

@@ -5,10 +5,11 @@
 // place a, is drawn by the last random number u from r = max(p_a - q_a, 0), or from p_a where no
 // draft is left (or r is nothing): the first v with r_0 + ... + r_v > u (r_0 + r_1 + ...).
 //
-// What a probability decides is decided with 64 bits' worth: u q is exact in fp64, p - q is exact, and the sums
-// are pairs of fp32 numbers within a thread and fp64 beyond, so the token does not depend on how the sum is
-// split (a fp32 sum of 10^5 probabilities would move a border by more than many of them are wide). Values whose
-// difference is not finite count as nothing, and so do negative ones.
+// u q is exact in fp64, and so is p - q. The sums are fp64 of four values each (two, where rows lie at any
+// place beside a draft) that are summed to 2^-45 of themselves; a thread adds V / 2048 such numbers at most, each addition
+// rounded to 2^-53. So a border between two tokens is off by less than 2^-45 + V 2^-64 of the whole, however the sum
+// is split (a fp32 sum of 10^5 probabilities would move it by more than many of them are wide). Values
+// whose difference is not finite count as nothing, and so do negative ones.
 //
 // Memory-bound: of a sequence's rows one pair is read whole, after two dependent reads (the drafted
 // tokens, then their probabilities) that say which. A cluster of up to eight blocks takes a sequence;
@@ -16,9 +17,11 @@
 // the cluster, and the one warp whose range the border falls into looks at the quarter once more, sixteen values to
 // a lane, so that one prefix sum finds the lane.
 //
-// 64 sequences of up to 7 drafts, 131072 values, fp32: 67 MB in 20 us, half of the copy rate; one sequence of 32000
-// values 7.4 us; 201 sequences of 50001 values, whose rows begin at any multiple of 4 bytes, 28 us. No unit is full
-// (issue 31%): it is the chain of four dependent reads, two joins in the cluster and the second look.
+// 64 sequences of up to 7 drafts, 131072 values, fp32: 20.3 us, in which 48 MB are read (a sequence whose drafts all
+// stand reads one row): 2.4 TB/s, 36% of the copy rate. One sequence of 32000 values 7.4 us. 201 sequences of 50001
+// values, whose rows begin at any multiple of 4 bytes: 18.5 us for looked-up drafts, 26 us beside a draft. No
+// unit is full (issue 31%): it is the latency of a chain of four dependent reads, two joins in the cluster and
+// the second look.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -63,27 +66,45 @@ __device__ __forceinline__ void load4(const T* at, float (&v)[4]) {
   for (int i = 0; i < 4; ++i) v[i] = as_f32(x[i]);
 }
 
-// A sum in two fp32 numbers, the second what the first rounded away (Knuth's two-sum, Dekker's for the difference): 47
-// bits or more, at a dozen fp32 instructions a value where fp64 additions and the conversions before them took eight
-// times the time (64 sequences, 131072 values: 87 us). Infinities and NaN show in the sum.
-struct Pair {
-  float high, low;
-  template <bool MINUS>
-  __device__ __forceinline__ void add(float pv, float qv) {
-    float d, e = 0.0f;
+// What two fp32 numbers' sum is rounded to, and by how much (Knuth's two-sum).
+__device__ __forceinline__ float two_sum(float a, float b, float& rest) {
+  const float t = __fadd_rn(a, b), x = __fsub_rn(t, a);
+  rest = __fadd_rn(__fsub_rn(a, __fsub_rn(t, x)), __fsub_rn(b, x));
+  return t;
+}
+
+// The sum of N values, or of what they have over as many others, added to an fp64 number. The N are added in fp32 with
+// what is rounded off kept (Dekker's rest for a difference: exact where neither number is negative), which leaves
+// an error of 2^-45 of their sum at most: 8 roundings, each 2^-24 of a rest of 2^-24. fp64 from the first value on
+// costs one or two conversions a value where this costs two for N values: the kernel took 87 us for 64 sequences
+// of 131072. Infinities and NaN show in the sum.
+template <bool MINUS, int N>
+__device__ __forceinline__ void add_to(double& sum, const float (&p)[N], const float (&q)[N]) {
+  static_assert(N == 2 || N == 4, "");
+  float d[N], e[N] = {};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
     if (MINUS) {
-      qv = fminf(qv, pv);                 // (a difference below zero is none)
-      d = __fsub_rn(pv, qv);
-      e = __fsub_rn(__fsub_rn(pv, d), qv);
+      const float qv = fminf(q[i], p[i]);          // (a difference below zero is none)
+      d[i] = __fsub_rn(p[i], qv);
+      e[i] = __fsub_rn(__fsub_rn(p[i], d[i]), qv);
     } else {
-      d = fmaxf(pv, 0.0f);
+      d[i] = fmaxf(p[i], 0.0f);
     }
-    const float t = __fadd_rn(high, d), b = __fsub_rn(t, high);
-    const float r = __fadd_rn(__fsub_rn(high, __fsub_rn(t, b)), __fsub_rn(d, b));
-    high = t;
-    low = __fadd_rn(low, MINUS ? __fadd_rn(r, e) : r);
   }
-};
+  float high, low;
+  if (N == 2) {
+    high = two_sum(d[0], d[1], low);
+    if (MINUS) low = __fadd_rn(low, __fadd_rn(e[0], e[1]));
+  } else {
+    float r0, r1, r;
+    const float t0 = two_sum(d[0], d[1], r0), t1 = two_sum(d[N - 2], d[N - 1], r1);
+    high = two_sum(t0, t1, r);
+    low = __fadd_rn(__fadd_rn(r0, r1), r);
+    if (MINUS) low = __fadd_rn(low, __fadd_rn(__fadd_rn(e[0], e[1]), __fadd_rn(e[N - 2], e[N - 1])));
+  }
+  sum += static_cast<double>(high) + static_cast<double>(low);
+}
 
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
@@ -169,7 +190,8 @@ __global__ void __launch_bounds__(THREADS, 4) verify_kernel(const VerifyParams p
     // (minus: the pair's other half; without one the loads are of the row alone)
     auto add = [&](auto with) {
       constexpr bool WITH = decltype(with)::value;
-      Pair f[4] = {};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[k] = 0.0;
       if (vectors) {
         const uint32_t steps = ((len + 3) / 4 * 8 + 31) / 32;
 #pragma unroll 1
@@ -181,24 +203,32 @@ __global__ void __launch_bounds__(THREADS, 4) verify_kernel(const VerifyParams p
             float pv[4], qv[4] = {};
             load4(row + v, pv);
             if (WITH) load4(minus + v, qv);
+            if (LOOKUP) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[k].add<WITH>(LOOKUP && v + i == except ? 0.0f : pv[i], qv[i]);
+              for (int i = 0; i < 4; ++i)
+                if (v + i == except) pv[i] = 0.0f;
+            }
+            add_to<WITH>(s[k], pv, qv);
           }
       } else {
         const uint32_t steps = (len + 3) / 4;
         constexpr int UN = WITH ? 2 : 4;
-#pragma unroll UN
-        for (uint32_t j = 0; j < steps; ++j)
+#pragma unroll 1
+        for (uint32_t j = 0; j < steps; j += UN) {
+          float pv[4][UN], qv[4][UN] = {};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t unit = quarter(k) + j, v = unit * 32 + lane;
-            if (unit >= quarter(k + 1) || v >= vocab) continue;
-            const float pv = as_f32(row[v]);
-            f[k].add<WITH>(LOOKUP && v == except ? 0.0f : pv, WITH ? as_f32(minus[v]) : 0.0f);
-          }
+          for (int i = 0; i < UN; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t unit = quarter(k) + j + i, v = unit * 32 + lane;
+              const bool in = unit < quarter(k + 1) && v < vocab;
+              pv[k][i] = in && (!LOOKUP || v != except) ? as_f32(row[v]) : 0.0f;
+              if (WITH) qv[k][i] = in ? as_f32(minus[v]) : 0.0f;
+            }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) add_to<WITH>(s[k], pv[k], qv[k]);
+        }
       }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) s[k] = static_cast<double>(f[k].high) + static_cast<double>(f[k].low);
     };
     if (slow) {                               // infinities, NaN or sums beyond fp32 among the values
 #pragma unroll
