@@ -573,8 +573,8 @@ int w4a16_kv4_release(const w4a16_kv4_tables* in, const w4a16_kv4_tables* out, c
  * = keep. weights, fp32: entry (layer, row, head, token) at the three strides, `capacity` tokens contiguous; the
  * kept tokens' weights go to kept [.., keep), which may be weights. ok[i] = 1; 0, with the row unchanged, where
  * the free pages do not reach that far down the list, where the row was named before, or (index flag) where it is out of
- * range or longer than `capacity`. Writes the tables `out` (which may be `in`). scratch:
- * w4a16_kv4_evict_scratch_ints ints. */
+ * range or longer than `capacity`. n is at most 2^20, and n rows' pages (of `keep` tokens each) at most 2^31 - 1. Writes
+ * the tables `out` (which may be `in`). scratch: w4a16_kv4_evict_scratch_ints ints. */
 int w4a16_kv4_evict(const w4a16_kv4_cache* cache, const w4a16_kv4_tables* in, const w4a16_kv4_tables* out,
                     const float* weights, int64_t w_layer_stride, int64_t w_row_stride, int64_t w_head_stride, float* kept,
                     int64_t k_layer_stride, int64_t k_row_stride, int64_t k_head_stride, int64_t capacity,

@@ -748,7 +748,8 @@ int w4a16_kv4_evict_scratch_ints(const w4a16_kv4_tables* in, int64_t n, int keep
   *ints_out = 0;
   const int st = kv4::check_tables(in);
   if (st != W4A16_OK) return st;
-  if (n < 0 || n > (1 << 20) || keep < 1) return W4A16_ERR_INVALID;
+  // (the device adds up in 32 bits how many pages are asked for)
+  if (n < 0 || n > (1 << 20) || keep < 1 || n * kv4::evict_pages(*in, keep) > 0x7fffffffLL) return W4A16_ERR_INVALID;
   *ints_out = n * (3 + kv4::evict_pages(*in, keep) + in->width) + 1 + in->rows;
   return W4A16_OK;
 }

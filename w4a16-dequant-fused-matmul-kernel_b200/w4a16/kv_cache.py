@@ -599,7 +599,9 @@ def kv4_evict(cache: KV4Cache, pages: KV4Pages, weights: Tensor, rows: Tensor, k
     assert sinks >= 0 and recent >= 0 and 1 <= keep <= _INT_MAX and sinks + recent <= keep, (
         f"keep={keep} must be positive, and hold sinks={sinks} and recent={recent}")
     _, R, W = pages._shape
-    out, buf, at = _tables_out(pages, out, n * (4 + min(-(-keep // cache.page_size), W) + W) + 1 + R)
+    need = min(-(-keep // cache.page_size), W)
+    assert n * need <= _INT_MAX, f"{n} rows of {need} pages are more than one call can ask for"
+    out, buf, at = _tables_out(pages, out, n * (4 + need + W) + 1 + R)
     ws, ks = weights.stride(), kept.stride()
     _on(d, _lib.lib().w4a16_kv4_evict, cache._ref, pages._ref, out._ref, weights.data_ptr(), ws[0], ws[1], ws[2],
         kept.data_ptr(), ks[0], ks[1], ks[2], weights.shape[3], rows.data_ptr(), n, keep, sinks, recent, at, at and at + 4 * n)
