@@ -527,8 +527,8 @@ int w4a16_kv4_attention_workspace_size(const w4a16_kv4_cache* cache, int64_t T, 
  * (nothing where it is new, t >= kv_lens[b] - queries), plus the sum over the sequence's queries and the kv head's
  * query heads that see it of exp(scale q . k - lse). q .. sinks as in w4a16_kv4_attention_sinks, lse [T, heads] what that
  * call gave (a query of -inf gives nothing). before and after, fp32: entry (sequence, kv head, token) at two
- * strides, tokens contiguous, `capacity` of them; they may be the same. What lies behind a sequence's length is
- * not written; a sequence longer than `capacity` is left out (index flag). workspace: 256-byte aligned, any contents;
+ * strides, tokens contiguous, `capacity` of them; the two are the same, or share no memory (else refused, as are
+ * entries of `after` that do). What lies behind a sequence's length is not written; a sequence longer than `capacity` is left out (index flag). workspace: 256-byte aligned, any contents;
  * calls that may run at the same time need one each.
  */
 int w4a16_kv4_attention_weights(const void* q, int dtype, int64_t T, int heads, int64_t q_token_stride,
@@ -571,7 +571,7 @@ int w4a16_kv4_release(const w4a16_kv4_tables* in, const w4a16_kv4_tables* out, c
  * positions; NaN: below every number), in their order, moved into fresh pages (the lowest free ids, in the order
  * of the requests; a page that other rows share stays as it is); the row's other pages are given back and kv_lens[rows[i]]
  * = keep. weights, fp32: entry (layer, row, head, token) at the three strides, `capacity` tokens contiguous; the
- * kept tokens' weights go to kept [.., keep), which may be weights. ok[i] = 1; 0, with the row unchanged, where
+ * kept tokens' weights go to kept [.., keep), which is weights or shares no memory with it. ok[i] = 1; 0, with the row unchanged, where
  * the free pages do not reach that far down the list, where the row was named before, or (index flag) where it is out of
  * range or longer than `capacity`. n is at most 2^20, and n rows' pages (of `keep` tokens each) at most 2^31 - 1. Writes
  * the tables `out` (which may be `in`). scratch: w4a16_kv4_evict_scratch_ints ints. */

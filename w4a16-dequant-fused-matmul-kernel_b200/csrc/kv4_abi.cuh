@@ -12,15 +12,78 @@ namespace w4a16 {
 namespace kv4 {
 namespace {
 
-// The checks every entry point makes of a cache.
-int check_cache(const w4a16_kv4_cache* c, DeviceState** dev) {
+// The checks every entry point makes of a cache; those that need no device, and all.
+int check_cache(const w4a16_kv4_cache* c) {
   if (c == nullptr || c->layers < 1 || c->layers > 0x7fffffffLL || c->pages < 1 || c->pages > 0x7fffffffLL || c->kv_heads < 1 ||
       c->kv_heads > 65535 || (c->head_dim != 64 && c->head_dim != 128) || c->page_size < BLK ||
       c->page_size % BLK != 0 || c->page_size > 4096 || c->pages * c->page_size > 0xffffffffLL || (c->group_size != 64 && c->group_size != c->head_dim))
     return W4A16_ERR_INVALID;
   if (c->pool == nullptr) return W4A16_ERR_INVALID;
   if (!aligned16(c->pool)) return W4A16_ERR_ALIGNMENT;
-  return current_device_state(dev);
+  return W4A16_OK;
+}
+int check_cache(const w4a16_kv4_cache* c, DeviceState** dev) {
+  const int st = check_cache(c);
+  return st != W4A16_OK ? st : current_device_state(dev);
+}
+
+// Collected weights as they lie in memory: up to three axes of n entries at a stride, each entry `tokens` floats.
+struct WeightsAxis {
+  long long n, stride;
+};
+struct WeightsMemory {
+  const float* at;
+  WeightsAxis given[3], axes[3];   // those of more than one entry: as they came, and from the largest stride down
+  int count = 0;
+  long long tokens;
+  __int128 low = 0, high;    // floats from `at`: the first, and the one behind the last
+
+  WeightsMemory(const float* p, std::initializer_list<WeightsAxis> all, long long tokens_) : at(p), tokens(tokens_), high(tokens_) {
+    for (const WeightsAxis& a : all) {
+      if (a.n <= 0) tokens = 0;          // nothing at all
+      if (a.n <= 1) continue;
+      given[count] = a;
+      int i = count++;
+      for (; i > 0 && magnitude(axes[i - 1].stride) < magnitude(a.stride); --i) axes[i] = axes[i - 1];
+      axes[i] = a;
+      (a.stride < 0 ? low : high) += static_cast<__int128>(a.n - 1) * a.stride;
+    }
+  }
+  static __int128 magnitude(__int128 x) { return x < 0 ? -x : x; }
+  // Whether each entry of an axis holds all of the axes below it without reaching the next.
+  bool nested() const {
+    __int128 extent = tokens;
+    for (int i = count - 1; i >= 0; --i) {
+      if (magnitude(axes[i].stride) < extent) return false;
+      extent += magnitude(axes[i].stride) * (axes[i].n - 1);
+    }
+    return true;
+  }
+  // Whether entries that lie `by` floats apart, and at any two places of the axes from i on, share some (nested ones).
+  bool meets(int i, __int128 by) const {
+    if (i == count) return magnitude(by) < tokens;
+    const __int128 s = magnitude(axes[i].stride);
+    const __int128 k = by / s - (by % s < 0);             // rounded down: only this one and the next come near enough
+    for (int next = 0; next < 2; ++next)
+      if (magnitude(k + next) < axes[i].n && meets(i + 1, by - (k + next) * s)) return true;
+    return false;
+  }
+};
+
+// Whether `to` can be written while `from` is read: no two entries of `to` share memory, and none of them
+// with another's of `from` (they are the same, or apart).
+bool can_write(const WeightsMemory& from, const WeightsMemory& to) {
+  if (to.tokens == 0) return true;
+  if (!to.nested()) return false;
+  bool same = from.count == to.count, alike = same;
+  for (int i = 0; i < std::min(from.count, to.count); ++i) {
+    same = same && from.given[i].stride == to.given[i].stride;
+    alike = alike && from.axes[i].n == to.axes[i].n && from.axes[i].stride == to.axes[i].stride;
+  }
+  const __int128 bytes = static_cast<__int128>(reinterpret_cast<uintptr_t>(to.at)) - static_cast<__int128>(reinterpret_cast<uintptr_t>(from.at));
+  if (bytes == 0) return same;
+  if (bytes + 4 * to.low >= 4 * from.high || bytes + 4 * to.high <= 4 * from.low) return true;
+  return alike && bytes % 4 == 0 && !to.meets(0, bytes / 4);
 }
 
 CacheView view_of(const w4a16_kv4_cache& c, int64_t layer) {
@@ -609,8 +672,12 @@ int w4a16_kv4_attention_weights(const void* q, int dtype, int64_t T, int heads, 
                                 int64_t after_head_stride, int64_t capacity, void* workspace, int64_t workspace_bytes,
                                 void* stream) {
   DeviceState* dev = nullptr;
-  const int st = kv4::check_cache(cache, &dev);
+  int st = kv4::check_cache(cache);
   if (st != W4A16_OK) return st;
+  if (!kv4::can_write({before, {{seqs, before_seq_stride}, {cache->kv_heads, before_head_stride}}, capacity},
+                      {after, {{seqs, after_seq_stride}, {cache->kv_heads, after_head_stride}}, capacity}))
+    return W4A16_ERR_INVALID;
+  if ((st = current_device_state(&dev)) != W4A16_OK) return st;
   int64_t need = 0;
   if (seqs > 0 && cu_q == nullptr) max_q = T / seqs;
   if (w4a16_kv4_attention_weights_workspace_size(cache, T, heads, seqs, max_q, capacity, &need) != W4A16_OK ||
@@ -622,10 +689,6 @@ int w4a16_kv4_attention_weights(const void* q, int dtype, int64_t T, int heads, 
   if (cu_q == nullptr && T % seqs != 0) return W4A16_ERR_INVALID;
   if (kv_lens == nullptr || (T > 0 && (q == nullptr || lse == nullptr)) || (table_width > 0 && block_table == nullptr) ||
       (capacity > 0 && (before == nullptr || after == nullptr)))
-    return W4A16_ERR_INVALID;
-  // in place the two have one layout
-  if (before == after && ((seqs > 1 && before_seq_stride != after_seq_stride) ||
-                          (cache->kv_heads > 1 && before_head_stride != after_head_stride)))
     return W4A16_ERR_INVALID;
   if (!aligned16(q) || q_token_stride % 8 != 0 || q_head_stride % 8 != 0) return W4A16_ERR_ALIGNMENT;
   if (workspace == nullptr || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
@@ -760,9 +823,14 @@ int w4a16_kv4_evict(const w4a16_kv4_cache* cache, const w4a16_kv4_tables* in, co
                     const int32_t* rows, int64_t n, int keep, int sinks, int recent, int32_t* ok, int32_t* scratch,
                     void* stream) {
   DeviceState* dev = nullptr;
-  int st = kv4::check_cache(cache, &dev);
+  int st = kv4::check_cache(cache);
   if (st != W4A16_OK) return st;
   if ((st = kv4::check_tables(in)) != W4A16_OK || (st = kv4::check_tables(out)) != W4A16_OK) return st;
+  if (n > 0 && !kv4::can_write(
+          {weights, {{cache->layers, w_layer_stride}, {in->rows, w_row_stride}, {cache->kv_heads, w_head_stride}}, capacity},
+          {kept, {{cache->layers, k_layer_stride}, {in->rows, k_row_stride}, {cache->kv_heads, k_head_stride}}, capacity}))
+    return W4A16_ERR_INVALID;
+  if ((st = current_device_state(&dev)) != W4A16_OK) return st;
   int64_t ints = 0;
   if ((st = w4a16_kv4_evict_scratch_ints(in, n, keep, &ints)) != W4A16_OK) return st;
   if (!kv4::same_shape(*in, *out) || in->pages != cache->pages || in->page_size != cache->page_size || sinks < 0 ||
@@ -771,10 +839,6 @@ int w4a16_kv4_evict(const w4a16_kv4_cache* cache, const w4a16_kv4_tables* in, co
   const long long items = cache->layers * n * cache->kv_heads;
   if (n > 0 && (weights == nullptr || kept == nullptr || rows == nullptr || ok == nullptr || scratch == nullptr ||
                 cache->layers > 0x7fffffffLL / 8 / (n * cache->kv_heads)))
-    return W4A16_ERR_INVALID;
-  // in place the two have one layout
-  if (kept == weights && ((cache->layers > 1 && w_layer_stride != k_layer_stride) || (in->rows > 1 && w_row_stride != k_row_stride) ||
-                          (cache->kv_heads > 1 && w_head_stride != k_head_stride)))
     return W4A16_ERR_INVALID;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   kv4::EvictParams p = {};

@@ -18,6 +18,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 
 #include "common.cuh"

@@ -388,9 +388,37 @@ def _check_weights(name: str, w: Tensor, shape: tuple, device_index: int) -> Non
         f"{name} must be fp32 {[*shape, 'tokens']} on the cache's device, the last axis contiguous")
 
 
-def _check_written(w: Tensor) -> None:
-    assert w.numel() == 0 or all(s > 0 or m == 1 for m, s in zip(w.shape, w.stride())), (
-        "weights that are written must not share memory between their entries")
+def _axes(w: Tensor) -> list[tuple[int, int]]:
+    """(stride, entries) of all axes but the last, the largest stride first; those of one entry left out."""
+    return sorted(((s, m) for m, s in zip(w.shape[:-1], w.stride()) if m != 1), reverse=True)
+
+
+def _span(w: Tensor) -> int:
+    """Floats from a non-empty tensor's first to behind its last."""
+    return 1 + sum((m - 1) * s for m, s in zip(w.shape, w.stride()))
+
+
+def _meet(axes: list[tuple[int, int]], tokens: int, by: int) -> bool:
+    """Whether entries of nested axes, of two tensors that lie ``by`` floats apart, share some."""
+    if not axes:
+        return abs(by) < tokens
+    (s, m), rest = axes[0], axes[1:]
+    return any(abs(k) < m and _meet(rest, tokens, by - k * s) for k in (by // s, by // s + 1))
+
+
+def _check_written(w: Tensor, read: Tensor) -> None:
+    if w.numel() == 0:
+        return
+    axes, extent = _axes(w), w.shape[-1]
+    for s, m in reversed(axes):
+        assert s >= extent, "weights that are written must not share memory between their entries"
+        extent += s * (m - 1)
+    by = w.data_ptr() - read.data_ptr()
+    if by >= 4 * _span(read) or by <= -4 * _span(w):
+        return
+    same = all(a == b or m == 1 for a, b, m in zip(w.stride(), read.stride(), w.shape))
+    assert same if by == 0 else axes == _axes(read) and by % 4 == 0 and not _meet(axes, w.shape[-1], by // 4), (
+        "weights that are written must be those that are read, or share no memory with them")
 
 
 def kv4_attention_weights(q: Tensor, cache: KV4Cache, layer: int, block_table: Tensor, kv_lens: Tensor, lse: Tensor,
@@ -405,8 +433,8 @@ def kv4_attention_weights(q: Tensor, cache: KV4Cache, layer: int, block_table: T
         weights: fp32 [sequences, kv_heads, tokens], what earlier calls collected; any strides but the last. Tokens that are
             new in this call (the queries' own) start from nothing, whatever it holds, so neither new rows nor
             places of rejected drafts have to be cleared.
-        out: where the sums go, all tokens of every sequence; default: ``weights``, where only those that a query sees
-            change. What lies behind a sequence's length is not written.
+        out: where the sums go, all tokens of every sequence; shares no memory with ``weights``, or is it. Default:
+            ``weights``, where only those that a query sees change. What lies behind a sequence's length is not written.
 
     Returns ``out``, or ``weights``. A sequence longer than the weights is left out, with the error of an index out of
     range. fp32 throughout; two calls on the same inputs give the same bits.
@@ -448,10 +476,14 @@ def kv4_attention_weights(q: Tensor, cache: KV4Cache, layer: int, block_table: T
     qt, qs, _ = q.stride()
     ws0, ws1, _ = weights.stride()
     as0, as1, _ = after.stride()
-    _on(d, _lib.lib().w4a16_kv4_attention_weights, q.data_ptr(), _CODES[q.dtype], T, H, qt, qs, cache._ref, layer,
-        block_table.data_ptr(), width, kv_lens.data_ptr(), _ptr(cu_q), B, max_q, q.shape[2] ** -0.5 if scale is None else scale,
-        min(window, _INT_MAX), min(sinks, _INT_MAX), lse.data_ptr(), weights.data_ptr(), ws0, ws1, after.data_ptr(), as0, as1,
-        wh[2], ws.data_ptr(), nbytes)
+    try:
+        _on(d, _lib.lib().w4a16_kv4_attention_weights, q.data_ptr(), _CODES[q.dtype], T, H, qt, qs, cache._ref, layer,
+            block_table.data_ptr(), width, kv_lens.data_ptr(), _ptr(cu_q), B, max_q, q.shape[2] ** -0.5 if scale is None else scale,
+            min(window, _INT_MAX), min(sinks, _INT_MAX), lse.data_ptr(), weights.data_ptr(), ws0, ws1, after.data_ptr(), as0, as1,
+            wh[2], ws.data_ptr(), nbytes)
+    except _lib.W4A16Error:
+        _check_written(after, weights)         # (the common case leaves it to the library to find an overlap)
+        raise
     return after
 
 
@@ -475,7 +507,7 @@ def _check_collecting(q: Tensor, cache: KV4Cache, layer: int, block_table: Tenso
     if out is not None:
         _check_weights("out", out, shape, d)
         assert out.shape == weights.shape, "out must have the shape of weights"
-    _check_written(weights if out is None else out)
+    _check_written(weights if out is None else out, weights)
 
 
 def _ints(name: str, t: Tensor, n: int, device_index: int) -> None:
@@ -572,7 +604,8 @@ def kv4_evict(cache: KV4Cache, pages: KV4Pages, weights: Tensor, rows: Tensor, k
             strides but the last.
         rows: int32 [n], the rows to look at; one of at most ``keep`` tokens stays as it is.
         out: where the new tables go; default: new ones. May be ``pages``.
-        out_weights: where the kept tokens' weights go ([..., :keep] of the rows evicted from); default: ``weights``.
+        out_weights: where the kept tokens' weights go ([..., :keep] of the rows evicted from); default: ``weights``. Another
+            tensor shares no memory with it.
 
     What is kept moves into fresh pages (the lowest free ids, in the order of the requests), so pages that other rows
     share stay as they are, and the row's old ones are given back: a row needs ``ceil(keep / page_size)`` free pages
@@ -595,7 +628,7 @@ def kv4_evict(cache: KV4Cache, pages: KV4Pages, weights: Tensor, rows: Tensor, k
         if out_weights is not None:
             _check_weights("out_weights", out_weights, shape[:3], d)
             assert out_weights.shape == weights.shape, "out_weights must have the shape of weights"
-        _check_written(kept)
+        _check_written(kept, weights)
     assert sinks >= 0 and recent >= 0 and 1 <= keep <= _INT_MAX and sinks + recent <= keep, (
         f"keep={keep} must be positive, and hold sinks={sinks} and recent={recent}")
     _, R, W = pages._shape
@@ -603,6 +636,10 @@ def kv4_evict(cache: KV4Cache, pages: KV4Pages, weights: Tensor, rows: Tensor, k
     assert n * need <= _INT_MAX, f"{n} rows of {need} pages are more than one call can ask for"
     out, buf, at = _tables_out(pages, out, n * (4 + need + W) + 1 + R)
     ws, ks = weights.stride(), kept.stride()
-    _on(d, _lib.lib().w4a16_kv4_evict, cache._ref, pages._ref, out._ref, weights.data_ptr(), ws[0], ws[1], ws[2],
-        kept.data_ptr(), ks[0], ks[1], ks[2], weights.shape[3], rows.data_ptr(), n, keep, sinks, recent, at, at and at + 4 * n)
+    try:
+        _on(d, _lib.lib().w4a16_kv4_evict, cache._ref, pages._ref, out._ref, weights.data_ptr(), ws[0], ws[1], ws[2],
+            kept.data_ptr(), ks[0], ks[1], ks[2], weights.shape[3], rows.data_ptr(), n, keep, sinks, recent, at, at and at + 4 * n)
+    except _lib.W4A16Error:
+        _check_written(kept, weights)          # (the common case leaves it to the library to find an overlap)
+        raise
     return out, buf.narrow(0, (at - buf.data_ptr()) // 4, n)
