@@ -526,10 +526,11 @@ int w4a16_kv4_attention_workspace_size(const w4a16_kv4_cache* cache, int64_t T, 
  * The attention weight that cached tokens collect: after[b, kv head, t] = what the token had, before[b, kv head, t]
  * (nothing where it is new, t >= kv_lens[b] - queries), plus the sum over the sequence's queries and the kv head's
  * query heads that see it of exp(scale q . k - lse). q .. sinks as in w4a16_kv4_attention_sinks, lse [T, heads] what that
- * call gave (a query of -inf gives nothing). before and after, fp32: entry (sequence, kv head, token) at two
- * strides, tokens contiguous, `capacity` of them; the two are the same, or share no memory (else refused, as are
- * entries of `after` that do). What lies behind a sequence's length is not written; a sequence longer than `capacity` is left out (index flag). workspace: 256-byte aligned, any contents;
- * calls that may run at the same time need one each.
+ * call gave (a query of -inf gives nothing; every other one counts, a draft's too that is rejected later). before and
+ * after, fp32: entry (sequence, kv head, token) at two strides, tokens contiguous, `capacity` of them; the two are the
+ * same, or share no memory (else refused, as are entries of `after` that do). What lies behind a sequence's length is not
+ * written; a sequence longer than `capacity` is left out (index flag). workspace: 256-byte aligned, any contents; calls
+ * that may run at the same time need one each.
  */
 int w4a16_kv4_attention_weights(const void* q, int dtype, int64_t T, int heads, int64_t q_token_stride,
                                 int64_t q_head_stride, const w4a16_kv4_cache* cache, int64_t layer,

@@ -65,7 +65,9 @@ class W4A16Attention(nn.Module):
         """``x`` [T, hidden] fp16, the new tokens of all rows of ``pages`` one after another; ``pages.kv_lens``
         counts them already. ``slots`` (``pages.slots``), ``positions``, ``cos_sin`` and ``sections`` as in
         :func:`qk_norm_rope_append`, ``cu_q`` and ``max_q`` as in :func:`kv4_attention`. ``weights`` [layers, rows,
-        kv_heads, tokens] fp32, what :func:`kv4_evict` goes by: this call's are added to those of ``layer``."""
+        kv_heads, tokens] fp32, what :func:`kv4_evict` goes by: this call's are added to those of ``layer``, from
+        all new tokens, drafts that :func:`verify_drafts` will reject among them (:func:`kv4_attention_weights` says how to
+        collect from those that stand alone)."""
         assert x.dim() == 2, f"x must be [tokens, hidden], got {tuple(x.shape)}"
         H, KV = self.heads, self.kv_heads
         qkv = self.qkv(x).view(x.shape[0], H + 2 * KV, self.head_dim)

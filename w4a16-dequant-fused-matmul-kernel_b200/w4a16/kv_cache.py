@@ -436,6 +436,12 @@ def kv4_attention_weights(q: Tensor, cache: KV4Cache, layer: int, block_table: T
         out: where the sums go, all tokens of every sequence; shares no memory with ``weights``, or is it. Default:
             ``weights``, where only those that a query sees change. What lies behind a sequence's length is not written.
 
+    Every query counts, those of drafts that are rejected later too: their own places start from nothing again, but what
+    they gave to older tokens stays. To collect from the drafts that stand alone, call this behind
+    :func:`w4a16.verify_drafts` with the lengths that the attention had (lower them afterwards), and with ``lse`` -inf
+    in the rows of the rejected drafts. With K drafts to a sequence: ``gone = torch.arange(K + 1, device=lse.device) >
+    accepted[:, None]; lse.unflatten(0, (-1, K + 1)).masked_fill_(gone[..., None], -math.inf)``.
+
     Returns ``out``, or ``weights``. A sequence longer than the weights is left out, with the error of an index out of
     range. fp32 throughout; two calls on the same inputs give the same bits.
     """
