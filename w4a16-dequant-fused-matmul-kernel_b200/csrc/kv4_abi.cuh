@@ -844,7 +844,6 @@ int w4a16_kv4_evict(const w4a16_kv4_cache* cache, const w4a16_kv4_tables* in, co
   kv4::EvictParams p = {};
   p.cache = kv4::view_of(*cache, 0);
   p.layer_bytes = cache->pages * cache->kv_heads * p.cache.page_bytes;
-  p.layers = static_cast<int>(cache->layers);
   p.in = kv4::tables_of(*in);
   p.out = kv4::tables_of(*out);
   p.weights = weights; p.w_sl = w_layer_stride; p.w_sr = w_row_stride; p.w_sh = w_head_stride;

@@ -31,7 +31,6 @@ constexpr int EVICT_KEYS = 4096;             // weights of a head that are kept 
 struct EvictParams {
   CacheView cache;           // layer 0
   long long layer_bytes;
-  int layers, head_dim, groups;
   Tables in, out;            // out may be in
   const float* weights;      // entry (layer, row, head, token)
   float* kept;               // where the kept tokens' weights go: may be weights

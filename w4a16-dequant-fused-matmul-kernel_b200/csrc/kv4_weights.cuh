@@ -6,7 +6,9 @@
 // The scores are those of the attention kernels, from the cache's codes: q . k = s_k (q . c) + b_k sum(q) per group of
 // channels, codes masked out of their words as fp16 subnormals, queries scaled by a power of two of their own row
 // (kv4_decode.cuh has the arithmetic). Tokens are the M side of mma.m16n8k16, eight query rows its N side, so
-// the sum over rows stays in a lane but for its last two steps. Nothing is rounded to 16 bits.
+// the sum over rows stays in a lane but for its last two steps. Scores, exponentials and sums are fp32. The scaled
+// queries are fp16 operands: channels down to 2^-24 of their row's largest are exact (odd nibbles hold 1/16 of
+// theirs), smaller ones within 2^-35 of it, less than the fp32 sum rounds off.
 //
 // A launch before (kv4_weights_prep_kernel) writes the queries in the order of the second operand's fragments, with
 // what a row's scores need (factor, sums, -lse log2(e)) beside them, and the prefix sums of the sequences' chunks:
@@ -15,10 +17,12 @@
 // stage. Each sum has one owner and a fixed order, so results do not depend on timing. Sequences of more than 64 rows
 // a kv head go to the tensor-memory kernel further down.
 //
-// Memory-bound by design (a token's keys are half of what the attention reads, and four bytes in and out); what it
-// takes is the issue of the codes' masks: 64 sequences of up to 8000 tokens, 64 heads of 128 channels on 8 kv heads
-// (172 MB) 50 us, 3.5 TB/s, issue slots 56%, ALU pipe 49%. Three blocks an SM, of 80 registers and with spills, took
-// 70 us; divisions by the group's heads 2.5 of now 50. One token over 777: 6.5 us, both launches.
+// Memory-bound by design (a token's keys are half of what the attention reads, and four bytes in and out), but no
+// unit is full: 64 sequences of up to 8000 tokens, 64 heads of 128 channels on 8 kv heads (172 MB) 49 us, 3.5 TB/s,
+// issue slots 56%, ALU pipe 49% (the codes' masks), 23% of an SM's warps there. What is left is latency: a warp
+// waits 1.6 cycles an instruction for its own results and 1.4 for memory, with one chunk in flight. Three blocks an SM, of
+// 80 registers and with spills, took 70 us; divisions by the group's heads 2.5 of now 49. One token over 777: 6.5 us, both
+// launches.
 #pragma once
 
 #include "kv4_prefill.cuh"
@@ -31,8 +35,9 @@ constexpr int WT_BLOCKS = 4, WT_TOKENS = WT_BLOCKS * BLK;       // blocks and to
 constexpr int WT_PREP = 256;
 
 // Of a tile of eight rows: fragment words [D / 32][32 lanes][4], then eight rows' (factor, sum of group 0, sum of
-// the last group, -lse log2(e)), then whether a row has a log-sum-exp of -inf. (Rows behind the last are 0, 0, 0, -inf:
-// they give nothing, but NaN where the others do.)
+// the last group, -lse log2(e)), then whether a row has a log-sum-exp of -inf. (Rows behind the last have channels and
+// sums of 0 and -inf for the last: they give nothing to a token with a finite pair. One whose pair is not is NaN
+// to the rows that see it.)
 __host__ __device__ constexpr int wt_tile_words(int D) { return D / 32 * 128 + 8 * 4 + 4; }
 
 struct WeightsParams {
@@ -646,7 +651,9 @@ __device__ __forceinline__ void tmem_ld_two(uint32_t at0, uint32_t at1, uint32_t
 // taken per step and then in pairs of fp32 numbers (rounded-off parts kept): thousands of steps would lose bits.
 //
 // Keys are codes less 8 (exact in fp16), so that a score's two terms are as small as they can be; eight rows share a
-// power of two where they lie within 2^13 of one another, which leaves two packed multiply-adds a score and group.
+// power of two where they lie within 2^13 of one another, which leaves two packed multiply-adds a score and group. A
+// row that far below its neighbours keeps its channels as fp16 down to 2^-15 of its own largest, and smaller ones
+// within 2^-26 of it: half of what fp32 rounds off a product with the largest.
 //
 // The exponentials are 16 a cycle and SM, 2 D operations a score about twice as fast at the tensor cores' rate. Two
 // prompts of 4001 and 2763 tokens over 6000 and 4145, 32 heads of 128 channels in two groups on 8 kv heads: 303 us,
