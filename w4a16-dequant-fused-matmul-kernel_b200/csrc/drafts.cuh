@@ -5,7 +5,7 @@
 // place a, is drawn by the last random number u from r = max(p_a - q_a, 0), or from p_a where no
 // draft is left (or r is nothing): the first v with r_0 + ... + r_v > u (r_0 + r_1 + ...).
 //
-// u q is exact in fp64, and so is p - q. The sums are fp64 of four values each (two, where rows lie at any
+// u q is exact in fp64, p - q within 2^-53 of itself. The sums are fp64 of four values each (two, where rows lie at any
 // place beside a draft) that are summed to 2^-45 of themselves; a thread adds V / 2048 such numbers at most, each addition
 // rounded to 2^-53. So a border between two tokens is off by less than 2^-45 + V 2^-64 of the whole, however the sum
 // is split (a fp32 sum of 10^5 probabilities would move it by more than many of them are wide). Values
@@ -20,7 +20,7 @@
 // 64 sequences of up to 7 drafts, 131072 values, fp32: 20.3 us, in which 48 MB are read (a sequence whose drafts all
 // stand reads one row): 2.4 TB/s, 36% of the copy rate. One sequence of 32000 values 7.4 us. 201 sequences of 50001
 // values, whose rows begin at any multiple of 4 bytes: 18.5 us for looked-up drafts, 26 us beside a draft. No
-// unit is full (issue 31%): it is the latency of a chain of four dependent reads, two joins in the cluster and
+// unit is full (issue 30%): it is the latency of a chain of four dependent reads, two joins in the cluster and
 // the second look.
 #pragma once
 

@@ -21,7 +21,7 @@
 // unit is full: 64 sequences of up to 8000 tokens, 64 heads of 128 channels on 8 kv heads (172 MB) 49 us, 3.5 TB/s,
 // issue slots 56%, ALU pipe 49% (the codes' masks), 23% of an SM's warps there. What is left is latency: a warp
 // waits 1.6 cycles an instruction for its own results and 1.4 for memory, with one chunk in flight. Three blocks an SM, of
-// 80 registers and with spills, took 70 us; divisions by the group's heads 2.5 of now 49. One token over 777: 6.5 us, both
+// 80 registers and with spills, took 70 us; divisions by the group's heads 2.5 of now 49. One token over 777: 7 us, both
 // launches.
 #pragma once
 

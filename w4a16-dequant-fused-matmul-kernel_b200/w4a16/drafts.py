@@ -59,8 +59,8 @@ def verify_drafts(target: Tensor, draft: Tensor | None, tokens: Tensor, uniforms
     Draft i of a sequence is accepted while ``uniforms[i] * q < p``: p and q are what the target and the draft
     model give it at its place. The token behind the a accepted ones is drawn by the last of ``uniforms`` from
     max(target[a] - draft[a], 0), or from target[a] itself where all were accepted (or nothing is left): the first
-    whose running sum exceeds that number times the whole. Differences are exact, and the sums within 2^-45 +
-    V 2^-64 of the whole, however large the batch.
+    whose running sum exceeds that number times the whole. The sums are within 2^-45 + V 2^-64 of the
+    whole, however large the batch.
 
     Args:
         target: [B, K + 1, V] probabilities (fp32, fp16 or bf16; they need not add up to 1, any strides but the
