@@ -103,3 +103,11 @@ def test_a_call_whose_result_overlaps_what_it_reads_is_refused():
     for kw in (dict(out_weights=buf[..., 1:33]), dict(out_weights=buf.transpose(1, 2)[..., :32])):
         with pytest.raises(AssertionError, match="share"):
             kv4_evict(Cache(), Pages(2, 4), buf[..., :32], torch.zeros(1, dtype=torch.int32), 5, **kw)
+
+
+def test_capacities_below_zero_are_refused():
+    lib = _lib.lib()
+    for strides, apart in (((0, 0, 0), 256), ((400, 400, 0), 256), ((400, 0, 0), 0), ((1, 1, 1), 4)):
+        assert lib.w4a16_kv4_evict(cache(layers=2), tables(), tables(), 4096, *strides, 4096 + apart, *strides, -5, 256, 1, 33, 0, 0, 256, 256, None) != 0
+        assert lib.w4a16_kv4_attention_weights(256, 0, 2, 8, 1024, 128, cache(), 0, 256, 1, 256, None, 2, 1, 1.0, 0, 0, 256, 4096, *strides[1:],
+                                               4096 + apart, *strides[1:], -5, 256, 1 << 20, None) != 0

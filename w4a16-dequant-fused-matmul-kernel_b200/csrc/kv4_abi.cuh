@@ -73,7 +73,7 @@ struct WeightsMemory {
 // Whether `to` can be written while `from` is read: no two entries of `to` share memory, and none of them
 // with another's of `from` (they are the same, or apart).
 bool can_write(const WeightsMemory& from, const WeightsMemory& to) {
-  if (to.tokens == 0) return true;
+  if (to.tokens <= 0) return true;       // (fewer than none are refused elsewhere)
   if (!to.nested()) return false;
   bool same = from.count == to.count, alike = same;
   for (int i = 0; i < std::min(from.count, to.count); ++i) {
